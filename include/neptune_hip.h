@@ -20,8 +20,9 @@
  *   - error conventions (RuntimeError / NotImplementedError,
  *     src/neptune_mlir/translators/common.py:187-197,217-224)
  *     -> neptune_status + neptune_last_error
- * Split-K decode, fp8 KV and the selective scan have no counterpart in the
- * reference; their contracts are stated next to each declaration.
+ * Split-K decode, fp8 KV, the paged cache's append and attention, the norm and
+ * rotation of queries and keys and the selective scan have no counterpart in
+ * the reference; their contracts are stated next to each declaration.
  */
 #ifndef NEPTUNE_HIP_H
 #define NEPTUNE_HIP_H
@@ -158,6 +159,59 @@ typedef struct neptune_scan_desc {
   int32_t delta_softplus;  /* 1: apply softplus (threshold 20) */
 } neptune_scan_desc;
 
+/* Norm and position rotation of queries and keys. q, qo [batch, heads_q, seq,
+ * head_dim], k, ko [batch, heads_kv, seq, head_dim] in dtype, head_dim
+ * contiguous, (batch, head, seq) strides in elements (zero: contiguous). Per
+ * head row x, at position p:
+ *   y = x * w / sqrt(mean(x^2) + eps)          (where a weight is given)
+ *   rotation of the first rot_dim elements by cos, sin [table_len, rot_dim / 2]:
+ *   (y_i, y_j) <- (y_i c - y_j s, y_j c + y_i s), c, s = cos, sin[p][pair],
+ *   pair i being (i, i + rot_dim / 2), or (2i, 2i + 1) with interleaved = 1.
+ * fp32 throughout, rounded once to dtype. */
+typedef struct neptune_rope_desc {
+  int64_t batch, heads_q, heads_kv, seq, head_dim;
+  int64_t rot_dim;   /* a multiple of 8, at most head_dim                    */
+  int64_t table_len; /* rows of cos and sin                                  */
+  int64_t q_stride[3], k_stride[3], qo_stride[3], ko_stride[3];
+  int32_t dtype; /* F32, F16 or BF16                                         */
+  int32_t interleaved;
+  float eps;
+  int32_t reserved;
+} neptune_rope_desc;
+
+/* New tokens of a ragged batch on their way into a paged cache. Row r of q, k, v
+ * ([tokens, heads, head_dim], (token, head) strides in elements, zero:
+ * contiguous) belongs to the sequence b with cu_seqlens[b] <= r <
+ * cu_seqlens[b + 1]; seq_lens[b] counts the sequence's tokens with the new ones,
+ * so the row's place is seq_lens[b] - (cu_seqlens[b + 1] - r). Pools, pages and
+ * block tables are neptune_paged_kv_desc's; any page size is taken here. */
+typedef struct neptune_append_desc {
+  int64_t tokens, batch, heads_q, heads_kv, head_dim; /* heads_q 0: no queries */
+  int64_t rot_dim; /* 0: no rotation; else as in neptune_rope_desc             */
+  int64_t table_len;
+  int64_t q_stride[2], k_stride[2], v_stride[2], qo_stride[2];
+  int32_t dtype;    /* F16 or BF16: q, k, v and qo                             */
+  int32_t kv_dtype; /* the pools': dtype, or FP8_E4M3                          */
+  int32_t interleaved;
+  float eps;
+} neptune_append_desc;
+
+/* Attention of a ragged batch of new tokens over a paged cache that already
+ * holds them (rows, sequences and pages as in neptune_append_desc). q, o
+ * [tokens, heads_q, head_dim] with (token, head) strides in elements (zero:
+ * contiguous). A row sees its sequence's tokens up to its own place; one whose
+ * place is negative sees none: O = 0, lse = -inf. Rows of no sequence (behind
+ * cu_seqlens[batch]) are left as they were. */
+typedef struct neptune_attn_paged_desc {
+  int64_t tokens, batch, heads_q, heads_kv, head_dim;
+  int64_t seq_kv; /* the longest sequence; longer ones are cut to it           */
+  int64_t q_stride[2], o_stride[2];
+  int32_t dtype;    /* F16 or BF16: q and o                                    */
+  int32_t kv_dtype; /* the pools': dtype, or FP8_E4M3 (dtype BF16)             */
+  float scale_log2; /* 0 => log2(e)/sqrt(head_dim)                             */
+  int32_t reserved;
+} neptune_attn_paged_desc;
+
 /* ---- discovery and errors ------------------------------------------- */
 
 NEPTUNE_API neptune_status neptune_hip_get_backend_info(neptune_backend_info *info);
@@ -266,6 +320,58 @@ NEPTUNE_API neptune_status neptune_decode_paged_fp8(const neptune_decode_desc *d
                                         const int32_t *seq_lens, void *o,
                                         float *lse, void *workspace,
                                         size_t workspace_bytes, void *stream);
+
+/* ---- queries, keys and the paged cache around a layer's attention ------ */
+
+/* qo, ko <- norm and rotation of q, k (neptune_rope_desc). No counterpart in the
+ * reference. q_weight and k_weight [head_dim] fp32 may be NULL (no norm of that
+ * operand); positions [batch, seq] int32. A position outside the tables is
+ * clamped into them (the row is then meaningless). qo may be q and ko k (same
+ * pointer and strides); an output that shares bytes with an input in any other
+ * way is NEPTUNE_ERR_INVALID_ARGUMENT. head_dim 32, 64 or 128; 16-byte aligned
+ * bases and strides of whole 16-byte units. */
+NEPTUNE_API neptune_status neptune_qk_norm_rope(const neptune_rope_desc *desc, const void *q,
+                                    const void *k, const float *q_weight,
+                                    const float *k_weight, const float *cos,
+                                    const float *sin, const int32_t *positions,
+                                    void *qo, void *ko, void *stream);
+
+/* k_pages, v_pages <- the new tokens' k (norm and rotation on the way) and v;
+ * qo <- q with norm and rotation (neptune_append_desc). No counterpart in the
+ * reference. cu_seqlens [batch + 1] may be NULL: one new token per sequence
+ * (tokens == batch). q, qo: NULL when heads_q is 0; qo may be q. q_weight,
+ * k_weight may be NULL (no norm), cos and sin NULL when rot_dim is 0. Into E4M3
+ * pools a value goes as code = RNE-saturate(x / scale) under its page's and
+ * head's k_scales, v_scales [num_pages, heads_kv], which the caller has set (a
+ * page of scale 0 takes zero codes); NULL otherwise. A row is not stored when its
+ * place is negative or past its block table, or the table's entry lies outside
+ * [0, num_pages); rows behind cu_seqlens[batch] are neither stored nor written to
+ * qo. Two rows sent to one slot leave either. head_dim 64 or 128; 16-byte aligned
+ * bases and strides of whole 16-byte units. */
+NEPTUNE_API neptune_status neptune_kv_append_paged(
+    const neptune_append_desc *desc, const neptune_paged_kv_desc *pages, const void *k,
+    const void *v, const void *q, const float *q_weight, const float *k_weight,
+    const float *cos, const float *sin, const int32_t *block_table,
+    const int32_t *cu_seqlens, const int32_t *seq_lens, void *k_pages, void *v_pages,
+    const float *k_scales, const float *v_scales, void *qo, void *stream);
+
+/* Workspace of neptune_attn_paged in bytes (0: none is needed). */
+NEPTUNE_API neptune_status neptune_attn_paged_workspace_bytes(
+    const neptune_attn_paged_desc *desc, size_t *bytes);
+
+/* o, lse <- attention of the new tokens (neptune_attn_paged_desc). No counterpart
+ * in the reference. lse (nullable) [tokens, heads_q] fp32, natural log. k_scales,
+ * v_scales [num_pages, heads_kv] for E4M3 pools, NULL otherwise. cu_seqlens may be
+ * NULL: one new token per sequence (tokens == batch). The page size must be a
+ * multiple of 16. The lengths are read on the device when the work runs, and the
+ * cut of the keys follows them; the workspace needs no clearing, must be 16-byte
+ * aligned and is in use until the call's work is done. Table entries outside the
+ * pool are clamped into it. o must share no byte with q or the pools. */
+NEPTUNE_API neptune_status neptune_attn_paged(
+    const neptune_attn_paged_desc *desc, const neptune_paged_kv_desc *pages, const void *q,
+    const void *k_pages, const void *v_pages, const float *k_scales, const float *v_scales,
+    const int32_t *block_table, const int32_t *cu_seqlens, const int32_t *seq_lens, void *o,
+    float *lse, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---- selective scan ---------------------------------------------------- */
 

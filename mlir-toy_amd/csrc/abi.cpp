@@ -445,6 +445,358 @@ neptune_status neptune_kv_quantize_fp8(int64_t batch, int64_t heads_kv, int64_t 
   return hip_result(launch_kv_quantize(L, (hipStream_t)stream), "kv_quantize launch");
 }
 
+namespace {
+
+bool is_float(int32_t dtype, bool f32) {
+  return dtype == NEPTUNE_DTYPE_F16 || dtype == NEPTUNE_DTYPE_BF16 ||
+         (f32 && dtype == NEPTUNE_DTYPE_F32);
+}
+
+// Bytes from the first element to past the last of a [sizes.., row] tensor;
+// 0 where that passes 2^62
+size_t span(const int64_t *sizes, const int64_t *strides, int n, int64_t row, int64_t esize) {
+  int64_t at = row, step;
+  for (int i = 0; i < n; ++i)
+    if (__builtin_mul_overflow(sizes[i] - 1, strides[i], &step) ||
+        __builtin_add_overflow(at, step, &at))
+      return 0;
+  return at > ((int64_t)1 << 62) / esize ? 0 : (size_t)(at * esize);
+}
+
+// A strided tensor of an entry point: its rows' strides resolved (zero:
+// contiguous), its bytes
+struct Strided {
+  const char *name;
+  const void *p;
+  int64_t stride[3];
+  size_t bytes;
+};
+
+// [sizes[0], sizes[1], sizes[2], dim] with `n` strides in the descriptor's order
+neptune_status resolve(const char *fn, const char *name, const void *p, const int64_t *in,
+                       const int64_t *sizes, int n, int64_t dim, int64_t esize, Strided *t) {
+  t->name = name;
+  t->p = p;
+  if (!p) return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: %s must be non-NULL", fn, name);
+  bool zero = true;
+  for (int i = 0; i < n; ++i) zero = zero && in[i] == 0;
+  int64_t run = dim;
+  for (int i = n - 1; i >= 0; --i) {
+    t->stride[i] = zero ? run : in[i];
+    if (sizes[i] == 1) {  // no step is taken along it
+      t->stride[i] = 16 / esize;
+      continue;
+    }
+    if (zero && __builtin_mul_overflow(run, sizes[i], &run))
+      return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: %s is too large", fn, name);
+    if (t->stride[i] <= 0)
+      return fail(NEPTUNE_ERR_INVALID_ARGUMENT,
+                  "%s: strides must be all zero (contiguous) or all positive", fn);
+    if (t->stride[i] % (16 / esize))
+      return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: strides must be multiples of 16 bytes", fn);
+  }
+  if (!aligned16(p))
+    return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: %s must be 16-byte aligned", fn, name);
+  t->bytes = span(sizes, t->stride, n, dim, esize);
+  if (!t->bytes) return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: %s is too large", fn, name);
+  return NEPTUNE_OK;
+}
+
+// out must share no byte with in
+neptune_status apart(const char *fn, const Strided &out, const Strided &in) {
+  if (overlaps(out.p, out.bytes, in.p, in.bytes))
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: %s overlaps %s", fn, out.name, in.name);
+  return NEPTUNE_OK;
+}
+
+bool same_place(const Strided &a, const Strided &b, int n) {
+  bool same = a.p == b.p;
+  for (int i = 0; i < n; ++i) same = same && a.stride[i] == b.stride[i];
+  return same;
+}
+
+// what the rotation and norm take beside their tensors
+neptune_status rope_check(const char *fn, int64_t head_dim, int64_t rot_dim, int64_t table_len,
+                          const float *cos, const float *sin, const float *q_weight,
+                          const float *k_weight, int32_t interleaved, float eps) {
+  if (rot_dim < 0 || rot_dim > head_dim || (rot_dim > 0 && table_len <= 0))
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT,
+                "%s: rot_dim %lld (at most head_dim %lld) over tables of %lld rows", fn,
+                (long long)rot_dim, (long long)head_dim, (long long)table_len);
+  if (rot_dim > 0 && (!cos || !sin))
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: cos and sin must be non-NULL", fn);
+  if (interleaved != 0 && interleaved != 1)
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: interleaved must be 0 or 1", fn);
+  if (!(eps >= 0.0f) || !std::isfinite(eps))
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: eps must be finite and >= 0", fn);
+  if (!aligned16(cos) || !aligned16(sin) || !aligned16(q_weight) || !aligned16(k_weight))
+    return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: tables and weights must be 16-byte aligned", fn);
+  return NEPTUNE_OK;
+}
+
+// the pools of a ragged batch's entry points
+neptune_status pools_check(const char *fn, const neptune_paged_kv_desc *pk, const void *k_pages,
+                           const void *v_pages, const float *k_scales, const float *v_scales,
+                           const int32_t *block_table, const int32_t *cu_seqlens,
+                           const int32_t *seq_lens, int64_t tokens, int64_t batch,
+                           int64_t heads_kv, int64_t head_dim, int32_t kv_dtype, Strided pools[2]) {
+  if (!pk) return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: pages desc is NULL", fn);
+  if (!block_table || !seq_lens)
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: block_table and seq_lens must be non-NULL", fn);
+  if (pk->num_pages <= 0 || pk->page_size <= 0 || pk->max_pages <= 0)
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT,
+                "%s: num_pages, page_size and max_pages must be positive", fn);
+  if (!cu_seqlens && tokens != batch)
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT,
+                "%s: without cu_seqlens a sequence has one new token: tokens %lld, batch %lld", fn,
+                (long long)tokens, (long long)batch);
+  const bool fp8 = kv_dtype == NEPTUNE_DTYPE_FP8_E4M3;
+  if (fp8 && (!k_scales || !v_scales))
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: E4M3 pools need k_scales and v_scales", fn);
+  const int64_t sizes[3] = {pk->num_pages, heads_kv, pk->page_size};
+  const struct { const char *name; const void *p; const int64_t *stride; } in[2] = {
+      {"k_pages", k_pages, pk->k_stride}, {"v_pages", v_pages, pk->v_stride}};
+  for (int i = 0; i < 2; ++i) {
+    for (int j = 0; j < 3; ++j)
+      if (in[i].stride[j] <= 0)
+        return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: pool strides must be positive", fn);
+    neptune_status st = resolve(fn, in[i].name, in[i].p, in[i].stride, sizes, 3, head_dim,
+                                fp8 ? 1 : 2, &pools[i]);
+    if (st != NEPTUNE_OK) return st;
+  }
+  return NEPTUNE_OK;
+}
+
+// the checks of an attn_paged descriptor, and the launch it describes (no tensors)
+neptune_status attn_paged_resolve(const neptune_attn_paged_desc *d, PagedAttnLaunch *L) {
+  if (!d) return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "attn_paged: desc is NULL");
+  if (d->tokens <= 0 || d->batch <= 0 || d->heads_q <= 0 || d->heads_kv <= 0 || d->head_dim <= 0 ||
+      d->seq_kv <= 0)
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT,
+                "attn_paged: sizes must be positive (tokens=%lld batch=%lld heads_q=%lld "
+                "heads_kv=%lld head_dim=%lld seq_kv=%lld)",
+                (long long)d->tokens, (long long)d->batch, (long long)d->heads_q,
+                (long long)d->heads_kv, (long long)d->head_dim, (long long)d->seq_kv);
+  if (d->heads_q % d->heads_kv)
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "attn_paged: heads_q (%lld) %% heads_kv (%lld) != 0",
+                (long long)d->heads_q, (long long)d->heads_kv);
+  if (!is_float(d->dtype, false))
+    return fail(NEPTUNE_ERR_UNSUPPORTED, "attn_paged: dtype must be F16 or BF16");
+  if (d->kv_dtype != d->dtype && d->kv_dtype != NEPTUNE_DTYPE_FP8_E4M3)
+    return fail(NEPTUNE_ERR_UNSUPPORTED, "attn_paged: kv_dtype must be dtype or FP8_E4M3");
+  if (!(d->scale_log2 >= 0.0f) || !std::isfinite(d->scale_log2))
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "attn_paged: scale_log2 must be finite and >= 0");
+  *L = PagedAttnLaunch();
+  L->tokens = d->tokens; L->batch = d->batch; L->heads_q = d->heads_q; L->heads_kv = d->heads_kv;
+  L->head_dim = d->head_dim; L->seq_kv = d->seq_kv; L->dtype = d->dtype;
+  L->fp8 = d->kv_dtype == NEPTUNE_DTYPE_FP8_E4M3;
+  L->page_size = 16;
+  L->scale_log2 = d->scale_log2 != 0.0f
+                      ? d->scale_log2
+                      : (float)(1.4426950408889634 / std::sqrt((double)d->head_dim));
+  return NEPTUNE_OK;
+}
+
+}  // namespace
+
+neptune_status neptune_qk_norm_rope(const neptune_rope_desc *d, const void *q, const void *k,
+                                    const float *q_weight, const float *k_weight, const float *cos,
+                                    const float *sin, const int32_t *positions, void *qo, void *ko,
+                                    void *stream) {
+  const char *fn = "qk_norm_rope";
+  if (!d) return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: desc is NULL", fn);
+  if (d->batch <= 0 || d->heads_q <= 0 || d->heads_kv <= 0 || d->seq <= 0 || d->head_dim <= 0 ||
+      d->rot_dim <= 0)
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT,
+                "%s: sizes must be positive (batch=%lld heads_q=%lld heads_kv=%lld seq=%lld "
+                "head_dim=%lld rot_dim=%lld)",
+                fn, (long long)d->batch, (long long)d->heads_q, (long long)d->heads_kv,
+                (long long)d->seq, (long long)d->head_dim, (long long)d->rot_dim);
+  if (!is_float(d->dtype, true))
+    return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: dtype must be F32, F16 or BF16", fn);
+  if (!positions) return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: positions must be non-NULL", fn);
+  neptune_status st = rope_check(fn, d->head_dim, d->rot_dim, d->table_len, cos, sin, q_weight,
+                                 k_weight, d->interleaved, d->eps);
+  if (st != NEPTUNE_OK) return st;
+  const int64_t esize = d->dtype == NEPTUNE_DTYPE_F32 ? 4 : 2;
+  const int64_t sq[3] = {d->batch, d->heads_q, d->seq}, sk[3] = {d->batch, d->heads_kv, d->seq};
+  Strided in[2], out[2];
+  if ((st = resolve(fn, "q", q, d->q_stride, sq, 3, d->head_dim, esize, &in[0])) != NEPTUNE_OK ||
+      (st = resolve(fn, "k", k, d->k_stride, sk, 3, d->head_dim, esize, &in[1])) != NEPTUNE_OK ||
+      (st = resolve(fn, "qo", qo, d->qo_stride, sq, 3, d->head_dim, esize, &out[0])) != NEPTUNE_OK ||
+      (st = resolve(fn, "ko", ko, d->ko_stride, sk, 3, d->head_dim, esize, &out[1])) != NEPTUNE_OK)
+    return st;
+  // in place, q and k may lie head by head in one buffer; an output elsewhere
+  // may meet neither input nor the other output
+  const auto in_place = [&](int i) { return same_place(out[i], in[i], 3); };
+  if (qo == ko) return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: qo overlaps ko", fn);
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2 && !in_place(i); ++j)
+      if ((st = apart(fn, out[i], in[j])) != NEPTUNE_OK) return st;
+  if (!in_place(0) && !in_place(1) && (st = apart(fn, out[0], out[1])) != NEPTUNE_OK)
+    return st;
+  RopeLaunch L;
+  L.q = q; L.k = k; L.qo = qo; L.ko = ko;
+  L.q_weight = q_weight; L.k_weight = k_weight; L.cos = cos; L.sin = sin; L.positions = positions;
+  L.batch = d->batch; L.heads_q = d->heads_q; L.heads_kv = d->heads_kv; L.seq = d->seq;
+  L.head_dim = d->head_dim; L.rot_dim = d->rot_dim; L.table_len = d->table_len;
+  for (int i = 0; i < 3; ++i) {
+    L.qs[i] = in[0].stride[i]; L.ks[i] = in[1].stride[i];
+    L.qos[i] = out[0].stride[i]; L.kos[i] = out[1].stride[i];
+  }
+  L.dtype = d->dtype; L.interleaved = d->interleaved; L.eps = d->eps;
+  const char *why = "";
+  if (!rope_supported(L, &why)) return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: %s", fn, why);
+  st = device_ready();
+  if (st != NEPTUNE_OK) return st;
+  return hip_result(launch_rope(L, (hipStream_t)stream), "qk_norm_rope launch");
+}
+
+neptune_status neptune_kv_append_paged(const neptune_append_desc *d,
+                                       const neptune_paged_kv_desc *pk, const void *k,
+                                       const void *v, const void *q, const float *q_weight,
+                                       const float *k_weight, const float *cos, const float *sin,
+                                       const int32_t *block_table, const int32_t *cu_seqlens,
+                                       const int32_t *seq_lens, void *k_pages, void *v_pages,
+                                       const float *k_scales, const float *v_scales, void *qo,
+                                       void *stream) {
+  const char *fn = "kv_append_paged";
+  if (!d) return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: desc is NULL", fn);
+  if (d->tokens <= 0 || d->batch <= 0 || d->heads_q < 0 || d->heads_kv <= 0 || d->head_dim <= 0)
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT,
+                "%s: sizes must be positive (tokens=%lld batch=%lld heads_q=%lld heads_kv=%lld "
+                "head_dim=%lld)",
+                fn, (long long)d->tokens, (long long)d->batch, (long long)d->heads_q,
+                (long long)d->heads_kv, (long long)d->head_dim);
+  if (!is_float(d->dtype, false))
+    return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: dtype must be F16 or BF16", fn);
+  if (d->kv_dtype != d->dtype && d->kv_dtype != NEPTUNE_DTYPE_FP8_E4M3)
+    return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: kv_dtype must be dtype or FP8_E4M3", fn);
+  neptune_status st = rope_check(fn, d->head_dim, d->rot_dim, d->table_len, cos, sin, q_weight,
+                                 k_weight, d->interleaved, d->eps);
+  if (st != NEPTUNE_OK) return st;
+  Strided pools[2], in[3], out;
+  st = pools_check(fn, pk, k_pages, v_pages, k_scales, v_scales, block_table, cu_seqlens, seq_lens,
+                   d->tokens, d->batch, d->heads_kv, d->head_dim, d->kv_dtype, pools);
+  if (st != NEPTUNE_OK) return st;
+  const int64_t sq[2] = {d->tokens, d->heads_q}, sk[2] = {d->tokens, d->heads_kv};
+  const int n_in = d->heads_q ? 3 : 2;
+  if ((st = resolve(fn, "k", k, d->k_stride, sk, 2, d->head_dim, 2, &in[0])) != NEPTUNE_OK ||
+      (st = resolve(fn, "v", v, d->v_stride, sk, 2, d->head_dim, 2, &in[1])) != NEPTUNE_OK)
+    return st;
+  if (d->heads_q) {
+    if ((st = resolve(fn, "q", q, d->q_stride, sq, 2, d->head_dim, 2, &in[2])) != NEPTUNE_OK ||
+        (st = resolve(fn, "qo", qo, d->qo_stride, sq, 2, d->head_dim, 2, &out)) != NEPTUNE_OK)
+      return st;
+    for (int j = 0; j < 3 && !same_place(out, in[2], 2); ++j)
+      if ((st = apart(fn, out, in[j])) != NEPTUNE_OK) return st;
+    for (int i = 0; i < 2; ++i)
+      if ((st = apart(fn, out, pools[i])) != NEPTUNE_OK) return st;
+  }
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < n_in; ++j)
+      if ((st = apart(fn, pools[i], in[j])) != NEPTUNE_OK) return st;
+  RopeLaunch L;
+  L.append = true;
+  L.fp8 = d->kv_dtype == NEPTUNE_DTYPE_FP8_E4M3;
+  L.q = q; L.k = k; L.v = v; L.qo = qo; L.ko = k_pages; L.vo = v_pages;
+  L.q_weight = q_weight; L.k_weight = k_weight; L.cos = cos; L.sin = sin;
+  L.cu_seqlens = cu_seqlens; L.seq_lens = seq_lens; L.block_table = block_table;
+  L.k_scales = k_scales; L.v_scales = v_scales;
+  L.batch = 1; L.seq = d->tokens; L.heads_q = d->heads_q; L.heads_kv = d->heads_kv;
+  L.head_dim = d->head_dim; L.rot_dim = d->rot_dim; L.table_len = d->table_len;
+  L.sequences = d->batch; L.page_size = pk->page_size; L.max_pages = pk->max_pages;
+  L.num_pages = pk->num_pages;
+  // (token, head) -> (batch, head, seq)
+  const auto rows = [](const Strided &t, int64_t *s) {
+    s[0] = 0;
+    s[1] = t.stride[1];
+    s[2] = t.stride[0];
+  };
+  rows(in[0], L.ks);
+  rows(in[1], L.vs);
+  if (d->heads_q) {
+    rows(in[2], L.qs);
+    rows(out, L.qos);
+  }
+  for (int i = 0; i < 3; ++i) {
+    L.kos[i] = pools[0].stride[i];
+    L.vos[i] = pools[1].stride[i];
+  }
+  L.dtype = d->dtype; L.interleaved = d->interleaved; L.eps = d->eps;
+  const char *why = "";
+  if (!rope_supported(L, &why)) return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: %s", fn, why);
+  st = device_ready();
+  if (st != NEPTUNE_OK) return st;
+  return hip_result(launch_rope(L, (hipStream_t)stream), "kv_append_paged launch");
+}
+
+neptune_status neptune_attn_paged_workspace_bytes(const neptune_attn_paged_desc *d,
+                                                  size_t *bytes) {
+  if (!bytes)
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "attn_paged_workspace_bytes: bytes is NULL");
+  PagedAttnLaunch L;
+  neptune_status st = attn_paged_resolve(d, &L);
+  if (st != NEPTUNE_OK) return st;
+  const char *why = "";
+  if (!attn_paged_supported(L, &why)) return fail(NEPTUNE_ERR_UNSUPPORTED, "attn_paged: %s", why);
+  *bytes = attn_paged_bytes(L);
+  return ok();
+}
+
+neptune_status neptune_attn_paged(const neptune_attn_paged_desc *d,
+                                  const neptune_paged_kv_desc *pk, const void *q,
+                                  const void *k_pages, const void *v_pages, const float *k_scales,
+                                  const float *v_scales, const int32_t *block_table,
+                                  const int32_t *cu_seqlens, const int32_t *seq_lens, void *o,
+                                  float *lse, void *workspace, size_t workspace_bytes,
+                                  void *stream) {
+  const char *fn = "attn_paged";
+  PagedAttnLaunch L;
+  neptune_status st = attn_paged_resolve(d, &L);
+  if (st != NEPTUNE_OK) return st;
+  Strided pools[2], tq, to;
+  st = pools_check(fn, pk, k_pages, v_pages, k_scales, v_scales, block_table, cu_seqlens, seq_lens,
+                   d->tokens, d->batch, d->heads_kv, d->head_dim, d->kv_dtype, pools);
+  if (st != NEPTUNE_OK) return st;
+  if (pk->max_pages < cdiv(d->seq_kv, pk->page_size))
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT,
+                "%s: max_pages (%lld) * page_size (%lld) < seq_kv (%lld)", fn,
+                (long long)pk->max_pages, (long long)pk->page_size, (long long)d->seq_kv);
+  const int64_t sizes[2] = {d->tokens, d->heads_q};
+  if ((st = resolve(fn, "q", q, d->q_stride, sizes, 2, d->head_dim, 2, &tq)) != NEPTUNE_OK ||
+      (st = resolve(fn, "o", o, d->o_stride, sizes, 2, d->head_dim, 2, &to)) != NEPTUNE_OK ||
+      (st = apart(fn, to, tq)) != NEPTUNE_OK ||
+      (st = apart(fn, to, pools[0])) != NEPTUNE_OK ||
+      (st = apart(fn, to, pools[1])) != NEPTUNE_OK)
+    return st;
+  L.q = q; L.k = k_pages; L.v = v_pages; L.k_scales = k_scales; L.v_scales = v_scales;
+  L.block_table = block_table; L.cu_seqlens = cu_seqlens; L.seq_lens = seq_lens;
+  L.o = o; L.lse = lse; L.workspace = workspace;
+  L.page_size = pk->page_size; L.max_pages = pk->max_pages; L.num_pages = pk->num_pages;
+  for (int i = 0; i < 2; ++i) {
+    L.qs[i] = tq.stride[i];
+    L.os[i] = to.stride[i];
+  }
+  for (int i = 0; i < 3; ++i) {
+    L.kps[i] = pools[0].stride[i];
+    L.vps[i] = pools[1].stride[i];
+  }
+  const char *why = "";
+  if (!attn_paged_supported(L, &why)) return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: %s", fn, why);
+  const size_t need = attn_paged_bytes(L);
+  if (need) {
+    if (!workspace || workspace_bytes < need)
+      return fail(NEPTUNE_ERR_WORKSPACE_TOO_SMALL, "%s: workspace %zu bytes, need %zu", fn,
+                  workspace ? workspace_bytes : (size_t)0, need);
+    if (!aligned16(workspace))
+      return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: workspace must be 16-byte aligned", fn);
+  }
+  st = device_ready();
+  if (st != NEPTUNE_OK) return st;
+  return hip_result(launch_attn_paged(L, (hipStream_t)stream), "attn_paged launch");
+}
+
 neptune_status neptune_selective_scan_fwd(const neptune_scan_desc *d, const void *u,
                                           const void *delta_raw, const float *A, const void *B,
                                           const void *C, const float *D, const void *z,

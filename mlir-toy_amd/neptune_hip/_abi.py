@@ -48,6 +48,10 @@ EXPORTED_SYMBOLS = (
     "neptune_decode_paged",
     "neptune_decode_paged_fp8",
     "neptune_kv_quantize_fp8",
+    "neptune_qk_norm_rope",
+    "neptune_kv_append_paged",
+    "neptune_attn_paged_workspace_bytes",
+    "neptune_attn_paged",
     "neptune_selective_scan_fwd",
 )
 
@@ -106,6 +110,69 @@ class PagedKvDesc(ctypes.Structure):
         ("max_pages", ctypes.c_int64),
         ("k_stride", ctypes.c_int64 * 3),
         ("v_stride", ctypes.c_int64 * 3),
+    ]
+
+
+class RopeDesc(ctypes.Structure):
+    """include/neptune_hip.h: neptune_rope_desc"""
+
+    _fields_ = [
+        ("batch", ctypes.c_int64),
+        ("heads_q", ctypes.c_int64),
+        ("heads_kv", ctypes.c_int64),
+        ("seq", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("rot_dim", ctypes.c_int64),
+        ("table_len", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("qo_stride", ctypes.c_int64 * 3),
+        ("ko_stride", ctypes.c_int64 * 3),
+        ("dtype", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class AppendDesc(ctypes.Structure):
+    """include/neptune_hip.h: neptune_append_desc"""
+
+    _fields_ = [
+        ("tokens", ctypes.c_int64),
+        ("batch", ctypes.c_int64),
+        ("heads_q", ctypes.c_int64),
+        ("heads_kv", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("rot_dim", ctypes.c_int64),
+        ("table_len", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64 * 2),
+        ("k_stride", ctypes.c_int64 * 2),
+        ("v_stride", ctypes.c_int64 * 2),
+        ("qo_stride", ctypes.c_int64 * 2),
+        ("dtype", ctypes.c_int32),
+        ("kv_dtype", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class AttnPagedDesc(ctypes.Structure):
+    """include/neptune_hip.h: neptune_attn_paged_desc"""
+
+    _fields_ = [
+        ("tokens", ctypes.c_int64),
+        ("batch", ctypes.c_int64),
+        ("heads_q", ctypes.c_int64),
+        ("heads_kv", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("seq_kv", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64 * 2),
+        ("o_stride", ctypes.c_int64 * 2),
+        ("dtype", ctypes.c_int32),
+        ("kv_dtype", ctypes.c_int32),
+        ("scale_log2", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
     ]
 
 
@@ -222,6 +289,21 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.neptune_decode_paged_fp8.restype = i32
     lib.neptune_kv_quantize_fp8.argtypes = [i64, i64, i64, i64, i64, vp, vp, vp, vp]
     lib.neptune_kv_quantize_fp8.restype = i32
+    lib.neptune_qk_norm_rope.argtypes = [ctypes.POINTER(RopeDesc)] + [vp] * 10
+    lib.neptune_qk_norm_rope.restype = i32
+    lib.neptune_kv_append_paged.argtypes = [
+        ctypes.POINTER(AppendDesc), ctypes.POINTER(PagedKvDesc),
+    ] + [vp] * 16
+    lib.neptune_kv_append_paged.restype = i32
+    lib.neptune_attn_paged_workspace_bytes.argtypes = [
+        ctypes.POINTER(AttnPagedDesc),
+        ctypes.POINTER(ctypes.c_size_t),
+    ]
+    lib.neptune_attn_paged_workspace_bytes.restype = i32
+    lib.neptune_attn_paged.argtypes = [
+        ctypes.POINTER(AttnPagedDesc), ctypes.POINTER(PagedKvDesc),
+    ] + [vp] * 11 + [ctypes.c_size_t, vp]
+    lib.neptune_attn_paged.restype = i32
     lib.neptune_selective_scan_fwd.argtypes = [
         ctypes.POINTER(ScanDesc), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp,
     ]

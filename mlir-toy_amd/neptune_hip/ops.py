@@ -408,6 +408,323 @@ def kv_quantize_fp8(kv: torch.Tensor, *, scale_block: int = 64):
     return codes, scales
 
 
+def _ptr(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def _check_rotation(name, cos, sin, weights, head_dim) -> tuple[int, int]:
+    """(rot_dim, table_len) of the tables, checked with the norm weights."""
+    if (cos is None) != (sin is None):
+        raise ValueError(f"{name}: give cos and sin together")
+    if cos is not None:
+        for what, m in (("cos", cos), ("sin", sin)):
+            if m[2] != torch.float32 or len(m[0]) != 2 or not _contiguous(m):
+                raise ValueError(f"{name}: {what} must be a contiguous float32 "
+                                 "[positions, rot_dim / 2] tensor")
+        if cos[0] != sin[0]:
+            raise ValueError(f"{name}: cos {tuple(cos[0])} and sin {tuple(sin[0])} must match")
+    for what, m in weights:
+        if m is not None and (m[2] != torch.float32 or tuple(m[0]) != (head_dim,) or
+                              not _contiguous(m)):
+            raise ValueError(f"{name}: {what} must be a contiguous float32 [{head_dim}] tensor")
+    return (0, 0) if cos is None else (2 * cos[0][1], cos[0][0])
+
+
+@functools.lru_cache(maxsize=_PLANS, typed=True)
+def _rope_plan(q, k, cos, sin, positions, q_weight, k_weight, q_out, k_out, eps, interleaved):
+    """The descriptor."""
+    if q[2] not in _TORCH_TO_DTYPE or k[2] != q[2]:
+        raise ValueError(f"q and k must share one of {list(_TORCH_TO_DTYPE)}")
+    strides = [_strides_bhs(m) for m in (q, k)]
+    B, Hq, S, D = q[0]
+    Hk = k[0][1]
+    if tuple(k[0]) != (B, Hk, S, D):
+        raise ValueError(f"shape mismatch: q {tuple(q[0])} k {tuple(k[0])}")
+    for what, m, src in (("q", q_out, q), ("k", k_out, k)):
+        if m is None:
+            strides.append((0, 0, 0))
+            continue
+        if m[0] != src[0] or m[2] != src[2]:
+            raise ValueError(f"out must match {what}'s shape and dtype")
+        strides.append(_strides_bhs(m))
+    if cos is None:
+        raise ValueError("qk_norm_rope takes cos and sin tables")
+    rot, rows = _check_rotation("qk_norm_rope", cos, sin,
+                                (("q_weight", q_weight), ("k_weight", k_weight)), D)
+    if positions[2] != torch.int32 or tuple(positions[0]) != (B, S) or not _contiguous(positions):
+        raise ValueError("positions must be a contiguous int32 [B, S] tensor")
+    _require_cuda(q, k, cos, sin, positions, q_weight, k_weight, q_out, k_out)
+    desc = _abi.RopeDesc()
+    desc.batch, desc.heads_q, desc.heads_kv, desc.seq, desc.head_dim = B, Hq, Hk, S, D
+    desc.rot_dim, desc.table_len = rot, rows
+    desc.q_stride[:], desc.k_stride[:], desc.qo_stride[:], desc.ko_stride[:] = strides
+    desc.dtype = _TORCH_TO_DTYPE[q[2]]
+    desc.interleaved = interleaved
+    desc.eps = eps
+    return ctypes.byref(desc)
+
+
+def qk_norm_rope(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    positions: torch.Tensor,
+    *,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    interleaved: bool = False,
+    out: tuple[torch.Tensor, torch.Tensor] | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of each query and key head and its position rotation, one pass.
+
+    q [B, Hq, S, D], k [B, Hkv, S, D] in float32, float16 or bfloat16 (any
+    strides of whole 16-byte units with D contiguous, such as transposed
+    [B, S, H, D] projections); cos, sin float32 [positions, rot_dim / 2] (the
+    first rot_dim of D elements turn: pairs (i, i + rot_dim / 2), or
+    (2i, 2i + 1) when ``interleaved``); positions int32 [B, S]. With
+    ``q_weight`` / ``k_weight`` float32 [D] the heads are normalised first:
+    x * w / sqrt(mean(x^2) + eps). ``out`` = (q_out, k_out) may be (q, k).
+    Returns (q_out, k_out), by default new contiguous tensors.
+    """
+    q_out, k_out = (None, None) if out is None else out
+    desc = _rope_plan(_meta(q), _meta(k), _meta(cos), _meta(sin), _meta(positions),
+                      _meta(q_weight), _meta(k_weight), _meta(q_out), _meta(k_out), float(eps),
+                      1 if interleaved else 0)
+    if out is None:
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    lib = load_library()
+    _launch(lib, q.device, lib.neptune_qk_norm_rope, desc, q.data_ptr(), k.data_ptr(),
+            _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(),
+            q_out.data_ptr(), k_out.data_ptr())
+    return q_out, k_out
+
+
+def _strides_th(name, meta, heads, head_dim, tokens, dtype) -> tuple[int, int]:
+    shape, stride = meta[0], meta[1]
+    if len(shape) != 3 or stride[-1] != 1:
+        raise ValueError(f"{name}: expected [tokens, heads, head_dim] with unit head_dim stride")
+    if tuple(shape) != (tokens, heads, head_dim) or meta[2] != dtype:
+        raise ValueError(f"{name} is {tuple(shape)} {meta[2]}, expected "
+                         f"{(tokens, heads, head_dim)} {dtype}")
+    return stride[:2]
+
+
+def _pool_plan(name, dtype, tokens, k_pages, v_pages, block_table, seq_lens, cu_seqlens,
+               k_scales, v_scales):
+    """(page descriptor, neptune dtype of the pools, batch) of a ragged batch."""
+    fp8 = k_pages[2] in (torch.uint8, torch.float8_e4m3fn)
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"{name} takes float16 or bfloat16 tensors")
+    if k_pages[2] != v_pages[2] or not (fp8 or k_pages[2] == dtype):
+        raise ValueError(f"{name}: the pools must be {dtype} or E4M3, both alike")
+    if len(k_pages[0]) != 4 or k_pages[0] != v_pages[0] or k_pages[1][-1] != 1 or \
+            v_pages[1][-1] != 1:
+        raise ValueError("k_pages / v_pages: matching [pages, Hkv, page_size, D] views, D contiguous")
+    npages, Hk, psize, _ = k_pages[0]
+    if len(block_table[0]) != 2:
+        raise ValueError("block_table must be [B, max_pages]")
+    B, max_pages = block_table[0]
+    want = {"block_table": (B, max_pages), "seq_lens": (B,), "cu_seqlens": (B + 1,)}
+    for what, m in (("block_table", block_table), ("seq_lens", seq_lens),
+                    ("cu_seqlens", cu_seqlens)):
+        if m is None:
+            continue
+        if m[2] != torch.int32 or not _contiguous(m):
+            raise ValueError(f"{what} must be a contiguous int32 tensor")
+        if tuple(m[0]) != want[what]:
+            raise ValueError(f"{what} is {tuple(m[0])}, expected {want[what]}")
+    if cu_seqlens is None and tokens != B:
+        raise ValueError(f"without cu_seqlens every sequence has one new token: {tokens} tokens, "
+                         f"{B} sequences")
+    if fp8:
+        for what, m in (("k_scales", k_scales), ("v_scales", v_scales)):
+            if m is None or m[2] != torch.float32 or not _contiguous(m) or \
+                    tuple(m[0]) != (npages, Hk):
+                raise ValueError(f"fp8 pages need {what}: contiguous float32 [num_pages, Hkv]")
+    elif k_scales is not None or v_scales is not None:
+        raise ValueError("k_scales / v_scales apply to E4M3 pools only")
+    pk = _abi.PagedKvDesc()
+    pk.num_pages, pk.page_size, pk.max_pages = npages, psize, max_pages
+    pk.k_stride[:] = k_pages[1][:3]
+    pk.v_stride[:] = v_pages[1][:3]
+    return pk, _abi.DTYPE_FP8_E4M3 if fp8 else _TORCH_TO_DTYPE[dtype], B
+
+
+@functools.lru_cache(maxsize=_PLANS, typed=True)
+def _append_plan(k, v, k_pages, v_pages, block_table, seq_lens, cu_seqlens, q, cos, sin, q_weight,
+                 k_weight, k_scales, v_scales, out, eps, interleaved):
+    """(descriptor, page descriptor)."""
+    T = k[0][0] if len(k[0]) == 3 else 0
+    pk, kv_dtype, B = _pool_plan("kv_append_paged", k[2], T, k_pages, v_pages, block_table,
+                                 seq_lens, cu_seqlens, k_scales, v_scales)
+    _, Hk, _, D = k_pages[0]
+    desc = _abi.AppendDesc()
+    desc.k_stride[:] = _strides_th("k", k, Hk, D, T, k[2])
+    desc.v_stride[:] = _strides_th("v", v, Hk, D, T, k[2])
+    Hq = 0
+    if q is not None:
+        Hq = q[0][1] if len(q[0]) == 3 else 0
+        desc.q_stride[:] = _strides_th("q", q, Hq, D, T, k[2])
+        if out is not None:
+            desc.qo_stride[:] = _strides_th("out", out, Hq, D, T, k[2])
+    elif out is not None or q_weight is not None:
+        raise ValueError("out and q_weight go with q")
+    rot, rows = _check_rotation("kv_append_paged", cos, sin,
+                                (("q_weight", q_weight), ("k_weight", k_weight)), D)
+    _require_cuda(k, v, k_pages, v_pages, block_table, seq_lens, cu_seqlens, q, cos, sin, q_weight,
+                  k_weight, k_scales, v_scales, out)
+    desc.tokens, desc.batch, desc.heads_q, desc.heads_kv, desc.head_dim = T, B, Hq, Hk, D
+    desc.rot_dim, desc.table_len = rot, rows
+    desc.dtype, desc.kv_dtype = _TORCH_TO_DTYPE[k[2]], kv_dtype
+    desc.interleaved, desc.eps = interleaved, eps
+    return ctypes.byref(desc), ctypes.byref(pk)
+
+
+def kv_append_paged(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    cu_seqlens: torch.Tensor | None = None,
+    *,
+    q: torch.Tensor | None = None,
+    cos: torch.Tensor | None = None,
+    sin: torch.Tensor | None = None,
+    interleaved: bool = False,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor | None:
+    """Write new tokens' keys and values into a paged cache, in place.
+
+    k, v [T, Hkv, D] float16 or bfloat16, the new tokens of all sequences one
+    after the other: sequence b has rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1
+    (without ``cu_seqlens`` one row each), and seq_lens[b] counts its tokens
+    with them, so that its last row lands at seq_lens[b] - 1. k_pages / v_pages
+    [num_pages, Hkv, page_size, D] views as in ``decode_paged``, of k's dtype or
+    E4M3 codes under the given k_scales / v_scales [num_pages, Hkv]; block_table
+    [B, max_pages], seq_lens [B], cu_seqlens [B + 1] int32 on the device.
+
+    Keys are normalised (``k_weight``) and rotated (``cos``, ``sin``,
+    ``interleaved``) at their positions on the way, as in ``qk_norm_rope``; with
+    ``q`` [T, Hq, D] the queries too, and [T, Hq, D] is returned (``out``, which
+    may be q, or a new tensor; None without q). A row without a slot (a
+    negative place, one past its table, a table entry outside the pool) is not
+    stored; rows behind the last sequence are left out of the cache and of the
+    result.
+    """
+    desc, pk = _append_plan(
+        _meta(k), _meta(v), _meta(k_pages), _meta(v_pages), _meta(block_table), _meta(seq_lens),
+        _meta(cu_seqlens), _meta(q), _meta(cos), _meta(sin), _meta(q_weight), _meta(k_weight),
+        _meta(k_scales), _meta(v_scales), _meta(out), float(eps), 1 if interleaved else 0)
+    if q is not None and out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lib = load_library()
+    _launch(lib, k.device, lib.neptune_kv_append_paged, desc, pk, k.data_ptr(), v.data_ptr(),
+            _ptr(q), _ptr(q_weight), _ptr(k_weight), _ptr(cos), _ptr(sin), block_table.data_ptr(),
+            _ptr(cu_seqlens), seq_lens.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+            _ptr(k_scales), _ptr(v_scales), _ptr(out))
+    return out
+
+
+@functools.lru_cache(maxsize=_PLANS, typed=True)
+def _attn_paged_plan(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, k_scales, v_scales,
+                     out, max_seq_len, scale):
+    """(descriptor, page descriptor, workspace bytes)."""
+    if len(q[0]) != 3:
+        raise ValueError("attention_paged takes q [tokens, Hq, D]")
+    T, Hq, _ = q[0]
+    pk, kv_dtype, B = _pool_plan("attention_paged", q[2], T, k_pages, v_pages, block_table,
+                                 seq_lens, cu_seqlens, k_scales, v_scales)
+    _, Hk, psize, D = k_pages[0]
+    desc = _abi.AttnPagedDesc()
+    desc.q_stride[:] = _strides_th("q", q, Hq, D, T, q[2])
+    if out is not None:
+        desc.o_stride[:] = _strides_th("out", out, Hq, D, T, q[2])
+    _require_cuda(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, k_scales, v_scales, out)
+    desc.tokens, desc.batch, desc.heads_q, desc.heads_kv, desc.head_dim = T, B, Hq, Hk, D
+    desc.seq_kv = max_seq_len if max_seq_len is not None else pk.max_pages * psize
+    desc.dtype, desc.kv_dtype = _TORCH_TO_DTYPE[q[2]], kv_dtype
+    desc.scale_log2 = scale_to_log2(scale, D)
+    n = ctypes.c_size_t()
+    lib = load_library()
+    check(lib.neptune_attn_paged_workspace_bytes(ctypes.byref(desc), ctypes.byref(n)), lib)
+    return ctypes.byref(desc), ctypes.byref(pk), n.value
+
+
+def attention_paged(
+    q: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    cu_seqlens: torch.Tensor | None = None,
+    *,
+    max_seq_len: int | None = None,
+    scale: float | None = None,
+    return_lse: bool = False,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+    k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None,
+):
+    """Causal attention of new tokens over a paged cache that holds them.
+
+    q [T, Hq, D] float16 or bfloat16, the new tokens of all sequences one after
+    the other, any number each: a chunk of a prompt, guessed tokens to check, a
+    single token, none (``cu_seqlens`` and ``seq_lens`` as in
+    ``kv_append_paged``, called before). k_pages / v_pages, block_table,
+    k_scales / v_scales as in ``decode_paged`` (pools of q's dtype, or E4M3 with
+    bfloat16 q; page sizes that are multiples of 16; D 64 or 128).
+    ``max_seq_len`` (default max_pages * page_size) bounds the lengths. A row
+    sees its sequence up to its own place; one with a negative place sees
+    nothing: output 0, log-sum-exp -inf. Rows behind the last sequence are left
+    as they were. Returns o [T, Hq, D] (and lse [T, Hq] fp32 if asked).
+    """
+    desc, pk, need = _attn_paged_plan(
+        _meta(q), _meta(k_pages), _meta(v_pages), _meta(block_table), _meta(seq_lens),
+        _meta(cu_seqlens), _meta(k_scales), _meta(v_scales), _meta(out),
+        None if max_seq_len is None else int(max_seq_len), None if scale is None else float(scale))
+    _check_workspace(workspace, q.device)
+    if workspace is None and need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+    lib = load_library()
+    _launch(lib, q.device, lib.neptune_attn_paged, desc, pk, q.data_ptr(), k_pages.data_ptr(),
+            v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales), block_table.data_ptr(),
+            _ptr(cu_seqlens), seq_lens.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(workspace),
+            0 if workspace is None else workspace.numel() * workspace.element_size())
+    return (out, lse) if return_lse else out
+
+
+def attention_paged_workspace_bytes(
+    tokens: int, batch: int, heads_q: int, heads_kv: int, head_dim: int, max_seq_len: int,
+    *, dtype: torch.dtype = torch.bfloat16, fp8: bool = False,
+) -> int:
+    """Bytes of ``attention_paged``'s workspace for such a call (0: none)."""
+    desc = _abi.AttnPagedDesc()
+    desc.tokens, desc.batch, desc.heads_q, desc.heads_kv = tokens, batch, heads_q, heads_kv
+    desc.head_dim, desc.seq_kv = head_dim, max_seq_len
+    if dtype not in _TORCH_TO_DTYPE:
+        raise ValueError(f"dtype must be one of {list(_TORCH_TO_DTYPE)}")
+    desc.dtype = _TORCH_TO_DTYPE[dtype]
+    desc.kv_dtype = _abi.DTYPE_FP8_E4M3 if fp8 else desc.dtype
+    n = ctypes.c_size_t()
+    lib = load_library()
+    check(lib.neptune_attn_paged_workspace_bytes(ctypes.byref(desc), ctypes.byref(n)), lib)
+    return n.value
+
+
 @functools.lru_cache(maxsize=_PLANS, typed=True)
 def _scan_plan(u, delta, A, B, C, D, z, delta_bias, delta_softplus):
     """The descriptor."""
