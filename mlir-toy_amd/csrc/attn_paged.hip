@@ -13,7 +13,7 @@
 // of 128: K and V are then read once for the group, and the causal edge of a tile
 // spans 128 / group tokens only. The lengths are on the device, so the launch
 // has an upper bound of work-groups and each finds its item (sequence, tile,
-// split of the keys) itself from cu_seqlens and seq_lens (Schedule).
+// split of the keys) itself from cu_seqlens and seq_lens (make_plan, find_item).
 //
 // A work-group is that of attn_fwd_tile.hip: 4 waves of 32 rows, 64-key blocks,
 // S^T = K . Q^T and O^T = V^T . P^T on v_mfma_f32_32x32x16, two LDS slots per
@@ -25,6 +25,7 @@
 // work-group's four waves; the K scale meets the scores, the V scale P before
 // its rounding.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_tile.h"
 #include "kernels.h"
@@ -32,8 +33,8 @@
 namespace neptune {
 namespace {
 
-constexpr int64_t kSlots = 512;   // two work-groups on each of 256 CUs
-constexpr int64_t kParts = 2 * kSlots;  // split items a launch makes at most (Schedule)
+constexpr int kSlots = 512;         // two work-groups on each of 256 CUs
+constexpr int kParts = 4 * kSlots;  // split items a launch makes at most (make_plan)
 
 struct PagedArgs {
   const uint16_t *q;
@@ -48,7 +49,7 @@ struct PagedArgs {
   int32_t T, B, Hq, Hk, group, Lmax, maxp, npages;
   int32_t ps16;                   // page size in runs of 16 tokens
   uint32_t ps16_inv;              // floor((2^32 - 1) / ps16)
-  int32_t parts;                  // 0: keys are never split
+  int32_t parts;                  // items of cut tiles per KV head at most (0: none is cut)
   int32_t prows;                  // rows of a split item's states
   float scale2;
 };
@@ -63,6 +64,29 @@ __device__ inline void page_of(const PagedArgs &a, int run, int *index, int *res
   }
   *index = q;
   *rest = r;
+}
+
+// Inclusive sum over the wave's lanes of non-negative x (max: the running
+// maximum), by DPP moves
+template <bool MAX = false>
+__device__ inline int wave_scan(int x) {
+  auto step = [&](auto ctrl, auto rows) {
+    const int y = __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value,
+                                              0xf, false);
+    x = MAX ? max(x, y) : x + y;
+  };
+  typedef std::integral_constant<int, 0xf> all;
+  step(std::integral_constant<int, 0x111>{}, all{});  // row_shr 1, 2, 4, 8
+  step(std::integral_constant<int, 0x112>{}, all{});
+  step(std::integral_constant<int, 0x114>{}, all{});
+  step(std::integral_constant<int, 0x118>{}, all{});
+  step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast 15
+  step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // row_bcast 31
+  return x;
+}
+template <bool MAX = false>
+__device__ inline int wave_total(int x) {
+  return __builtin_amdgcn_readlane(wave_scan<MAX>(x), 63);
 }
 
 struct Item {
@@ -93,68 +117,116 @@ __device__ inline Seq sequence(const PagedArgs &a, int b) {
   return s;
 }
 
-// Splits of a sequence's tiles. A work-group's time is its chain of key blocks,
-// so chains longer than the launch's work over kSlots work-groups (work: tile
-// blocks, a tile's taken as the mean of its sequence's first and last tile's)
-// are cut into that many or longer. A split costs its states, written and read:
-// worth at least 4 blocks, 12 for a full tile.
-__device__ inline int splits_of(const Seq &s, int group, int chain) {
-  const int least = 4 + min(s.n * group, BM) / 16;
-  return max(s.blocks / max(chain, least), 1);
+// The cut of the keys. A work-group's time is its chain of key blocks, and a
+// launch's at least its blocks over kSlots work-groups, so chains longer than
+// that (chain) are cut. A tile of n splits takes blocks / n + 3 + n rows / 62
+// blocks of time, the latter two for the combine's launch and for writing and
+// reading the states of all rows (rows: full tiles of the launch; 128 rows of
+// states are 133 KB, a block some 1.65 us, memory 5 TB/s): least at n =
+// sqrt(62 blocks / rows), and no cut where that takes longer than the whole.
+__host__ __device__ inline int splits_of(int blocks, int chain, float rows) {
+  int n = blocks / (chain > 4 ? chain : 4);
+  const int best = (int)sqrtf(62.0f * (float)blocks / rows);
+  n = n < best ? n : best;
+  if (n < 2) return 1;
+  const int per = (blocks + n - 1) / n;
+  return (float)(blocks - per - 3) * 62.0f > (float)n * rows ? n : 1;
 }
 
-// Item idx of the launch (per_tile: tile idx) of one KV head, false if there is
-// none. Sequences in order, a sequence's tiles from the last (under the causal
-// mask the longest), a tile's splits together. Every wave works it out by
-// itself, one sequence per lane.
-__device__ inline bool find_item(const PagedArgs &a, int lane, int idx, bool per_tile, Item *it) {
-  int chain = 0x7fffffff;
-  if (a.parts) {
-    uint64_t work = 0;  // in half blocks
-    for (int b = lane; b < a.B; b += 64) {
-      const Seq s = sequence(a, b);
-      const int first = max(s.len - s.n + 1 + BN - 1, 0) / BN;
-      work += (uint64_t)s.tiles * (uint32_t)(s.blocks + min(first, s.blocks));
-    }
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-      const uint32_t lo = __shfl_xor((int)(uint32_t)work, off, 64);
-      const uint32_t hi = __shfl_xor((int)(uint32_t)(work >> 32), off, 64);
-      work += ((uint64_t)hi << 32) | lo;
-    }
-    work = (work * (uint32_t)a.Hk + 2 * kSlots - 1) / (2 * kSlots);
-    chain = work > 0x7fffffff ? 0x7fffffff : (int)work;
+// The launch's work in half key blocks (a tile's taken as the mean of its
+// sequence's first and last tile's) over `slots` work-groups, rounded up.
+__host__ __device__ inline int chain_of(uint64_t half_blocks, int slots) {
+  const uint64_t c = (half_blocks + 2 * slots - 1) / (2 * slots);
+  return c > 0x3fffffff ? 0x3fffffff : (int)c;
+}
+__host__ __device__ inline uint64_t half_blocks(int64_t tiles, int n, int len, int blocks) {
+  const int first = len - n + 1 > 0 ? (len - n + BN) / BN : 0;
+  return (uint64_t)tiles * (uint32_t)(blocks + (first < blocks ? first : blocks));
+}
+// Items for one round of kSlots, or shorter ones for two where the longest of
+// one round would outlast them: a round's lengths differ by up to a factor of
+// two, and only a second one fills up behind the short ones.
+__host__ __device__ inline int choose_chain(int one, int two, int longest1, int longest2) {
+  return longest1 <= one + longest2 / 2 ? one : two;
+}
+
+struct Plan {
+  int chain;
+  float rows;
+  Seq first;  // of the wave's lane as sequence 0 .. 63
+};
+
+// Every wave of the launch works the plan out by itself, one sequence per lane,
+// from integers and correctly rounded single operations alone: all agree.
+__device__ inline Plan make_plan(const PagedArgs &a, int lane) {
+  Plan p;
+  p.first = sequence(a, lane);
+  p.chain = 0x3fffffff;
+  p.rows = 1.0f;
+  if (!a.parts) return p;
+  // sums over the launch's tiles: half blocks, blocks (exactly, by 21 bits)
+  uint64_t work = 0, whole = 0;
+  int rows = 0;
+  for (int b = lane; b < a.B; b += 64) {
+    const Seq s = b < 64 ? p.first : sequence(a, b);
+    work += half_blocks(s.tiles, s.n, s.len, s.blocks);
+    whole += (uint64_t)s.tiles * (uint32_t)s.blocks;
+    rows += s.n * a.group;
   }
+  auto sum64 = [](uint64_t x) {
+    return (uint64_t)wave_total((int)(x & 0x1fffff)) +
+           ((uint64_t)wave_total((int)((x >> 21) & 0x1fffff)) << 21) +
+           ((uint64_t)wave_total((int)(x >> 42)) << 42);
+  };
+  const uint64_t total = sum64(work);
+  whole = sum64(whole);
+  p.rows = (float)wave_total(rows) * (float)a.Hk / (float)BM;
+  const int one = chain_of(total * (uint32_t)a.Hk, kSlots);
+  const int two = chain_of(total * (uint32_t)a.Hk, 2 * kSlots);
+  int longest1 = 0, longest2 = 0;
+  for (int b = lane; b < a.B; b += 64) {
+    const Seq s = b < 64 ? p.first : sequence(a, b);
+    if (!s.n) continue;
+    const int n1 = splits_of(s.blocks, one, p.rows), n2 = splits_of(s.blocks, two, p.rows);
+    longest1 = max(longest1, (s.blocks + n1 - 1) / n1);
+    longest2 = max(longest2, (s.blocks + n2 - 1) / n2);
+  }
+  // blocks / chain items come of a tile at most, so this many keep to a.parts
+  const uint64_t least = (whole + (uint32_t)a.parts - 1) / (uint32_t)a.parts;
+  const int chosen = choose_chain(one, two, wave_total<true>(longest1), wave_total<true>(longest2));
+  p.chain = max(chosen, (int)(least > 0x3fffffff ? 0x3fffffff : least));
+  return p;
+}
+
+// Item idx of one KV head, false if there is none. Sequences in order, a
+// sequence's tiles from the last (under the causal mask the longest), a tile's
+// splits together. take > 0 (it divides BM): instead the idx-th run of `take` rows
+// in a cut tile, split the run's first row in its tile.
+__device__ inline bool find_item(const PagedArgs &a, const Plan &p, int lane, int idx, int take,
+                                 Item *it) {
   int base = 0, parts = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const Seq s = sequence(a, b0 + lane);
-    const int sp = a.parts ? splits_of(s, a.group, chain) : 1;
-    const int mine = per_tile ? s.tiles : s.tiles * sp;
+    const Seq s = b0 ? sequence(a, b0 + lane) : p.first;
+    const int sp = a.parts ? splits_of(s.blocks, p.chain, p.rows) : 1;
     const int mparts = sp > 1 ? s.tiles * sp : 0;
-    int sum = mine, psum = mparts;  // inclusive sums over the lanes
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int u = __shfl_up(sum, off, 64), v = __shfl_up(psum, off, 64);
-      if (lane >= off) {
-        sum += u;
-        psum += v;
-      }
-    }
+    const int mine = take ? (sp > 1 ? (s.n * a.group + take - 1) / take : 0) : s.tiles * sp;
+    const int sum = wave_scan(mine), psum = wave_scan(mparts);
     const uint64_t past = __ballot(base + sum > idx);
     if (past) {
       const int at = __builtin_ctzll(past);
-      auto take = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+      auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
       it->b = b0 + at;
-      it->n = take(s.n);
-      it->row0 = take(s.row0);
-      it->len = take(s.len);
-      it->tiles = take(s.tiles);
-      it->splits = take(sp);
-      const int rest = idx - (base + take(sum) - take(mine));
-      const int down = per_tile ? rest : rest / it->splits;
+      it->n = of(s.n);
+      it->row0 = of(s.row0);
+      it->len = of(s.len);
+      it->tiles = of(s.tiles);
+      it->splits = of(sp);
+      const int rest = idx - (base + of(sum) - of(mine));
+      // tiles before this one in the items' order
+      const int down = take ? it->tiles - 1 - rest * take / BM : rest / it->splits;
       it->tile = it->tiles - 1 - down;
-      it->split = per_tile ? 0 : rest - down * it->splits;
-      it->part = parts + take(psum) - take(mparts) + down * it->splits;
+      it->split = take ? rest * take % BM : rest - down * it->splits;
+      it->part = parts + of(psum) - of(mparts) + down * it->splits;
       return true;
     }
     base += __builtin_amdgcn_readlane(sum, 63);
@@ -163,11 +235,317 @@ __device__ inline bool find_item(const PagedArgs &a, int lane, int idx, bool per
   return false;
 }
 
+typedef int v2i32 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) v2i32 lds_v2i32;
+
 // bf16 bits of 4 E4M3 codes (exact)
 __device__ inline u32x2 widen4(uint32_t c) {
   const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.0f, false);
   const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.0f, true);
   return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+}
+
+// A tile of at most 32 rows (generated or guessed tokens, a chunk's last few): the
+// wide form would compute in one wave of four and hold 32 KB in flight between
+// barriers, and such an item is bound by memory. Here the four waves share out
+// the item's keys in steps of 32, each streaming its own through 16 KB of LDS
+// with no barrier: K of step i + N is issued once step i's scores are formed, V
+// once its P.V is (N slots per operand: 1 for 16-bit head_dim 128, 2 or 4 for
+// smaller rows), so a wave has copies in flight at all times. E4M3 codes stay codes in
+// LDS and are widened as operands are read. The running max moves with every
+// step, so a row's largest p is 1. At the end the waves' states merge in LDS, a
+// quarter of the head_dim each.
+constexpr int NARROW = 32;
+
+template <class E, int HD, bool FP8>
+__device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, int w, int lane,
+                                   int kb0, int nv, const uint8_t *smem, f32x2 *mlbox) {
+  typedef typename E::vec8 V8;
+  constexpr int STEP = 32;
+  constexpr int RB = HD * (FP8 ? 1 : 2);        // bytes of a row
+  constexpr int TILE = STEP * RB;
+  constexpr int REGION = 16384;                 // LDS per wave
+  constexpr int N = REGION / (2 * TILE);        // slots per operand
+  constexpr int UNITS = RB / 16, RPC = 64 / UNITS;  // 16-byte units per row, rows per 1 KiB chunk
+  constexpr int CH = TILE / 1024;               // chunks per tile
+  constexpr int NST = HD / 16, NB = HD / 32;
+  const int lq = lane & 31, g = lane >> 5;
+  const uint8_t *const mine = smem + w * REGION;
+  auto kslot = [&](int i) { return mine + (i % N) * TILE; };
+  auto vslot = [&](int i) { return mine + (N + i % N) * TILE; };
+  // 256 bytes hold 1, 2 or 4 rows: the unit that row r's unit u goes to
+  auto kswz = [](int r) {
+    return UNITS == 16 ? r & 15 : UNITS == 8 ? (r >> 1) & 7 : (r >> 2) & 3;
+  };
+  auto vswz = [](int r) {
+    return FP8 ? (UNITS == 8 ? (r >> 1) & 7 : (r >> 2) & 3)
+               : (UNITS == 16 ? (r & 3) << 2 : ((r >> 1) & 1) << 2);
+  };
+
+  const int off = it.len - it.n, base_row = it.tile * BM;
+  const int rows = min(it.n * a.group - base_row, NARROW);
+  const int row = base_row + min(lq, rows - 1);
+  const int tok = row / a.group, hr = row - tok * a.group;
+  const int pos = off + tok;
+  const int lo = __builtin_amdgcn_readfirstlane(off + base_row / a.group);
+  const int last = off + (base_row + rows - 1) / a.group;  // the last row's place
+  // the wave's steps of the item's
+  const int s0 = 2 * kb0, s1 = min(2 * (kb0 + nv), last < 0 ? 0 : last / STEP + 1);
+  const int share = (max(s1 - s0, 0) + 3) >> 2;
+  const int t0 = __builtin_amdgcn_readfirstlane(s0 + w * share);
+  const int ns = __builtin_amdgcn_readfirstlane(max(min(t0 + share, s1) - t0, 0));
+
+  const char *kp = a.k + hk * a.kps1, *vp = a.v + hk * a.vps1;
+  const int32_t *tab = a.btab + (int64_t)it.b * a.maxp;
+  const int last_run = (it.len - 1) >> 4;
+  const bool once = it.tiles == 1;  // no other work-group reads these keys
+  int tab0 = 0, tabv = 0, sc0 = 0;
+  float kscv = 0.0f, vscv = 0.0f;
+  auto load_tab = [&](int first) {
+    tab0 = first;
+    const int j = first + lane;
+    tabv = j < a.maxp ? tab[j] : 0;
+  };
+  auto load_scales = [&](int first) {
+    sc0 = first;
+    const int j = first + lane;
+    const int page = min(max(j < a.maxp ? tab[j] : 0, 0), a.npages - 1);
+    kscv = a.ksc[(int64_t)page * a.Hk + hk];
+    vscv = a.vsc[(int64_t)page * a.Hk + hk];
+  };
+  if (ns > 0) {
+    int index, rest;
+    page_of(a, min(2 * t0, last_run), &index, &rest);
+    load_tab(index);
+    if constexpr (FP8) load_scales(index);
+  }
+  u32x4 qf[NST];
+  {
+    const uint16_t *qp = a.q + (int64_t)(it.row0 + tok) * a.qs0 +
+                         (int64_t)(hk * a.group + hr) * a.qs1 + 8 * g;
+#pragma unroll
+    for (int st = 0; st < NST; ++st)
+      qf[st] = lq < rows ? *(const u32x4 *)(qp + 16 * st) : u32x4{0, 0, 0, 0};
+  }
+  settle(kscv);
+  settle(vscv);
+#pragma unroll
+  for (int st = 0; st < NST; ++st) settle(qf[st]);
+  settle(tabv);
+
+  // one operand's copy of step i: two runs of 16 rows, each within a page, rows
+  // behind the sequence's end from its last
+  const int crow = lane / UNITS, cunit = lane & (UNITS - 1);
+  auto copy = [&](int i, auto is_v, const uint8_t *tile) {
+    constexpr bool V = decltype(is_v)::value;
+    const int64_t tokb = V ? a.vtok : a.ktok;
+    static_for<2>([&](auto H) {
+      constexpr int h = decltype(H)::value;
+      const int run = min(2 * (t0 + i) + h, last_run);
+      int index, rest;
+      page_of(a, run, &index, &rest);
+      if (index - tab0 >= 64) {
+        load_tab(max(index - 1, 0));  // V's first run may lie a page before K's second
+        settle(tabv);
+      }
+      int page = __builtin_amdgcn_readlane(tabv, index - tab0);
+      page = min(max(page, 0), a.npages - 1);
+      const char *src = (V ? vp + page * a.vps0 : kp + page * a.kps0) + (int64_t)(rest * 16) * tokb;
+      const int most = it.len - 1 - run * 16;
+      auto issue = [&](auto nt) {
+#pragma unroll
+        for (int c = 0; c < CH / 2; ++c) {
+          const int r = crow + RPC * c;  // of the run
+          const int u = cunit ^ (V ? vswz(16 * h + r) : kswz(16 * h + r));
+          dma16<decltype(nt)::value>(src, (uint32_t)(min(r, most) * tokb + u * 16),
+                                     lds_offset(tile + (h * CH / 2 + c) * 1024));
+        }
+      };
+      if (once)
+        issue(std::true_type{});
+      else
+        issue(std::false_type{});
+    });
+  };
+  auto copy_k = [&](int i) { copy(i, std::false_type{}, kslot(i)); };
+  auto copy_v = [&](int i) { copy(i, std::true_type{}, vslot(i)); };
+
+  f32x16 o[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[nb][r] = 0.0f;
+  float m = kNegFltMax, lsum = 0.0f;
+  static_for<N>([&](auto J) {
+    if (decltype(J)::value < ns) {
+      copy_k(decltype(J)::value);
+      copy_v(decltype(J)::value);
+    }
+  });
+  // waits until the copies issued after a tile are all that is in flight: `pairs`
+  // whole steps' (at most N - 1) and X tiles
+  auto wait_tiles = [&](int pairs, auto extra) {
+    constexpr int X = decltype(extra)::value;
+    static_for<N>([&](auto P) {
+      constexpr int n = decltype(P)::value;
+      if (min(pairs, N - 1) == n) __builtin_amdgcn_s_waitcnt(waitcnt_vm(CH * (2 * n + X)));
+    });
+    asm volatile("" ::: "memory");  // no read of the tile before the wait
+  };
+
+  for (int i = 0; i < ns; ++i) {
+    const int later = ns - 1 - i;
+    const int key0 = (t0 + i) * STEP;
+    wait_tiles(later, std::integral_constant<int, 1>{});  // K(i) is there
+    f32x16 s = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    {
+      const uint8_t *kt = kslot(i) + lq * RB;
+#pragma unroll
+      for (int st = 0; st < NST; ++st) {
+        u32x4 A;
+        if constexpr (FP8) {
+          const u32x2 c = *(const u32x2 *)(kt + ((st ^ kswz(lq)) << 4) + 8 * g);
+          const u32x2 x = widen4(c[0]), y = widen4(c[1]);
+          A = u32x4{x[0], x[1], y[0], y[1]};
+        } else {
+          A = *(const u32x4 *)(kt + (((2 * st + g) ^ kswz(lq)) << 4));
+        }
+        s = E::mfma32(as_vec8<V8>(A), as_vec8<V8>(qf[st]), s);
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(kWaitLgkm0);  // K(i) has been read
+    if (later >= N) copy_k(i + N);
+    float vs[2] = {1.0f, 1.0f};
+    if constexpr (FP8) {
+      // the scales of both runs: K's before the mask, V's with P
+      static_for<2>([&](auto H) {
+        constexpr int h = decltype(H)::value;
+        int index, rest;
+        page_of(a, min(2 * (t0 + i) + h, last_run), &index, &rest);
+        if (index - sc0 >= 64) {
+          load_scales(index);
+          settle(kscv);
+          settle(vscv);
+        }
+        const float ks = a.scale2 * __builtin_bit_cast(
+            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, kscv), index - sc0));
+        vs[h] = __builtin_bit_cast(
+            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vscv), index - sc0));
+#pragma unroll
+        for (int r = 0; r < 8; ++r) s[8 * h + r] *= ks;
+      });
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] *= a.scale2;
+    }
+    if (key0 + STEP - 1 > lo) {
+      const int lim = pos - key0 - 4 * g;  // element r holds key 4 g + 8 (r >> 2) + (r & 3)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (8 * (r >> 2) + (r & 3) > lim) s[r] = -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    mx = pair_max(mx);
+    if (__any(mx > m)) {
+      const float m_new = fmaxf(m, mx);
+      const float alpha = fast_exp2(m - m_new);
+      lsum *= alpha;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[nb][r] *= alpha;
+      m = m_new;
+    }
+    u32x4 pf[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float p0 = fast_exp2(s[8 * c + 2 * j] - m), p1 = fast_exp2(s[8 * c + 2 * j + 1] - m);
+        lsum += p0 + p1;
+        pf[c][j] = FP8 ? E::pack2(p0 * vs[c], p1 * vs[c]) : E::pack2(p0, p1);
+      }
+    if (later >= N)
+      wait_tiles(N - 1, std::integral_constant<int, 1>{});  // V(i) is there, K(i + N) after it
+    else
+      wait_tiles(later, std::integral_constant<int, 0>{});
+    const uint8_t *vt = vslot(i);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        u32x4 A;
+        const int s16 = lane & 15, dh = (lane >> 4) & 1;
+        if constexpr (FP8) {
+          // lane pair (2 j, 2 j + 1) of 16 names the row of k-slot j
+          const int j = s16 >> 1, r = 16 * c + 4 * g + (j & 3) + 8 * (j >> 2);
+          const v2i32 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i32 *)as_lds(
+              vt + r * RB + (((2 * nb + dh) ^ vswz(r)) << 4) + 8 * (s16 & 1)));
+          const u32x2 y = widen4((uint32_t)x[0]), z = widen4((uint32_t)x[1]);
+          A = u32x4{y[0], y[1], z[0], z[1]};
+        } else {
+          const int j = s16 >> 2, r = 16 * c + 4 * g + j;
+          const uint8_t *p = vt + r * RB + (((4 * nb + 2 * dh) ^ vswz(j)) << 4) + 8 * (s16 & 3);
+          const u32x2 y = __builtin_bit_cast(u32x2, lds_read_tr16(p));
+          const u32x2 z = __builtin_bit_cast(u32x2, lds_read_tr16(p + 8 * RB));
+          A = u32x4{y[0], y[1], z[0], z[1]};
+        }
+        o[nb] = E::mfma32(as_vec8<V8>(A), as_vec8<V8>(pf[c]), o[nb]);
+      }
+    __builtin_amdgcn_s_waitcnt(kWaitLgkm0);  // V(i) has been read
+    if (later >= N) copy_v(i + N);
+  }
+
+  // the waves' states, merged lane by lane, NB of a row's 4 NB vectors a wave
+  const float ltot = pair_sum(lsum);
+  f32x4 *const box = (f32x4 *)mine + lane;
+#pragma unroll
+  for (int v = 0; v < 4 * NB; ++v)
+    box[v * 64] = f32x4{o[v >> 2][4 * (v & 3)], o[v >> 2][4 * (v & 3) + 1],
+                        o[v >> 2][4 * (v & 3) + 2], o[v >> 2][4 * (v & 3) + 3]};
+  mlbox[w * 64 + lane] = f32x2{m, ltot};
+  __syncthreads();
+  float M = kNegFltMax, L = 0.0f, wgt[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) M = fmaxf(M, mlbox[k * 64 + lane][0]);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const f32x2 ml = mlbox[k * 64 + lane];
+    wgt[k] = fast_exp2(ml[0] - M);
+    L = fmaf(wgt[k], ml[1], L);
+  }
+  if (lq >= rows) return;
+  const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+  auto quot = [&](float v) {
+    const float q0 = v * inv;
+    return __builtin_fmaf(__builtin_fmaf(-q0, L, v), inv, q0);
+  };
+  const int64_t t = it.row0 + tok;
+  const int64_t part = ((int64_t)(it.part + it.split) * a.Hk + hk) * a.prows + lq;
+#pragma unroll
+  for (int k = 0; k < NB; ++k) {
+    const int v = w * NB + k, d = 32 * (v >> 2) + 8 * (v & 3) + 4 * g;
+    f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4 y = *((const f32x4 *)(smem + j * REGION) + v * 64 + lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = fmaf(wgt[j], y[e], x[e]);
+    }
+    if (it.splits > 1)
+      *(f32x4 *)(a.po + part * HD + d) = x;
+    else
+      *(u32x2 *)(a.o + t * a.os0 + (int64_t)(hk * a.group + hr) * a.os1 + d) =
+          u32x2{E::pack2(quot(x[0]), quot(x[1])), E::pack2(quot(x[2]), quot(x[3]))};
+  }
+  if (w == 0 && g == 0) {
+    if (it.splits > 1)
+      *(f32x2 *)(a.pml + part * 2) = f32x2{M, L};
+    else if (a.lse)
+      a.lse[t * a.Hq + hk * a.group + hr] = L > 0.0f ? row_lse(M, L) : -INFINITY;
+  }
 }
 
 template <class E, int HD, bool FP8>
@@ -181,7 +559,8 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   constexpr int NQK = 2 * NST, NPV = 4 * NB;  // MFMAs per key block
   constexpr int CHUNKS = TL::CHUNKS, RPC = TL::RPC;
   // K slots 0 and 1, then V slots 0 and 1; block t uses slot t & 1
-  __shared__ __attribute__((aligned(16))) uint8_t smem[4 * TILE];
+  __shared__ __attribute__((aligned(16))) uint8_t smem[65536];
+  __shared__ f32x2 mlbox[NT];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -192,9 +571,10 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   // kv heads fastest: with a multiple of 8 of them, id % 8 (the XCD) fixes the
   // head modulo 8 and the tiles of a head share an L2
   const int hk = __builtin_amdgcn_readfirstlane((int)(blockIdx.x % (uint32_t)a.Hk));
+  const Plan plan = make_plan(a, lane);
   const int idx = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / (uint32_t)a.Hk));
   Item it;
-  if (!find_item(a, lane, idx, false, &it)) return;
+  if (!find_item(a, plan, lane, idx, 0, &it)) return;
   const int rows = it.n * a.group;
   const int off = it.len - it.n;  // place of the sequence's first new token
   const int r0 = it.tile * BM + w * 32;
@@ -212,6 +592,10 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   const int per = (all + it.splits - 1) / it.splits;
   const int kb0 = __builtin_amdgcn_readfirstlane(it.split * per);
   const int nv = __builtin_amdgcn_readfirstlane(min(max(all - kb0, 0), per));
+  if (rows - it.tile * BM <= NARROW) {
+    narrow_item<E, HD, FP8>(a, it, hk, w, lane, kb0, nv, smem, mlbox);
+    return;
+  }
   const int nkw = __builtin_amdgcn_readfirstlane(
       r0 < rows ? min(max(blocks_to(r0 + 31) - kb0, 0), nv) : 0);
   const int lo_w = __builtin_amdgcn_readfirstlane(off + min(r0, rows - 1) / a.group);
@@ -220,14 +604,13 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   const int32_t *tab = a.btab + (int64_t)it.b * a.maxp;
   const int last_key = it.len - 1;
 
-  // the window of the block table: lane j holds entry tab0 + j. It starts at a
-  // page of the block before the one being copied and moves when a copy passes it
+  // the window of the block table: lane j holds entry tab0 + j; the copies' pages
+  // only ever move on
   int tab0 = 0, tabv = 0;
   auto load_tab = [&](int first) {
     tab0 = first;
     const int j = first + lane;
     tabv = j < a.maxp ? tab[j] : 0;
-    settle(tabv);
   };
   // the wave's run of block t: its page's byte offset in each pool, and the
   // tokens of it that exist less one (a run behind the end takes the last run)
@@ -237,7 +620,10 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
     run = key >> 4;
     int index, rest;
     page_of(a, run, &index, &rest);
-    if (index - tab0 >= 64) load_tab(max(index - 4, 0));
+    if (index - tab0 >= 64) {
+      load_tab(index);
+      settle(tabv);
+    }
     int page = __builtin_amdgcn_readlane(tabv, index - tab0);
     page = min(max(page, 0), a.npages - 1);
     *ko = page * a.kps0 + (int64_t)(rest * 16) * a.ktok;
@@ -260,7 +646,7 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
     if (most >= 15) {
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c)
-        dma16(base, offs[c], lds_offset(tile + (CHUNKS * w + c) * 1024));
+        dma16_sbase(base, offs[c], lds_offset(tile + (CHUNKS * w + c) * 1024));
     } else {
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c) {
@@ -277,9 +663,10 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   u32x4 k8[N8], v8[N8];
   auto load8 = [&](const char *base, int64_t tokb, int most, u32x4 *dst) {
 #pragma unroll
-    for (int c = 0; c < N8; ++c)
-      dst[c] = *(const u32x4 *)(base + min(lane / LPR8 + ROWS8 * c, most) * tokb +
-                                (lane % LPR8) * 16);
+    for (int c = 0; c < N8; ++c) {
+      const int r = lane / LPR8 + ROWS8 * c;
+      dst[c] = *(const u32x4 *)(base + (uint32_t)(min(r, most) * (int)tokb + (lane % LPR8) * 16));
+    }
   };
   auto store8 = [&](const u32x4 *src, const uint8_t *tile, bool is_v) {
 #pragma unroll
@@ -333,18 +720,33 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
 #pragma unroll
     for (int st = 0; st < NST; ++st)
       qf[st] = row < rows ? *(const u32x4 *)(qp + 16 * st) : u32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int st = 0; st < NST; ++st) settle(qf[st]);
   }
+  // E4M3: the scales of the block-table entries sc0 .. sc0 + 63, a lane each
+  int sc0 = 0;
+  float kscv = 0.0f, vscv = 0.0f;
+  auto load_scales = [&](int first) {
+    sc0 = first;
+    const int j = first + lane;
+    const int page = min(max(j < a.maxp ? tab[j] : 0, 0), a.npages - 1);
+    kscv = a.ksc[(int64_t)page * a.Hk + hk];
+    vscv = a.vsc[(int64_t)page * a.Hk + hk];
+  };
+  if constexpr (FP8) {
+    if (nv > 0) load_scales(tab0);
+    settle(kscv);
+    settle(vscv);
+  }
+  // Q and the table land before the first copy is issued
+#pragma unroll
+  for (int st = 0; st < NST; ++st) settle(qf[st]);
+  settle(tabv);
   if (nv > 0) {
     load_k(0);
-    put_k(0);
     load_v(0);
+    put_k(0);
+    if (nv > 1) load_k(1);
     put_v(0);
-  }
-  if (nv > 1) {
-    load_k(1);
-    put_k(1);
+    if (nv > 1) put_k(1);
   }
 
   // per-lane LDS byte offsets of the operand reads
@@ -358,22 +760,6 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
       va[nb] = (4 * g + i) * ROWB + (((4 * nb + 2 * dh) ^ tile_swizzle<HD, true>(i)) << 4) + 8 * q;
-  }
-
-  // E4M3: the scales of the block-table entries sc0 .. sc0 + 63, a lane each
-  int sc0 = 0;
-  float kscv = 0.0f, vscv = 0.0f;
-  auto load_scales = [&](int first) {
-    sc0 = first;
-    const int j = first + lane;
-    const int page = min(max(j < a.maxp ? tab[j] : 0, 0), a.npages - 1);
-    kscv = a.ksc[(int64_t)page * a.Hk + hk];
-    vscv = a.vsc[(int64_t)page * a.Hk + hk];
-  };
-  if constexpr (FP8) {
-    int index, rest;
-    page_of(a, kb0 * (BN / 16), &index, &rest);
-    if (nv > 0) load_scales(index);
   }
 
   f32x16 o[NB];
@@ -429,28 +815,48 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
       const u32x4 vp0 = v_operand(vt, 0), vp1 = v_operand(vt, 1);
       const int key0 = (kb0 + jb) * BN;
       float sc = a.scale2;
-      float vs[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+      // E4M3: V's scales meet P. Over a block within one page K's scale goes with
+      // the score scale and V's into the exponent (lv), so they cost no operation
+      // an element; the sum is then of scaled p, and unscaled by one product (iv).
+      // Across pages, or where the exponent would not hold the scale, each run's
+      // are multiplied in: K's here, before the mask (a zero scale must not meet
+      // -inf), V's with P.
+      float vs[4] = {1.0f, 1.0f, 1.0f, 1.0f}, lv = 0.0f, iv = 1.0f;
+      bool apart = false;
       if constexpr (FP8) {
-        // each run's scales: K's meets the scores here (before the mask: a zero
-        // scale must not meet -inf), V's meets P
         int index, rest;
         page_of(a, key0 >> 4, &index, &rest);
-        if (index + 3 - sc0 >= 64) load_scales(index);
-        const int runs = last_key / 16 - (key0 >> 4);  // runs behind the end take the last one's
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float ks = sc * __builtin_bit_cast(
-              float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, kscv), index - sc0));
-          vs[c] = __builtin_bit_cast(
-              float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vscv), index - sc0));
-#pragma unroll
-          for (int r = 0; r < 8; ++r) s[c >> 1][8 * (c & 1) + r] *= ks;
-          if (c < runs && ++rest == a.ps16) {
-            rest = 0;
-            ++index;
-          }
+        if (index + 3 - sc0 >= 64) {
+          load_scales(index);
+          // here, not where they are read: that would drain the loads above too
+          settle(kscv);
+          settle(vscv);
         }
-        sc = 1.0f;
+        auto scale_at = [&](float v, int i) {
+          return __builtin_bit_cast(
+              float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i - sc0));
+        };
+        const int runs = last_key / 16 - (key0 >> 4);  // runs behind the end take the last one's
+        const float v0 = scale_at(vscv, index);
+        apart = (rest + 3 >= a.ps16 && runs > 0) || !(v0 >= 0x1p-64f && v0 <= 0x1p64f);
+        if (apart) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float ks = sc * scale_at(kscv, index);
+            vs[c] = scale_at(vscv, index);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) s[c >> 1][8 * (c & 1) + r] *= ks;
+            if (c < runs && ++rest == a.ps16) {
+              rest = 0;
+              ++index;
+            }
+          }
+          sc = 1.0f;
+        } else {
+          sc *= scale_at(kscv, index);
+          lv = __builtin_amdgcn_logf(v0);
+          iv = 1.0f / v0;
+        }
       }
       if (key0 + BN - 1 > lo_w) {
         // element (kb, r) holds key key0 + 4 g + c with c = 32 kb + 8 (r >> 2)
@@ -466,7 +872,7 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
       float rs;
       u32x4 pf[4];
       auto expo = [&]() {
-        const float nm = -m;
+        const float nm = FP8 ? lv - m : -m;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int kb = c >> 1, hh = c & 1;
@@ -476,7 +882,20 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
             const float p1 = fast_exp2(fmaf(s[kb][8 * hh + 2 * i + 1], sc, nm));
             rs = c + i == 0 ? p0 : rs + p0;
             rs += p1;
-            pf[c][i] = FP8 ? E::pack2(p0 * vs[c], p1 * vs[c]) : E::pack2(p0, p1);
+            pf[c][i] = E::pack2(p0, p1);
+          }
+        }
+        if constexpr (FP8) {
+          rs *= iv;
+          if (apart) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float p0 = fast_exp2(fmaf(s[c >> 1][8 * (c & 1) + 2 * i], sc, nm));
+                const float p1 = fast_exp2(fmaf(s[c >> 1][8 * (c & 1) + 2 * i + 1], sc, nm));
+                pf[c][i] = E::pack2(p0 * vs[c], p1 * vs[c]);
+              }
           }
         }
       };
@@ -583,46 +1002,80 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
     a.lse[t * a.Hq + hk * a.group + hr] = ltot > 0.0f ? row_lse(m, ltot) : -INFINITY;
 }
 
-// Combine of a split tile's states, one work-group per (tile, kv head) and 8 (16
-// at head_dim 64) of its rows: HD / 4 lanes per row, four elements each.
-// M = max m_s, l = sum 2^(m_s - M) l_s, O = sum 2^(m_s - M) O_s / l. A split with
-// l_s = 0 (no visible key) may have left no O_s and is passed over.
-template <class E, int HD>
-__global__ __launch_bounds__(NT) void attn_paged_combine(PagedArgs a) {
-  constexpr int LPR = HD / 4, ROWS = NT / LPR;
+// Combine of the cut tiles' states: M = max m_s, l = sum 2^(m_s - M) l_s, O = sum
+// 2^(m_s - M) O_s / l. HD / 4 lanes per row, four elements each, and SG groups of
+// them per row, group g taking splits g, g + SG, .. four at a time; a work-group
+// takes `take` rows of a tile. A split with l_s = 0 (no visible key) may have left
+// no O_s and is passed over.
+template <class E, int HD, int SG>
+__global__ __launch_bounds__(NT) void attn_paged_combine(PagedArgs a, int take) {
+  constexpr int LPR = HD / 4, ROWS = NT / LPR / SG;
+  __shared__ float st[SG > 1 ? NT : 1][6];
   const int lane = threadIdx.x & 63;
-  const int hk = __builtin_amdgcn_readfirstlane((int)(blockIdx.x % (uint32_t)a.Hk));
-  const int idx = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / (uint32_t)a.Hk));
+  const int grp = threadIdx.x / LPR, sg = grp % SG, d = 4 * (threadIdx.x % LPR);
+  const Plan plan = make_plan(a, lane);
+  const uint32_t hk = blockIdx.x % (uint32_t)a.Hk;
   Item it;
-  if (!find_item(a, lane, idx, true, &it) || it.splits <= 1) return;
-  const int r = blockIdx.y * ROWS + threadIdx.x / LPR, row = it.tile * BM + r;
-  if (r >= BM || row >= it.n * a.group) return;
-  const int d = 4 * (threadIdx.x % LPR);
-  const int64_t part = ((int64_t)it.part * a.Hk + hk) * a.prows + r;
+  if (!find_item(a, plan, lane, (int)(blockIdx.x / (uint32_t)a.Hk), take, &it)) return;
+  const int r0 = it.split;
+  const int rows = min(min(it.n * a.group - it.tile * BM, BM), r0 + take);
   const int64_t step = (int64_t)a.Hk * a.prows;
-  float M = kNegFltMax;
-  for (int s = 0; s < it.splits; ++s) M = fmaxf(M, a.pml[(part + s * step) * 2]);
-  float l = 0.0f;
-  f32x4 acc = {0, 0, 0, 0};
-  for (int s = 0; s < it.splits; ++s) {
-    const f32x2 ml = *(const f32x2 *)(a.pml + (part + s * step) * 2);
-    if (ml[1] == 0.0f) continue;
-    const float wgt = fast_exp2(ml[0] - M);
-    l = fmaf(wgt, ml[1], l);
-    const f32x4 os = *(const f32x4 *)(a.po + (part + s * step) * HD + d);
+  for (int rr = r0; rr < rows; rr += ROWS) {
+    const int r = rr + grp / SG;
+    const bool live = r < rows;
+    const int64_t part = ((int64_t)it.part * a.Hk + hk) * a.prows + min(r, rows - 1);
+    float M = kNegFltMax, l = 0.0f;
+    f32x4 acc = {0, 0, 0, 0};
+    auto join = [&](float m1, float l1, f32x4 o1) {
+      if (l1 == 0.0f) return;
+      const float m_new = fmaxf(M, m1);
+      const float w0 = fast_exp2(M - m_new), w1 = fast_exp2(m1 - m_new);
+      l = l * w0 + l1 * w1;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) acc[k] = fmaf(wgt, os[k], acc[k]);
+      for (int k = 0; k < 4; ++k) acc[k] = acc[k] * w0 + o1[k] * w1;
+      M = m_new;
+    };
+    for (int s = sg; s < it.splits; s += 4 * SG) {
+      f32x2 ml[4];
+      f32x4 os[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t at = part + min(s + i * SG, it.splits - 1) * step;
+        ml[i] = *(const f32x2 *)(a.pml + at * 2);
+        os[i] = *(const f32x4 *)(a.po + at * HD + d);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (s + i * SG < it.splits) join(ml[i][0], ml[i][1], os[i]);
+    }
+    if constexpr (SG > 1) {
+      float *mine = st[threadIdx.x];
+      mine[0] = M;
+      mine[1] = l;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mine[2 + k] = acc[k];
+      __syncthreads();
+    }
+    if (sg == 0 && live) {
+#pragma unroll
+      for (int i = 1; i < SG; ++i) {
+        const float *o = st[threadIdx.x + i * LPR];
+        join(o[0], o[1], f32x4{o[2], o[3], o[4], o[5]});
+      }
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      auto quot = [&](float v) {
+        const float q0 = v * inv;
+        return __builtin_fmaf(__builtin_fmaf(-q0, l, v), inv, q0);
+      };
+      const int row = it.tile * BM + r;
+      const int tok = row / a.group, h = hk * a.group + row - tok * a.group;
+      const int64_t t = it.row0 + tok;
+      *(u32x2 *)(a.o + t * a.os0 + h * a.os1 + d) =
+          u32x2{E::pack2(quot(acc[0]), quot(acc[1])), E::pack2(quot(acc[2]), quot(acc[3]))};
+      if (d == 0 && a.lse) a.lse[t * a.Hq + h] = l > 0.0f ? row_lse(M, l) : -INFINITY;
+    }
+    if constexpr (SG > 1) __syncthreads();  // the states are read before the next rows'
   }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  auto quot = [&](float v) {
-    const float q0 = v * inv;
-    return __builtin_fmaf(__builtin_fmaf(-q0, l, v), inv, q0);
-  };
-  const int tok = row / a.group, h = hk * a.group + row - tok * a.group;
-  const int64_t t = it.row0 + tok;
-  *(u32x2 *)(a.o + t * a.os0 + h * a.os1 + d) =
-      u32x2{E::pack2(quot(acc[0]), quot(acc[1])), E::pack2(quot(acc[2]), quot(acc[3]))};
-  if (d == 0 && a.lse) a.lse[t * a.Hq + h] = l > 0.0f ? row_lse(M, l) : -INFINITY;
 }
 
 // Tiles of one KV head at most: every sequence ends a tile of its own
@@ -631,9 +1084,10 @@ int64_t most_tiles(const PagedAttnLaunch &L) {
   return std::min((rows + (BM - 1) * L.batch) / BM, rows);
 }
 
+// Whether the device may cut keys: a split takes 4 blocks at least, and one
+// sequence of at least 2 kSlots items is never cut (its mean chain is at least
+// half its longest).
 bool may_split(const PagedAttnLaunch &L) {
-  // a split is worth 4 blocks at least, so two need 8; one sequence of at least
-  // 2 kSlots items is never cut (its mean chain is at least half its longest)
   if ((L.seq_kv + BN - 1) / BN < 8) return false;
   const int64_t tiles = L.tokens * (L.heads_q / L.heads_kv) / BM;
   return !(L.batch == 1 && tiles * L.heads_kv >= 2 * kSlots);
@@ -643,15 +1097,55 @@ int64_t part_rows(const PagedAttnLaunch &L) {
   return std::min<int64_t>(BM, L.tokens * (L.heads_q / L.heads_kv));
 }
 
+// Splits of every tile of a batch whose sequences are all alike and of the
+// greatest length (make_plan, on the host)
+int likely_splits(const PagedAttnLaunch &L, int64_t tiles) {
+  const int64_t group = L.heads_q / L.heads_kv, n = (L.tokens + L.batch - 1) / L.batch;
+  const int blocks = (int)((L.seq_kv + BN - 1) / BN);
+  const uint64_t work =
+      half_blocks(tiles, (int)n, (int)L.seq_kv, blocks) * (uint64_t)(L.batch * L.heads_kv);
+  const float rows = (float)(L.tokens * group) * (float)L.heads_kv / (float)BM;
+  const int one = chain_of(work, kSlots), two = chain_of(work, 2 * kSlots);
+  const int n1 = splits_of(blocks, one, rows), n2 = splits_of(blocks, two, rows);
+  return splits_of(blocks, choose_chain(one, two, (blocks + n1 - 1) / n1, (blocks + n2 - 1) / n2),
+                   rows);
+}
+
+// Items of cut tiles per KV head that a launch has work-groups and room for:
+// those of the like batch, and kSlots over all heads at least, so that a few
+// long sequences among many short ones can be cut
+int64_t most_parts(const PagedAttnLaunch &L) {
+  if (!may_split(L)) return 0;
+  const int64_t group = L.heads_q / L.heads_kv, n = (L.tokens + L.batch - 1) / L.batch;
+  const int64_t tiles = (n * group + BM - 1) / BM;
+  const int64_t splits = likely_splits(L, tiles);
+  const int64_t likely = splits > 1 ? tiles * L.batch * (splits + 1) : 0;
+  const int64_t most = most_tiles(L) * ((L.seq_kv + BN - 1) / BN / 4);
+  return std::min(most, std::min(std::max(likely, kSlots / L.heads_kv), kParts / L.heads_kv));
+}
+
 template <class E, int HD, bool FP8>
 hipError_t launch_t(const PagedArgs &a, const PagedAttnLaunch &L, hipStream_t s) {
   const int64_t tiles = most_tiles(L);
-  const int64_t items = (tiles + (a.parts ? kParts / L.heads_kv : 0)) * L.heads_kv;
-  hipLaunchKernelGGL((attn_paged<E, HD, FP8>), dim3((unsigned)items), dim3(NT), 0, s, a);
+  hipLaunchKernelGGL((attn_paged<E, HD, FP8>), dim3((unsigned)((tiles + a.parts) * L.heads_kv)),
+                     dim3(NT), 0, s, a);
   if (a.parts) {
-    constexpr int ROWS = NT / (HD / 4);
-    const dim3 grid((unsigned)(tiles * L.heads_kv), (unsigned)((a.prows + ROWS - 1) / ROWS));
-    hipLaunchKernelGGL((attn_paged_combine<E, HD>), grid, dim3(NT), 0, s, a);
+    auto combine = [&](auto G) {
+      constexpr int SG = decltype(G)::value;
+      constexpr int ROWS = NT / (HD / 4) / SG;
+      // rows of cut tiles at most; runs of them, short ones (a wait for memory
+      // each) as long as the GPU holds the work-groups at once
+      const int64_t rows = std::min<int64_t>(L.tokens * a.group, (int64_t)a.parts / 2 * BM);
+      int take = ROWS;
+      auto runs = [&]() { return (rows + (int64_t)(take - 1) * L.batch) / take; };
+      while (take < BM && runs() * L.heads_kv > 2048) take *= 2;
+      hipLaunchKernelGGL((attn_paged_combine<E, HD, SG>), dim3((unsigned)(runs() * L.heads_kv)),
+                         dim3(NT), 0, s, a, take);
+    };
+    if (a.parts >= 8 * tiles)
+      combine(std::integral_constant<int, 8>{});
+    else
+      combine(std::integral_constant<int, 1>{});
   }
   return hipGetLastError();
 }
@@ -688,8 +1182,7 @@ bool attn_paged_supported(const PagedAttnLaunch &L, const char **why) {
 }
 
 size_t attn_paged_bytes(const PagedAttnLaunch &L) {
-  if (!may_split(L)) return 0;
-  const size_t parts = (size_t)(kParts / L.heads_kv + 1) * L.heads_kv;
+  const size_t parts = (size_t)most_parts(L) * L.heads_kv;
   return parts * part_rows(L) * (L.head_dim + 2) * 4;
 }
 
@@ -720,10 +1213,10 @@ hipError_t launch_attn_paged(const PagedAttnLaunch &L, hipStream_t s) {
   a.npages = (int32_t)L.num_pages;
   a.ps16 = (int32_t)(L.page_size / 16);
   a.ps16_inv = 0xffffffffu / (uint32_t)a.ps16;
-  a.parts = may_split(L) ? 1 : 0;
+  a.parts = (int32_t)most_parts(L);
   a.prows = (int32_t)part_rows(L);
   a.po = (float *)L.workspace;
-  a.pml = a.po + (size_t)(kParts / L.heads_kv + 1) * L.heads_kv * a.prows * L.head_dim;
+  a.pml = a.po + (size_t)a.parts * L.heads_kv * a.prows * L.head_dim;
   a.scale2 = L.scale_log2;
   if (L.fp8)
     return L.head_dim == 64 ? launch_t<Bf16Tag, 64, true>(a, L, s)

@@ -89,6 +89,32 @@ def test_long_tables_of_small_pages():
         check_attention(cache, q, o, lse)
 
 
+@pytest.mark.parametrize("D,kt", [(64, BF16), (128, BF16), (64, FP8), (128, FP8)], ids=str)
+@pytest.mark.parametrize("new", [2, 40])
+def test_whole_chains_over_small_pages(new, D, kt):
+    """A chain of thousands of keys in one work-group, window after window of
+    the block table: beside a prompt so large that no keys are cut."""
+    cache = Cache([(new, 4501), (8700, 8700)], 1, D, 16, kt, seed=6)
+    q = _q(cache, 16, BF16)
+    o, lse = _run(cache, q)
+    cache.batch = [(new, 4501)]
+    check_attention(cache, q[:new], o[:new], lse[:new])
+
+
+@pytest.mark.parametrize("new", [1, 3, 8, 9, 31, 32, 33, 40])
+@pytest.mark.parametrize("D,qt,kt", [(64, F16, F16), (128, BF16, BF16), (64, BF16, FP8),
+                                     (128, BF16, FP8)], ids=str)
+def test_few_rows(new, D, qt, kt):
+    """Tiles around the 32 rows of the narrow form, whole and cut, and a chunk's
+    last few rows."""
+    for group, batch in ((1, [(new, new + 7), (new, 100), (new, 31), (new, 2000)]),
+                         (4, [(new, new), (new, 777)]), (1, [(128 + new, 500)])):
+        cache = Cache(batch, 2, D, 32, kt, seed=new)
+        q = _q(cache, 2 * group, qt)
+        o, lse = _run(cache, q)
+        check_attention(cache, q, o, lse)
+
+
 @pytest.mark.parametrize("n", [63, 64, 65, 200])
 def test_many_sequences(n):
     """Around and past a wave's 64 sequences, some with no new token."""
