@@ -11,13 +11,23 @@
 // D/8 lanes hold a row, eight elements each. Lane l of the rotated part holds
 // both sides of pairs 4l .. 4l+3, so a rotation never leaves the lane: two
 // 4-element runs R/2 apart, or eight neighbours interleaved, with one float4 of
-// cos and of sin either way. Consecutive groups of lanes take consecutive heads
-// of a token, so a wave reads whole heads side by side. A group takes HPG heads
-// of its token, all loaded before the first is used: the token's table row,
-// position and page are then looked up once for them.
+// cos and of sin either way. Weights and angles make two factors per element, once
+// for a token: z_e = r (y_e P_e + y_partner Q_e), r the row's 1 / rms.
 //
-// Bound: HBM for prompts, the chain of dependent loads (sequence, length, table
-// row) and the launch for single tokens.
+// A group of lanes takes HPG heads of one token, all loaded before the first is
+// used; position, page, angles and factors are then worked out once for them.
+// Neighbouring groups take neighbouring heads of the token, and a work-group's rows
+// are all queries, all keys or all values, so bases, strides and weights are
+// scalar. HPG 4 where that leaves work-groups for every CU, else 1.
+//
+// Bound: HBM for prompts, the chain of dependent loads (sequence, length, page or
+// angles) and the launch below. Measured (us; a copy of as many bytes): 16384
+// tokens of 32 + 8 bf16 heads with norms 66 (62), 15000 tokens into a token-major
+// cache 46 (42), 16 tokens 2.8 and 32 tokens appended 3.1 (an empty copy 2.0).
+// Factors per element, scalar bases by operand and the rows' loads behind the
+// chain's first brought them from 104, 67, 2.9 and 3.3.
+#include <type_traits>
+
 #include "device_common.h"
 #include "kernels.h"
 
@@ -32,6 +42,15 @@ struct F32Elem {
   static constexpr int SIZE = 4;
   __device__ static inline f32x4 load(raw r) { return r; }
   __device__ static inline raw store(f32x4 x) { return x; }
+  // two neighbouring runs
+  __device__ static inline void load8(const char *p, raw &a, raw &b) {
+    a = *(const raw *)p;
+    b = *(const raw *)(p + 16);
+  }
+  __device__ static inline void store8(char *p, raw a, raw b) {
+    *(raw *)p = a;
+    *(raw *)(p + 16) = b;
+  }
 };
 template <class E>
 struct Elem16 {
@@ -44,23 +63,44 @@ struct Elem16 {
   __device__ static inline raw store(f32x4 x) {
     return raw{E::pack2(x[0], x[1]), E::pack2(x[2], x[3])};
   }
+  __device__ static inline void load8(const char *p, raw &a, raw &b) {
+    const u32x4 v = *(const u32x4 *)p;
+    a = raw{v[0], v[1]};
+    b = raw{v[2], v[3]};
+  }
+  __device__ static inline void store8(char *p, raw a, raw b) {
+    *(u32x4 *)p = u32x4{a[0], a[1], b[0], b[1]};
+  }
+};
+
+// One operand: rows in, rows out (keys and values of an append: the pool)
+struct RopeSide {
+  const char *in;
+  char *out;
+  const float *w, *scales;  // norm weight; scales of an E4M3 pool (nullable)
+  int64_t is[3], os[3];     // byte strides (batch, head, token); pool (page, head, place)
+  int32_t heads, runs;      // runs: groups of lanes per token
+  uint32_t runs_inv;
+  uint32_t first;           // the operand's first work-group
 };
 
 struct RopeArgs {
-  const char *q, *k, *v;
-  char *qo, *ko, *vo;  // append: ko and vo are the pools
-  const float *qw, *kw, *cos, *sin;
-  const int32_t *pos;                       // qk_norm_rope: position of each token
-  const int32_t *cu, *lens, *btab;          // append
-  const float *ksc, *vsc;                   // E4M3 pools
-  // byte strides (batch, head, token); of a pool (page, head, place)
-  int64_t qs[3], ks[3], vs[3], qos[3], kos[3], vos[3];
-  int32_t Hq, Hk, heads;                    // heads: all rows of a token
-  int32_t S, tokens, runs;                  // runs: groups of lanes per token
-  int32_t half, P, interleaved;             // pairs rotated, table rows
+  RopeSide side[3];  // queries, keys, values (append)
+  const float *cos, *sin;
+  const int32_t *pos;              // qk_norm_rope: position of each token
+  const int32_t *cu, *lens, *btab; // append
+  int32_t S, tokens;
+  uint32_t S_inv;
+  int32_t half, P, interleaved;    // pairs rotated, table rows
   int32_t B, ps, maxp, npages;
   float eps, inv_dim;
 };
+
+// floor(x / d), inv = floor((2^32 - 1) / d): the estimate is that or one less
+__device__ inline uint32_t divide(uint32_t x, uint32_t d, uint32_t inv) {
+  const uint32_t q = __umulhi(x, inv);
+  return x - q * d >= d ? q + 1 : q;
+}
 
 // sum over aligned groups of N (4, 8 or 16) lanes, in every lane: DPP moves
 template <int N>
@@ -77,59 +117,87 @@ __device__ inline float group_sum(float x) {
   return x;
 }
 
-// four E4M3 codes of x / scale: nearest even, saturated (a NaN keeps its code;
-// the instruction turns what passes 448 into NaN, so it is cut off first). A
-// page of scale 0 holds zeros.
-__device__ inline uint32_t codes4(f32x4 x, float scale) {
-  float y[4];
+// Eight E4M3 codes of x / scale (inv = 1 / scale, cut to the largest float):
+// nearest even, saturated (the instruction turns what passes 448 into NaN, so it
+// is cut off first, by a minimum that would also swallow a NaN: where the values'
+// sum is not finite, each is looked at). A page of scale 0 holds zeros.
+__device__ inline u32x2 codes8(f32x4 a, f32x4 b, float scale, float inv) {
+  float y[8], sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    y[i] = scale == 0.0f ? 0.0f : x[i] / scale;
-    y[i] = y[i] > 448.0f ? 448.0f : y[i];
-    y[i] = y[i] < -448.0f ? -448.0f : y[i];
+  for (int i = 0; i < 8; ++i) {
+    y[i] = scale == 0.0f ? 0.0f : (i < 4 ? a[i & 3] : b[i & 3]) * inv;
+    sum += y[i];
   }
-  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
+  if (__any(!(fabsf(sum) <= 3.4e38f))) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      y[i] = y[i] > 448.0f ? 448.0f : y[i];
+      y[i] = y[i] < -448.0f ? -448.0f : y[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __builtin_amdgcn_fmed3f(y[i], -448.0f, 448.0f);
+  }
+  u32x2 c;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
+    c[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], lo, true);
+  }
+  return c;
 }
 
-template <class E, int D, bool APPEND, bool FP8, int HPG>
-__global__ __launch_bounds__(NT) void norm_rope(RopeArgs a) {
+// KIND: 0 queries, 1 keys, 2 values
+template <class E, int D, bool APPEND, bool FP8, int HPG, int KIND>
+__device__ inline void rows(const RopeArgs &a) {
   typedef typename E::raw raw;
   constexpr int LPR = D / 8;
+  constexpr bool TO_POOL = APPEND && KIND > 0;
   const int lane = threadIdx.x & 63, l = threadIdx.x % LPR;
-  const uint32_t gid = blockIdx.x * (NT / LPR) + threadIdx.x / LPR;
-  const int at = (int)(gid / (uint32_t)a.runs), run = (int)(gid - (uint32_t)at * a.runs);
+  const RopeSide &x = a.side[KIND];
+  const uint32_t gid = (blockIdx.x - x.first) * (NT / LPR) + threadIdx.x / LPR;
+  const int at = (int)divide(gid, x.runs, x.runs_inv), run = (int)gid - at * x.runs;
   const int tok = min(at, a.tokens - 1);
   bool live = at < a.tokens;
 
-  // this lane's two runs of four elements, the rotated ones' pairs 4l ..
-  const bool turns = 4 * l < a.half;
-  const int offa = turns && !a.interleaved ? 4 * l : 8 * l;
-  const int offb = turns && !a.interleaved ? 4 * l + a.half : 8 * l + 4;
-  const int64_t t0 = APPEND ? 0 : tok / a.S, t1 = APPEND ? tok : tok - (int)t0 * a.S;
-  auto source = [&](int h) {
-    const char *base = h < a.Hq ? a.q : h < a.Hq + a.Hk ? a.k : a.v;
-    const int64_t *st = h < a.Hq ? a.qs : h < a.Hq + a.Hk ? a.ks : a.vs;
-    const int hh = h < a.Hq ? h : h < a.Hq + a.Hk ? h - a.Hq : h - a.Hq - a.Hk;
-    return base + t0 * st[0] + hh * st[1] + t1 * st[2];
-  };
+  // An append's chain to the token's place and slot begins here; the rows are
+  // loaded behind its first link, so that they arrive while it is followed. (The
+  // one link of a plain rotation does better behind the rows: 76 / 82 us, 16384
+  // tokens, one head a group.)
+  const int t0 = APPEND ? 0 : (int)divide(tok, a.S, a.S_inv), t1 = APPEND ? tok : tok - t0 * a.S;
+  int t, page = -1, place = 0, end = 0x7fffffff;
+  if constexpr (APPEND)
+    if (a.cu && lane < a.B) end = a.cu[lane + 1];
+
+  // this lane's two runs of four elements, the rotated ones' pairs 4l ..; flat: all
+  // lanes' runs are neighbours
+  const bool flat = KIND == 2 || a.interleaved || a.half == 0;
+  const bool turns = KIND < 2 && 4 * l < a.half;
+  const int offa = turns && !flat ? 4 * l : 8 * l;
+  const int offb = turns && !flat ? 4 * l + a.half : 8 * l + 4;
+  const char *src = x.in + (APPEND ? 0 : t0 * x.is[0]) + t1 * x.is[2];
   raw xa[HPG], xb[HPG];
+  auto row_in = [&](int i) { return src + min(run + i * x.runs, x.heads - 1) * x.is[1]; };
+  if (flat) {
 #pragma unroll
-  for (int i = 0; i < HPG; ++i) {
-    const char *p = source(min(run + i * a.runs, a.heads - 1));
-    xa[i] = *(const raw *)(p + offa * E::SIZE);
-    xb[i] = *(const raw *)(p + offb * E::SIZE);
+    for (int i = 0; i < HPG; ++i) E::load8(row_in(i) + 8 * E::SIZE * l, xa[i], xb[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < HPG; ++i) {
+      xa[i] = *(const raw *)(row_in(i) + offa * E::SIZE);
+      xb[i] = *(const raw *)(row_in(i) + offb * E::SIZE);
+    }
   }
 
-  // the token's position, and its slot in the cache
-  int t, page = -1, place = 0;
+  float scale[HPG];
+  if constexpr (!APPEND) t = a.pos[tok];
   if constexpr (APPEND) {
     int b = tok, left = 1;
     if (a.cu) {
       // the sequence: as many ends lie at or before the row
       b = 0;
       for (int j = 0; j < a.B; j += 64) {
-        const int end = j + lane < a.B ? a.cu[j + lane + 1] : 0x7fffffff;
+        if (j) end = j + lane < a.B ? a.cu[j + lane + 1] : 0x7fffffff;
 #pragma unroll
         for (int g = 0; g < 64 / LPR; ++g) {
           const int other = __builtin_amdgcn_readlane(tok, g * LPR);
@@ -142,82 +210,120 @@ __global__ __launch_bounds__(NT) void norm_rope(RopeArgs a) {
       left = a.cu[b + 1] - tok;
     }
     t = a.lens[b] - left;
-    const int index = (int)((uint32_t)max(t, 0) / (uint32_t)a.ps);
-    place = max(t, 0) - index * a.ps;
-    if (t >= 0 && index < a.maxp) page = a.btab[(int64_t)b * a.maxp + index];
-  } else {
-    t = a.pos[tok];
+    if constexpr (KIND > 0) {
+      const int index = (int)((uint32_t)max(t, 0) / (uint32_t)a.ps);
+      place = max(t, 0) - index * a.ps;
+      if (t >= 0 && index < a.maxp) page = a.btab[(int64_t)b * a.maxp + index];
+      // a key or value without a slot is not stored
+      live = live && page >= 0 && page < a.npages;
+      if constexpr (FP8)
+#pragma unroll
+        for (int i = 0; i < HPG; ++i)
+          scale[i] = live ? x.scales[(int64_t)page * x.heads + min(run + i * x.runs, x.heads - 1)]
+                          : 0.0f;
+    }
   }
-  f32x4 c = {1, 1, 1, 1}, s = {0, 0, 0, 0};
-  if (turns) {
-    const int64_t row = (int64_t)min(max(t, 0), a.P - 1) * a.half + 4 * l;
-    c = *(const f32x4 *)(a.cos + row);
-    s = *(const f32x4 *)(a.sin + row);
-  }
-  const bool stored = APPEND && page >= 0 && page < a.npages;
 
+  // the factors of the lane's elements, and of their partners: the other run's
+  // element, or (interleaved) the neighbour
+  f32x4 pa = {1, 1, 1, 1}, pb = {1, 1, 1, 1}, qa = {0, 0, 0, 0}, qb = {0, 0, 0, 0};
+  if constexpr (KIND < 2) {
+    // all four loads are in flight before the first is waited for
+    f32x4 c = pa, s = qa;
+    if (a.half) {
+      const int64_t row = (int64_t)min(max(t, 0), a.P - 1) * a.half + min(4 * l, a.half - 4);
+      c = *(const f32x4 *)(a.cos + row);
+      s = *(const f32x4 *)(a.sin + row);
+    }
+    if (x.w) {
+      pa = *(const f32x4 *)(x.w + offa);
+      pb = *(const f32x4 *)(x.w + offb);
+    }
+    asm volatile("" : "+v"(c), "+v"(s), "+v"(pa), "+v"(pb));
+    if (turns) {
+      if (a.interleaved) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          qa[2 * j] = -pa[2 * j + 1] * s[j];
+          qa[2 * j + 1] = pa[2 * j] * s[j];
+          qb[2 * j] = -pb[2 * j + 1] * s[2 + j];
+          qb[2 * j + 1] = pb[2 * j] * s[2 + j];
+          pa[2 * j] *= c[j];
+          pa[2 * j + 1] *= c[j];
+          pb[2 * j] *= c[2 + j];
+          pb[2 * j + 1] *= c[2 + j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          qa[j] = -pb[j] * s[j];
+          qb[j] = pa[j] * s[j];
+          pa[j] *= c[j];
+          pb[j] *= c[j];
+        }
+      }
+    }
+  }
+
+  char *dst = TO_POOL ? x.out + page * x.os[0] + place * x.os[2]
+                                 : x.out + (APPEND ? 0 : t0 * x.os[0]) + t1 * x.os[2];
 #pragma unroll
   for (int i = 0; i < HPG; ++i) {
-    const int h = run + i * a.runs;
-    const bool is_q = h < a.Hq, is_v = APPEND && h >= a.Hq + a.Hk;
+    const int h = run + i * x.runs;
     f32x4 ya = E::load(xa[i]), yb = E::load(xb[i]);
-    if (!is_v) {
-      const float *w = is_q ? a.qw : a.kw;
-      if (w) {
+    if constexpr (KIND < 2) {  // values pass as they are
+      float r = 1.0f;
+      if (x.w) {
         float ss = 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) ss = fmaf(ya[j], ya[j], fmaf(yb[j], yb[j], ss));
-        const float r = 1.0f / sqrtf(fmaf(group_sum<LPR>(ss), a.inv_dim, a.eps));
-        const f32x4 wa = *(const f32x4 *)(w + offa), wb = *(const f32x4 *)(w + offb);
+        // v_rsq_f32: 1 ulp
+        r = __builtin_amdgcn_rsqf(fmaf(group_sum<LPR>(ss), a.inv_dim, a.eps));
+      }
+      f32x4 za, zb;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          ya[j] = ya[j] * r * wa[j];
-          yb[j] = yb[j] * r * wb[j];
+      for (int j = 0; j < 4; ++j) {
+        // (a selection, not a branch: elements behind rot_dim have no partner)
+        const float oa = a.interleaved ? ya[j ^ 1] : yb[j], ob = a.interleaved ? yb[j ^ 1] : ya[j];
+        za[j] = ya[j] * pa[j];
+        zb[j] = yb[j] * pb[j];
+        if (turns) {
+          za[j] = fmaf(oa, qa[j], za[j]);
+          zb[j] = fmaf(ob, qb[j], zb[j]);
         }
       }
-      if (turns) {
-        f32x4 za, zb;
-        if (a.interleaved) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            za[2 * j] = ya[2 * j] * c[j] - ya[2 * j + 1] * s[j];
-            za[2 * j + 1] = ya[2 * j + 1] * c[j] + ya[2 * j] * s[j];
-            zb[2 * j] = yb[2 * j] * c[2 + j] - yb[2 * j + 1] * s[2 + j];
-            zb[2 * j + 1] = yb[2 * j + 1] * c[2 + j] + yb[2 * j] * s[2 + j];
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            za[j] = ya[j] * c[j] - yb[j] * s[j];
-            zb[j] = yb[j] * c[j] + ya[j] * s[j];
-          }
-        }
-        ya = za;
-        yb = zb;
-      }
+      ya = za * r;
+      yb = zb * r;
     }
-    if (!live || h >= a.heads) continue;
-    if (APPEND && !is_q) {
-      if (!stored) continue;
-      const int hh = is_v ? h - a.Hq - a.Hk : h - a.Hq;
-      const int64_t *st = is_v ? a.vos : a.kos;
-      char *p = (is_v ? a.vo : a.ko) + page * st[0] + hh * st[1] + place * st[2];
-      if constexpr (FP8) {
-        const float scale = (is_v ? a.vsc : a.ksc)[(int64_t)page * a.Hk + hh];
-        *(uint32_t *)(p + offa) = codes4(ya, scale);
-        *(uint32_t *)(p + offb) = codes4(yb, scale);
+    if (!live || h >= x.heads) continue;
+    char *p = dst + h * x.os[1];
+    if constexpr (FP8 && TO_POOL) {
+      const u32x2 c = codes8(ya, yb, scale[i], fminf(1.0f / scale[i], 3.4e38f));
+      if (flat) {
+        *(u32x2 *)(p + 8 * l) = c;
+      } else {
+        *(uint32_t *)(p + offa) = c[0];
+        *(uint32_t *)(p + offb) = c[1];
+      }
+    } else {
+      if (flat) {
+        E::store8(p + 8 * E::SIZE * l, E::store(ya), E::store(yb));
       } else {
         *(raw *)(p + offa * E::SIZE) = E::store(ya);
         *(raw *)(p + offb * E::SIZE) = E::store(yb);
       }
-    } else {
-      const int hh = is_q ? h : h - a.Hq;
-      const int64_t *st = is_q ? a.qos : a.kos;
-      char *p = (is_q ? a.qo : a.ko) + t0 * st[0] + hh * st[1] + t1 * st[2];
-      *(raw *)(p + offa * E::SIZE) = E::store(ya);
-      *(raw *)(p + offb * E::SIZE) = E::store(yb);
     }
   }
+}
+
+template <class E, int D, bool APPEND, bool FP8, int HPG>
+__global__ __launch_bounds__(NT) void norm_rope(RopeArgs a) {
+  if (blockIdx.x < a.side[1].first)
+    rows<E, D, APPEND, FP8, HPG, 0>(a);
+  else if (!APPEND || blockIdx.x < a.side[2].first)
+    rows<E, D, APPEND, FP8, HPG, 1>(a);
+  else if constexpr (APPEND)
+    rows<E, D, APPEND, FP8, HPG, 2>(a);
 }
 
 template <class E, int D, bool APPEND, bool FP8>
@@ -225,12 +331,28 @@ hipError_t launch_hpg(RopeArgs a, hipStream_t s) {
   constexpr int GPB = NT / (D / 8);  // groups of lanes per work-group
   auto go = [&](auto H) {
     constexpr int HPG = decltype(H)::value;
-    a.runs = (a.heads + HPG - 1) / HPG;
-    const int64_t groups = (int64_t)a.tokens * a.runs;
-    hipLaunchKernelGGL((norm_rope<E, D, APPEND, FP8, HPG>), dim3((unsigned)((groups + GPB - 1) / GPB)),
-                       dim3(NT), 0, s, a);
+    uint32_t blocks = 0;
+    for (int i = 0; i < (APPEND ? 3 : 2); ++i) {
+      RopeSide &x = a.side[i];
+      x.first = blocks;
+      if (!x.heads) continue;
+      x.runs = (x.heads + HPG - 1) / HPG;
+      x.runs_inv = 0xffffffffu / (uint32_t)x.runs;
+      blocks += (uint32_t)(((int64_t)a.tokens * x.runs + GPB - 1) / GPB);
+    }
+    hipLaunchKernelGGL((norm_rope<E, D, APPEND, FP8, HPG>), dim3(blocks), dim3(NT), 0, s, a);
   };
-  go(std::integral_constant<int, 1>{});
+  // Several heads a group spare it most of its instructions, but leave fewer
+  // work-groups: from 8 for every CU on. Measured (us, 1 / 2 / 4 / 8 heads): 16384
+  // tokens of 32 + 8 heads 75 / 70 / 66 / 64; of 16 + 4 head_dim-64 heads 18.7 /
+  // 16.1 / 15.0 / 14.2; 2000 tokens of 32 + 8 11.1 / 10.4 / 9.8 / 10.9; 1300 into
+  // E4M3 pages 10.6 / 9.3 / 9.4 / 10.4; below, 500 tokens 4.3 / 4.2 / 4.9 / 5.5; 16
+  // 2.75 / 2.9 / 3.4 / 4.4.
+  const int64_t heads = a.side[0].heads + (APPEND ? 2 : 1) * (int64_t)a.side[1].heads;
+  if (a.tokens * heads >= 2048 * GPB)
+    go(std::integral_constant<int, 4>{});
+  else
+    go(std::integral_constant<int, 1>{});
   return hipGetLastError();
 }
 
@@ -284,24 +406,24 @@ bool rope_supported(const RopeLaunch &L, const char **why) {
 }
 
 hipError_t launch_rope(const RopeLaunch &L, hipStream_t s) {
-  RopeArgs a;
+  RopeArgs a = {};
   const int64_t size = L.dtype == 0 ? 4 : 2, kv = L.fp8 ? 1 : size;
-  a.q = (const char *)L.q; a.k = (const char *)L.k; a.v = (const char *)L.v;
-  a.qo = (char *)L.qo; a.ko = (char *)L.ko; a.vo = (char *)L.vo;
-  a.qw = L.q_weight; a.kw = L.k_weight; a.cos = L.cos; a.sin = L.sin;
-  a.pos = L.positions; a.cu = L.cu_seqlens; a.lens = L.seq_lens; a.btab = L.block_table;
-  a.ksc = L.k_scales; a.vsc = L.v_scales;
+  a.side[0] = {(const char *)L.q, (char *)L.qo, L.q_weight, nullptr};
+  a.side[1] = {(const char *)L.k, (char *)L.ko, L.k_weight, L.k_scales};
+  a.side[2] = {(const char *)L.v, (char *)L.vo, nullptr, L.v_scales};
+  const int64_t *const in[3] = {L.qs, L.ks, L.vs}, *const out[3] = {L.qos, L.kos, L.vos};
   for (int i = 0; i < 3; ++i) {
-    a.qs[i] = L.qs[i] * size; a.ks[i] = L.ks[i] * size; a.vs[i] = L.vs[i] * size;
-    a.qos[i] = L.qos[i] * size;
-    a.kos[i] = L.kos[i] * (L.append ? kv : size);
-    a.vos[i] = L.vos[i] * kv;
+    a.side[i].heads = (int32_t)(i ? L.heads_kv : L.heads_q);
+    for (int j = 0; j < 3; ++j) {
+      a.side[i].is[j] = in[i][j] * size;
+      a.side[i].os[j] = out[i][j] * (L.append && i ? kv : size);
+    }
   }
-  a.Hq = (int32_t)L.heads_q;
-  a.Hk = (int32_t)L.heads_kv;
-  a.heads = a.Hq + (L.append ? 2 : 1) * a.Hk;
+  a.cos = L.cos; a.sin = L.sin;
+  a.pos = L.positions; a.cu = L.cu_seqlens; a.lens = L.seq_lens; a.btab = L.block_table;
   a.S = (int32_t)L.seq;
   a.tokens = (int32_t)(L.batch * L.seq);
+  a.S_inv = 0xffffffffu / (uint32_t)a.S;
   a.half = (int32_t)(L.rot_dim / 2);
   a.P = (int32_t)L.table_len;
   a.interleaved = L.interleaved;
