@@ -25,6 +25,7 @@
 // work-group's four waves; the K scale meets the scores, the V scale P before
 // its rounding.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "attn_tile.h"
@@ -48,22 +49,22 @@ struct PagedArgs {
   int64_t ktok, vtok;             // place, bytes
   int32_t T, B, Hq, Hk, group, Lmax, maxp, npages;
   int32_t ps16;                   // page size in runs of 16 tokens
-  uint32_t ps16_inv;              // floor((2^32 - 1) / ps16)
+  uint32_t ps16_inv, group_inv, Hk_inv;  // floor((2^32 - 1) / ..), for quotient()
   int32_t parts;                  // items of cut tiles per KV head at most (0: none is cut)
   int32_t prows;                  // rows of a split item's states
   float scale2;
 };
 
-// run / ps16 and the rest, exactly: the estimate is the quotient or one less
+// floor(x / d), inv = floor((2^32 - 1) / d): the estimate is that or one less
+__device__ inline int quotient(int x, int d, uint32_t inv) {
+  const uint32_t q = __umulhi((uint32_t)x, inv);
+  return (int)((uint32_t)x - q * (uint32_t)d >= (uint32_t)d ? q + 1 : q);
+}
+
+// run / ps16 and the rest
 __device__ inline void page_of(const PagedArgs &a, int run, int *index, int *rest) {
-  int q = (int)__umulhi((uint32_t)run, a.ps16_inv);
-  int r = run - q * a.ps16;
-  if (r >= a.ps16) {
-    ++q;
-    r -= a.ps16;
-  }
-  *index = q;
-  *rest = r;
+  *index = quotient(run, a.ps16, a.ps16_inv);
+  *rest = run - *index * a.ps16;
 }
 
 // Inclusive sum over the wave's lanes of non-negative x (max: the running
@@ -104,16 +105,21 @@ struct Seq {
   int n, row0, len, tiles, blocks;
 };
 __device__ inline Seq sequence(const PagedArgs &a, int b) {
-  Seq s = {0, 0, 0, 0, 0};
-  if (b < a.B) {
-    const int lo = a.cu ? min(max(a.cu[b], 0), a.T) : b;
-    const int hi = a.cu ? min(max(a.cu[b + 1], lo), a.T) : b + 1;
-    s.n = hi - lo;
-    s.row0 = lo;
-    s.len = min(max(a.lens[b], 0), a.Lmax);
-    s.tiles = (s.n * a.group + BM - 1) / BM;
-    s.blocks = (s.len + BN - 1) / BN;
+  const int i = min(b, a.B - 1);
+  int len = a.lens[i], lo = i, hi = i + 1;
+  if (a.cu) {
+    lo = a.cu[i];
+    hi = a.cu[i + 1];
   }
+  asm volatile("" : "+v"(len), "+v"(lo), "+v"(hi));  // all three in flight at once
+  lo = min(max(lo, 0), a.T);
+  hi = min(max(hi, lo), a.T);
+  Seq s;
+  s.n = b < a.B ? hi - lo : 0;
+  s.row0 = lo;
+  s.len = b < a.B ? min(max(len, 0), a.Lmax) : 0;
+  s.tiles = (s.n * a.group + BM - 1) / BM;
+  s.blocks = (s.len + BN - 1) / BN;
   return s;
 }
 
@@ -124,13 +130,27 @@ __device__ inline Seq sequence(const PagedArgs &a, int b) {
 // reading the states of all rows (rows: full tiles of the launch; 128 rows of
 // states are 133 KB, a block some 1.65 us, memory 5 TB/s): least at n =
 // sqrt(62 blocks / rows), and no cut where that takes longer than the whole.
-__host__ __device__ inline int splits_of(int blocks, int chain, float rows) {
-  int n = blocks / (chain > 4 ? chain : 4);
-  const int best = (int)sqrtf(62.0f * (float)blocks / rows);
-  n = n < best ? n : best;
+inline int splits_of(int blocks, int chain, float rows) {
+  int n = std::min(blocks / std::max(chain, 4), (int)std::sqrt(62.0f * (float)blocks / rows));
   if (n < 2) return 1;
   const int per = (blocks + n - 1) / n;
   return (float)(blocks - per - 3) * 62.0f > (float)n * rows ? n : 1;
+}
+// The same on the device, by single operations that every wave of the launch
+// rounds alike (chain_inv: share of the longest chain; rows_inv: 62 / rows). The
+// quotient blocks / chain is never taken too large: its estimate is off by 2^-22
+// of it at most, the factor in chain_inv is 2^-21 less than 1, and the quarter
+// block keeps whole quotients whole up to 2^19 blocks.
+__device__ inline int splits_of(int blocks, float chain_inv, float rows, float rows_inv) {
+  const float x = (float)blocks;
+  const float most = __builtin_amdgcn_sqrtf(x * rows_inv);
+  const float quot = (x + 0.25f) * chain_inv;
+  const float n = floorf(fminf(quot, most));
+  const float per = ceilf(x * __builtin_amdgcn_rcpf(n));
+  return n >= 2.0f && (x - per - 3.0f) * 62.0f > n * rows ? (int)n : 1;
+}
+__device__ inline float inv_chain(int chain) {
+  return __builtin_amdgcn_rcpf((float)max(chain, 4)) * (1.0f - 0x1p-21f);
 }
 
 // The launch's work in half key blocks (a tile's taken as the mean of its
@@ -151,28 +171,26 @@ __host__ __device__ inline int choose_chain(int one, int two, int longest1, int 
 }
 
 struct Plan {
-  int chain;
-  float rows;
-  Seq first;  // of the wave's lane as sequence 0 .. 63
+  float chain_inv, rows, rows_inv;  // of splits_of
+  Seq first;                        // of the wave's lane as sequence 0 .. 63
 };
 
-// Every wave of the launch works the plan out by itself, one sequence per lane,
-// from integers and correctly rounded single operations alone: all agree.
+// Every wave of the launch works the plan out by itself, one sequence per lane.
 __device__ inline Plan make_plan(const PagedArgs &a, int lane) {
   Plan p;
   p.first = sequence(a, lane);
-  p.chain = 0x3fffffff;
-  p.rows = 1.0f;
+  p.chain_inv = p.rows = p.rows_inv = 0.0f;
   if (!a.parts) return p;
   // sums over the launch's tiles: half blocks, blocks (exactly, by 21 bits)
   uint64_t work = 0, whole = 0;
   int rows = 0;
-  for (int b = lane; b < a.B; b += 64) {
-    const Seq s = b < 64 ? p.first : sequence(a, b);
+  auto add = [&](const Seq &s) {
     work += half_blocks(s.tiles, s.n, s.len, s.blocks);
     whole += (uint64_t)s.tiles * (uint32_t)s.blocks;
     rows += s.n * a.group;
-  }
+  };
+  add(p.first);
+  for (int b0 = 64; b0 < a.B; b0 += 64) add(sequence(a, b0 + lane));
   auto sum64 = [](uint64_t x) {
     return (uint64_t)wave_total((int)(x & 0x1fffff)) +
            ((uint64_t)wave_total((int)((x >> 21) & 0x1fffff)) << 21) +
@@ -180,21 +198,26 @@ __device__ inline Plan make_plan(const PagedArgs &a, int lane) {
   };
   const uint64_t total = sum64(work);
   whole = sum64(whole);
-  p.rows = (float)wave_total(rows) * (float)a.Hk / (float)BM;
+  p.rows = (float)wave_total(rows) * (float)a.Hk * (1.0f / BM);
+  p.rows_inv = 62.0f * __builtin_amdgcn_rcpf(p.rows);
   const int one = chain_of(total * (uint32_t)a.Hk, kSlots);
   const int two = chain_of(total * (uint32_t)a.Hk, 2 * kSlots);
+  const float inv1 = inv_chain(one), inv2 = inv_chain(two);
   int longest1 = 0, longest2 = 0;
-  for (int b = lane; b < a.B; b += 64) {
-    const Seq s = b < 64 ? p.first : sequence(a, b);
-    if (!s.n) continue;
-    const int n1 = splits_of(s.blocks, one, p.rows), n2 = splits_of(s.blocks, two, p.rows);
-    longest1 = max(longest1, (s.blocks + n1 - 1) / n1);
-    longest2 = max(longest2, (s.blocks + n2 - 1) / n2);
-  }
-  // blocks / chain items come of a tile at most, so this many keep to a.parts
-  const uint64_t least = (whole + (uint32_t)a.parts - 1) / (uint32_t)a.parts;
+  auto longest = [&](const Seq &s) {
+    const float x = s.n ? (float)s.blocks : 0.0f;
+    const float n1 = (float)splits_of(s.blocks, inv1, p.rows, p.rows_inv);
+    const float n2 = (float)splits_of(s.blocks, inv2, p.rows, p.rows_inv);
+    longest1 = max(longest1, (int)ceilf(x * __builtin_amdgcn_rcpf(n1)));
+    longest2 = max(longest2, (int)ceilf(x * __builtin_amdgcn_rcpf(n2)));
+  };
+  longest(p.first);
+  for (int b0 = 64; b0 < a.B; b0 += 64) longest(sequence(a, b0 + lane));
+  // blocks / chain items come of a tile at most, so this many (whole / parts,
+  // rounded up) keep to a.parts
+  const float least = (float)whole * __builtin_amdgcn_rcpf((float)a.parts) * (1.0f + 0x1p-20f);
   const int chosen = choose_chain(one, two, wave_total<true>(longest1), wave_total<true>(longest2));
-  p.chain = max(chosen, (int)(least > 0x3fffffff ? 0x3fffffff : least));
+  p.chain_inv = inv_chain(max(chosen, (int)fminf(ceilf(least), 0x1p30f)));
   return p;
 }
 
@@ -207,10 +230,10 @@ __device__ inline bool find_item(const PagedArgs &a, const Plan &p, int lane, in
   int base = 0, parts = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const Seq s = b0 ? sequence(a, b0 + lane) : p.first;
-    const int sp = a.parts ? splits_of(s.blocks, p.chain, p.rows) : 1;
+    const int sp = a.parts ? splits_of(s.blocks, p.chain_inv, p.rows, p.rows_inv) : 1;
     const int mparts = sp > 1 ? s.tiles * sp : 0;
     const int mine = take ? (sp > 1 ? (s.n * a.group + take - 1) / take : 0) : s.tiles * sp;
-    const int sum = wave_scan(mine), psum = wave_scan(mparts);
+    const int sum = wave_scan(mine), psum = a.parts ? wave_scan(mparts) : 0;
     const uint64_t past = __ballot(base + sum > idx);
     if (past) {
       const int at = __builtin_ctzll(past);
@@ -223,7 +246,9 @@ __device__ inline bool find_item(const PagedArgs &a, const Plan &p, int lane, in
       it->splits = of(sp);
       const int rest = idx - (base + of(sum) - of(mine));
       // tiles before this one in the items' order
-      const int down = take ? it->tiles - 1 - rest * take / BM : rest / it->splits;
+      const int down = take             ? it->tiles - 1 - rest * take / BM
+                       : it->splits > 1 ? rest / it->splits
+                                        : rest;
       it->tile = it->tiles - 1 - down;
       it->split = take ? rest * take % BM : rest - down * it->splits;
       it->part = parts + of(psum) - of(mparts) + down * it->splits;
@@ -285,10 +310,10 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
   const int off = it.len - it.n, base_row = it.tile * BM;
   const int rows = min(it.n * a.group - base_row, NARROW);
   const int row = base_row + min(lq, rows - 1);
-  const int tok = row / a.group, hr = row - tok * a.group;
+  const int tok = quotient(row, a.group, a.group_inv), hr = row - tok * a.group;
   const int pos = off + tok;
-  const int lo = __builtin_amdgcn_readfirstlane(off + base_row / a.group);
-  const int last = off + (base_row + rows - 1) / a.group;  // the last row's place
+  const int lo = __builtin_amdgcn_readfirstlane(off + quotient(base_row, a.group, a.group_inv));
+  const int last = off + quotient(base_row + rows - 1, a.group, a.group_inv);  // the last row's place
   // the wave's steps of the item's
   const int s0 = 2 * kb0, s1 = min(2 * (kb0 + nv), last < 0 ? 0 : last / STEP + 1);
   const int share = (max(s1 - s0, 0) + 3) >> 2;
@@ -570,9 +595,8 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
 
   // kv heads fastest: with a multiple of 8 of them, id % 8 (the XCD) fixes the
   // head modulo 8 and the tiles of a head share an L2
-  const int hk = __builtin_amdgcn_readfirstlane((int)(blockIdx.x % (uint32_t)a.Hk));
   const Plan plan = make_plan(a, lane);
-  const int idx = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / (uint32_t)a.Hk));
+  const int idx = quotient((int)blockIdx.x, a.Hk, a.Hk_inv), hk = (int)blockIdx.x - idx * a.Hk;
   Item it;
   if (!find_item(a, plan, lane, idx, 0, &it)) return;
   const int rows = it.n * a.group;
@@ -581,15 +605,15 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
 
   // this lane's row: query head hk * group + hr of token tok, at place pos
   const int row = r0 + lq;
-  const int tok = min(row, rows - 1) / a.group, hr = min(row, rows - 1) - tok * a.group;
+  const int tok = quotient(min(row, rows - 1), a.group, a.group_inv), hr = min(row, rows - 1) - tok * a.group;
   const int pos = off + tok;
   // blocks seen by rows up to r: through the place of its token
   auto blocks_to = [&](int r) {
-    const int last = off + min(r, rows - 1) / a.group;
+    const int last = off + quotient(min(r, rows - 1), a.group, a.group_inv);
     return last < 0 ? 0 : last / BN + 1;
   };
   const int all = blocks_to(it.tile * BM + BM - 1);
-  const int per = (all + it.splits - 1) / it.splits;
+  const int per = it.splits > 1 ? (all + it.splits - 1) / it.splits : all;
   const int kb0 = __builtin_amdgcn_readfirstlane(it.split * per);
   const int nv = __builtin_amdgcn_readfirstlane(min(max(all - kb0, 0), per));
   if (rows - it.tile * BM <= NARROW) {
@@ -598,7 +622,7 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   }
   const int nkw = __builtin_amdgcn_readfirstlane(
       r0 < rows ? min(max(blocks_to(r0 + 31) - kb0, 0), nv) : 0);
-  const int lo_w = __builtin_amdgcn_readfirstlane(off + min(r0, rows - 1) / a.group);
+  const int lo_w = __builtin_amdgcn_readfirstlane(off + quotient(min(r0, rows - 1), a.group, a.group_inv));
 
   const char *kp = a.k + hk * a.kps1, *vp = a.v + hk * a.vps1;
   const int32_t *tab = a.btab + (int64_t)it.b * a.maxp;
@@ -1014,9 +1038,9 @@ __global__ __launch_bounds__(NT) void attn_paged_combine(PagedArgs a, int take) 
   const int lane = threadIdx.x & 63;
   const int grp = threadIdx.x / LPR, sg = grp % SG, d = 4 * (threadIdx.x % LPR);
   const Plan plan = make_plan(a, lane);
-  const uint32_t hk = blockIdx.x % (uint32_t)a.Hk;
+  const int idx = quotient((int)blockIdx.x, a.Hk, a.Hk_inv), hk = (int)blockIdx.x - idx * a.Hk;
   Item it;
-  if (!find_item(a, plan, lane, (int)(blockIdx.x / (uint32_t)a.Hk), take, &it)) return;
+  if (!find_item(a, plan, lane, idx, take, &it)) return;
   const int r0 = it.split;
   const int rows = min(min(it.n * a.group - it.tile * BM, BM), r0 + take);
   const int64_t step = (int64_t)a.Hk * a.prows;
@@ -1068,7 +1092,8 @@ __global__ __launch_bounds__(NT) void attn_paged_combine(PagedArgs a, int take) 
         return __builtin_fmaf(__builtin_fmaf(-q0, l, v), inv, q0);
       };
       const int row = it.tile * BM + r;
-      const int tok = row / a.group, h = hk * a.group + row - tok * a.group;
+      const int tok = quotient(row, a.group, a.group_inv);
+      const int h = hk * a.group + row - tok * a.group;
       const int64_t t = it.row0 + tok;
       *(u32x2 *)(a.o + t * a.os0 + h * a.os1 + d) =
           u32x2{E::pack2(quot(acc[0]), quot(acc[1])), E::pack2(quot(acc[2]), quot(acc[3]))};
@@ -1213,6 +1238,8 @@ hipError_t launch_attn_paged(const PagedAttnLaunch &L, hipStream_t s) {
   a.npages = (int32_t)L.num_pages;
   a.ps16 = (int32_t)(L.page_size / 16);
   a.ps16_inv = 0xffffffffu / (uint32_t)a.ps16;
+  a.group_inv = 0xffffffffu / (uint32_t)a.group;
+  a.Hk_inv = 0xffffffffu / (uint32_t)a.Hk;
   a.parts = (int32_t)most_parts(L);
   a.prows = (int32_t)part_rows(L);
   a.po = (float *)L.workspace;
