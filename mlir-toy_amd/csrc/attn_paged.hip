@@ -25,7 +25,6 @@
 // work-group's four waves; the K scale meets the scores, the V scale P before
 // its rounding.
 #include <algorithm>
-#include <cmath>
 #include <type_traits>
 
 #include "attn_tile.h"
@@ -35,7 +34,8 @@ namespace neptune {
 namespace {
 
 constexpr int kSlots = 512;         // two work-groups on each of 256 CUs
-constexpr int kParts = 4 * kSlots;  // split items a launch makes at most (make_plan)
+constexpr int kParts = 2 * kSlots;  // items of cut tiles in a launch at most (make_plan)
+constexpr int NARROW = 32;          // rows up to which a tile takes the narrow form
 
 struct PagedArgs {
   const uint16_t *q;
@@ -50,7 +50,8 @@ struct PagedArgs {
   int32_t T, B, Hq, Hk, group, Lmax, maxp, npages;
   int32_t ps16;                   // page size in runs of 16 tokens
   uint32_t ps16_inv, group_inv, Hk_inv;  // floor((2^32 - 1) / ..), for quotient()
-  int32_t parts;                  // items of cut tiles per KV head at most (0: none is cut)
+  int32_t items, slots, parts;    // per KV head: work-groups, those of one round, items of
+                                  // cut tiles at most (0: no keys are cut)
   int32_t prows;                  // rows of a split item's states
   float scale2;
 };
@@ -67,14 +68,11 @@ __device__ inline void page_of(const PagedArgs &a, int run, int *index, int *res
   *rest = run - *index * a.ps16;
 }
 
-// Inclusive sum over the wave's lanes of non-negative x (max: the running
-// maximum), by DPP moves
-template <bool MAX = false>
+// Inclusive sum over the wave's lanes, by DPP moves
 __device__ inline int wave_scan(int x) {
   auto step = [&](auto ctrl, auto rows) {
-    const int y = __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value,
-                                              0xf, false);
-    x = MAX ? max(x, y) : x + y;
+    x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xf,
+                                     false);
   };
   typedef std::integral_constant<int, 0xf> all;
   step(std::integral_constant<int, 0x111>{}, all{});  // row_shr 1, 2, 4, 8
@@ -85,10 +83,7 @@ __device__ inline int wave_scan(int x) {
   step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // row_bcast 31
   return x;
 }
-template <bool MAX = false>
-__device__ inline int wave_total(int x) {
-  return __builtin_amdgcn_readlane(wave_scan<MAX>(x), 63);
-}
+__device__ inline int wave_total(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
 struct Item {
   int b, n, row0;   // sequence, its new tokens, its first row of q
@@ -125,49 +120,24 @@ __device__ inline Seq sequence(const PagedArgs &a, int b) {
 
 // The cut of the keys. A work-group's time is its chain of key blocks, and a
 // launch's at least its blocks over kSlots work-groups, so chains longer than
-// that (chain) are cut. A tile of n splits takes blocks / n + 3 + n rows / 62
+// that (make_plan) are cut. A tile of n splits takes blocks / n + 3 + n rows / 62
 // blocks of time, the latter two for the combine's launch and for writing and
 // reading the states of all rows (rows: full tiles of the launch; 128 rows of
 // states are 133 KB, a block some 1.65 us, memory 5 TB/s): least at n =
 // sqrt(62 blocks / rows), and no cut where that takes longer than the whole.
-inline int splits_of(int blocks, int chain, float rows) {
-  int n = std::min(blocks / std::max(chain, 4), (int)std::sqrt(62.0f * (float)blocks / rows));
-  if (n < 2) return 1;
-  const int per = (blocks + n - 1) / n;
-  return (float)(blocks - per - 3) * 62.0f > (float)n * rows ? n : 1;
-}
-// The same on the device, by single operations that every wave of the launch
-// rounds alike (chain_inv: share of the longest chain; rows_inv: 62 / rows). The
-// quotient blocks / chain is never taken too large: its estimate is off by 2^-22
-// of it at most, the factor in chain_inv is 2^-21 less than 1, and the quarter
-// block keeps whole quotients whole up to 2^19 blocks.
-__device__ inline int splits_of(int blocks, float chain_inv, float rows, float rows_inv) {
+// rows_inv: 62 / rows. The quotient blocks / chain is cut to a whole number (a
+// quarter block keeps whole ones whole), but for a tile of few rows rounded to
+// one: those wait for memory, and more of them side by side help (24 x 12 heads,
+// 1 over 7300: 185 / 214 us).
+// (Uncontracted, so that every wave of both kernels rounds alike.)
+__device__ inline int splits_of(int blocks, bool few, float chain_inv, float rows, float rows_inv) {
+#pragma clang fp contract(off)
   const float x = (float)blocks;
   const float most = __builtin_amdgcn_sqrtf(x * rows_inv);
   const float quot = (x + 0.25f) * chain_inv;
-  const float n = floorf(fminf(quot, most));
+  const float n = floorf(fminf(few && quot >= 1.5f ? quot + 0.5f : quot, most));
   const float per = ceilf(x * __builtin_amdgcn_rcpf(n));
   return n >= 2.0f && (x - per - 3.0f) * 62.0f > n * rows ? (int)n : 1;
-}
-__device__ inline float inv_chain(int chain) {
-  return __builtin_amdgcn_rcpf((float)max(chain, 4)) * (1.0f - 0x1p-21f);
-}
-
-// The launch's work in half key blocks (a tile's taken as the mean of its
-// sequence's first and last tile's) over `slots` work-groups, rounded up.
-__host__ __device__ inline int chain_of(uint64_t half_blocks, int slots) {
-  const uint64_t c = (half_blocks + 2 * slots - 1) / (2 * slots);
-  return c > 0x3fffffff ? 0x3fffffff : (int)c;
-}
-__host__ __device__ inline uint64_t half_blocks(int64_t tiles, int n, int len, int blocks) {
-  const int first = len - n + 1 > 0 ? (len - n + BN) / BN : 0;
-  return (uint64_t)tiles * (uint32_t)(blocks + (first < blocks ? first : blocks));
-}
-// Items for one round of kSlots, or shorter ones for two where the longest of
-// one round would outlast them: a round's lengths differ by up to a factor of
-// two, and only a second one fills up behind the short ones.
-__host__ __device__ inline int choose_chain(int one, int two, int longest1, int longest2) {
-  return longest1 <= one + longest2 / 2 ? one : two;
 }
 
 struct Plan {
@@ -175,50 +145,68 @@ struct Plan {
   Seq first;                        // of the wave's lane as sequence 0 .. 63
 };
 
-// Every wave of the launch works the plan out by itself, one sequence per lane.
+// The plan of a launch, by every wave for itself, one sequence per lane. The chain
+// starts at the launch's blocks (a tile's taken as the mean of its sequence's first
+// and last tile's) over kSlots work-groups and grows until the items fit: into one
+// round of the GPU where the tiles themselves do, else into the launch's
+// work-groups, and in any case into the room for states. One round of items that
+// differ by up to a factor of two in length did better than two of half as long
+// ones wherever tried (8 mixed E4M3 sequences 97 / 120 us, 1 over 32768 28.8 / 31.7,
+// 500 over 7000 71 / 98), and a few items more than one round cost nearly a second
+// (16 x 1-4 over 8000, 520 items 77, 512 at most 68). Where growing would leave a
+// quarter of the GPU idle, the first chain stands if its items are at most 4/3 of a
+// round (24 x 12 heads: 576 items 185, 288 items 214).
 __device__ inline Plan make_plan(const PagedArgs &a, int lane) {
+#pragma clang fp contract(off)
   Plan p;
   p.first = sequence(a, lane);
   p.chain_inv = p.rows = p.rows_inv = 0.0f;
   if (!a.parts) return p;
-  // sums over the launch's tiles: half blocks, blocks (exactly, by 21 bits)
-  uint64_t work = 0, whole = 0;
-  int rows = 0;
+  uint64_t work = 0;  // half blocks
+  int rows = 0, tiles = 0;
   auto add = [&](const Seq &s) {
-    work += half_blocks(s.tiles, s.n, s.len, s.blocks);
-    whole += (uint64_t)s.tiles * (uint32_t)s.blocks;
+    const int first = max(s.len - s.n + BN, 0) / BN;
+    work += (uint64_t)s.tiles * (uint32_t)(s.blocks + min(first, s.blocks));
     rows += s.n * a.group;
+    tiles += s.tiles;
   };
   add(p.first);
   for (int b0 = 64; b0 < a.B; b0 += 64) add(sequence(a, b0 + lane));
-  auto sum64 = [](uint64_t x) {
-    return (uint64_t)wave_total((int)(x & 0x1fffff)) +
-           ((uint64_t)wave_total((int)((x >> 21) & 0x1fffff)) << 21) +
-           ((uint64_t)wave_total((int)(x >> 42)) << 42);
-  };
-  const uint64_t total = sum64(work);
-  whole = sum64(whole);
+  // (exactly, by 21 bits)
+  const uint64_t total = (uint64_t)wave_total((int)(work & 0x1fffff)) +
+                         ((uint64_t)wave_total((int)((work >> 21) & 0x1fffff)) << 21) +
+                         ((uint64_t)wave_total((int)(work >> 42)) << 42);
+  tiles = wave_total(tiles);
   p.rows = (float)wave_total(rows) * (float)a.Hk * (1.0f / BM);
   p.rows_inv = 62.0f * __builtin_amdgcn_rcpf(p.rows);
-  const int one = chain_of(total * (uint32_t)a.Hk, kSlots);
-  const int two = chain_of(total * (uint32_t)a.Hk, 2 * kSlots);
-  const float inv1 = inv_chain(one), inv2 = inv_chain(two);
-  int longest1 = 0, longest2 = 0;
-  auto longest = [&](const Seq &s) {
-    const float x = s.n ? (float)s.blocks : 0.0f;
-    const float n1 = (float)splits_of(s.blocks, inv1, p.rows, p.rows_inv);
-    const float n2 = (float)splits_of(s.blocks, inv2, p.rows, p.rows_inv);
-    longest1 = max(longest1, (int)ceilf(x * __builtin_amdgcn_rcpf(n1)));
-    longest2 = max(longest2, (int)ceilf(x * __builtin_amdgcn_rcpf(n2)));
-  };
-  longest(p.first);
-  for (int b0 = 64; b0 < a.B; b0 += 64) longest(sequence(a, b0 + lane));
-  // blocks / chain items come of a tile at most, so this many (whole / parts,
-  // rounded up) keep to a.parts
-  const float least = (float)whole * __builtin_amdgcn_rcpf((float)a.parts) * (1.0f + 0x1p-20f);
-  const int chosen = choose_chain(one, two, wave_total<true>(longest1), wave_total<true>(longest2));
-  p.chain_inv = inv_chain(max(chosen, (int)fminf(ceilf(least), 0x1p30f)));
-  return p;
+  const uint64_t even = (total * (uint32_t)a.Hk + 2 * kSlots - 1) / (2 * kSlots);
+  const int chain0 = (int)min(max(even, (uint64_t)4), (uint64_t)1 << 25);
+  int chain = chain0;
+  bool fits = false, first_fits = false;
+  while (true) {
+    p.chain_inv = __builtin_amdgcn_rcpf((float)chain);
+    int items = 0, parts = 0;
+    auto count = [&](const Seq &s) {
+      const int sp =
+          splits_of(s.blocks, s.n * a.group <= NARROW, p.chain_inv, p.rows, p.rows_inv);
+      items += s.tiles * sp;
+      parts += sp > 1 ? s.tiles * sp : 0;
+    };
+    count(p.first);
+    for (int b0 = 64; b0 < a.B; b0 += 64) count(sequence(a, b0 + lane));
+    items = wave_total(items);
+    const bool room = items <= a.items && wave_total(parts) <= a.parts;
+    if (fits) return p;  // back at the first chain
+    if (chain == chain0) first_fits = room;
+    // past 2^25 blocks, longer than any sequence, nothing is cut
+    fits = chain >= 1 << 25 || (room && (tiles >= a.slots || items <= a.slots));
+    if (fits) {
+      if (chain == chain0 || !first_fits || 4 * items >= 3 * a.slots) return p;
+      chain = chain0;
+    } else {
+      chain += max(chain >> 3, 1);
+    }
+  }
 }
 
 // Item idx of one KV head, false if there is none. Sequences in order, a
@@ -230,7 +218,8 @@ __device__ inline bool find_item(const PagedArgs &a, const Plan &p, int lane, in
   int base = 0, parts = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const Seq s = b0 ? sequence(a, b0 + lane) : p.first;
-    const int sp = a.parts ? splits_of(s.blocks, p.chain_inv, p.rows, p.rows_inv) : 1;
+    const int sp = a.parts ? splits_of(s.blocks, s.n * a.group <= NARROW, p.chain_inv, p.rows, p.rows_inv)
+                           : 1;
     const int mparts = sp > 1 ? s.tiles * sp : 0;
     const int mine = take ? (sp > 1 ? (s.n * a.group + take - 1) / take : 0) : s.tiles * sp;
     const int sum = wave_scan(mine), psum = a.parts ? wave_scan(mparts) : 0;
@@ -270,6 +259,81 @@ __device__ inline u32x2 widen4(uint32_t c) {
   return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
 }
 
+// Infinities and NaN of V behind the mask. A masked key's p is 0, but 0 times them
+// is NaN, and a matrix product cannot leave a key out for some of its rows. So in
+// blocks that any row of a tile does not see whole, V is looked over in LDS before
+// its use, such values (hardly ever: a new token whose V overflowed) become 0, and
+// the rows that do see them have them added at the end (add_special). All-ones
+// exponents (E4M3: all-ones magnitudes) carry into the bit above them.
+template <class E, bool FP8>
+struct Special {
+  static constexpr uint32_t ONES = FP8 ? 0x7f7f7f7fu
+                                       : std::is_same<E, Bf16Tag>::value ? 0x7f807f80u : 0x7c007c00u;
+  static constexpr uint32_t UNIT = FP8 ? 0x01010101u
+                                       : std::is_same<E, Bf16Tag>::value ? 0x00800080u : 0x04000400u;
+  static constexpr uint32_t TOP = FP8 ? 0x80808080u : 0x80008000u;
+  __device__ static inline uint32_t marks(uint32_t x) { return ((x & ONES) + UNIT) & TOP; }
+  __device__ static inline uint32_t marks(u32x4 x) {
+    return marks(x[0]) | marks(x[1]) | marks(x[2]) | marks(x[3]);
+  }
+  __device__ static inline u32x4 without(u32x4 x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t m = marks(x[i]);
+      x[i] &= ~(FP8 ? (m >> 7) * 0xffu : (m >> 15) * 0xffffu);
+    }
+    return x;
+  }
+  // takes them out of N KiB of LDS; whether there were any
+  template <int N>
+  __device__ static inline bool scrub(const uint8_t *p, int lane) {
+    u32x4 *at = (u32x4 *)p + lane;
+    u32x4 x[N];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = at[64 * i];
+#pragma unroll
+    for (int i = 0; i < N; ++i) m |= marks(x[i]);
+    const bool found = __any(m != 0);
+    if (__builtin_expect(found, 0)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) at[64 * i] = without(x[i]);
+    }
+    return found;
+  }
+};
+
+// o (element 4 rq + e of o[nb]: head_dim 32 nb + 8 rq + 4 g + e) += the special
+// values of V's keys lo .. hi - 1 up to the row's place
+template <class E, int HD, bool FP8>
+__device__ inline void add_special(const PagedArgs &a, const Item &it, int hk, int lo, int hi,
+                                   int pos, int g, f32x16 (&o)[HD / 32]) {
+  const int32_t *tab = a.btab + (int64_t)it.b * a.maxp;
+#pragma unroll 1
+  for (int j = lo; j < hi; ++j) {
+    int index, rest;
+    page_of(a, j >> 4, &index, &rest);
+    const int page = min(max(tab[index], 0), a.npages - 1);
+    const char *v = a.v + hk * a.vps1 + page * a.vps0 + (int64_t)(rest * 16 + (j & 15)) * a.vtok;
+#pragma unroll
+    for (int nb = 0; nb < HD / 32; ++nb)
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        const int d = 32 * nb + 8 * rq + 4 * g;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x;
+          if constexpr (FP8)
+            x = (((const uint8_t *)v)[d + e] & 0x7f) == 0x7f ? __builtin_nanf("") : 0.0f;
+          else
+            x = E::to_f32(((const uint16_t *)v)[d + e]);
+          if (j <= pos && !(fabsf(x) <= 3.4e38f)) o[nb][4 * rq + e] += x;
+        }
+        __builtin_amdgcn_sched_barrier(0);  // few registers at a time
+      }
+  }
+}
+
 // A tile of at most 32 rows (generated or guessed tokens, a chunk's last few): the
 // wide form would compute in one wave of four and hold 32 KB in flight between
 // barriers, and such an item is bound by memory. Here the four waves share out
@@ -280,8 +344,6 @@ __device__ inline u32x2 widen4(uint32_t c) {
 // LDS and are widened as operands are read. The running max moves with every
 // step, so a row's largest p is 1. At the end the waves' states merge in LDS, a
 // quarter of the head_dim each.
-constexpr int NARROW = 32;
-
 template <class E, int HD, bool FP8>
 __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, int w, int lane,
                                    int kb0, int nv, const uint8_t *smem, f32x2 *mlbox) {
@@ -407,6 +469,7 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
       copy_v(decltype(J)::value);
     }
   });
+  bool special = false;
   // waits until the copies issued after a tile are all that is in flight: `pairs`
   // whole steps' (at most N - 1) and X tiles
   auto wait_tiles = [&](int pairs, auto extra) {
@@ -463,7 +526,8 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] *= a.scale2;
     }
-    if (key0 + STEP - 1 > lo) {
+    const bool masked = key0 + STEP - 1 > lo;
+    if (masked) {
       const int lim = pos - key0 - 4 * g;  // element r holds key 4 g + 8 (r >> 2) + (r & 3)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
@@ -490,39 +554,46 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
       for (int j = 0; j < 4; ++j) {
         const float p0 = fast_exp2(s[8 * c + 2 * j] - m), p1 = fast_exp2(s[8 * c + 2 * j + 1] - m);
         lsum += p0 + p1;
-        pf[c][j] = FP8 ? E::pack2(p0 * vs[c], p1 * vs[c]) : E::pack2(p0, p1);
+        // (a masked key's page may hold any scale)
+        pf[c][j] = FP8 ? E::pack2(p0 == 0.0f ? 0.0f : p0 * vs[c], p1 == 0.0f ? 0.0f : p1 * vs[c])
+                       : E::pack2(p0, p1);
       }
     if (later >= N)
       wait_tiles(N - 1, std::integral_constant<int, 1>{});  // V(i) is there, K(i + N) after it
     else
       wait_tiles(later, std::integral_constant<int, 0>{});
     const uint8_t *vt = vslot(i);
+    auto v_operand = [&](int c, int nb) {
+      const int s16 = lane & 15, dh = (lane >> 4) & 1;
+      if constexpr (FP8) {
+        // lane pair (2 j, 2 j + 1) of 16 names the row of k-slot j
+        const int j = s16 >> 1, r = 16 * c + 4 * g + (j & 3) + 8 * (j >> 2);
+        const v2i32 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i32 *)as_lds(
+            vt + r * RB + (((2 * nb + dh) ^ vswz(r)) << 4) + 8 * (s16 & 1)));
+        const u32x2 y = widen4((uint32_t)x[0]), z = widen4((uint32_t)x[1]);
+        return u32x4{y[0], y[1], z[0], z[1]};
+      } else {
+        const int j = s16 >> 2, r = 16 * c + 4 * g + j;
+        const uint8_t *p = vt + r * RB + (((4 * nb + 2 * dh) ^ vswz(j)) << 4) + 8 * (s16 & 3);
+        const u32x2 y = __builtin_bit_cast(u32x2, lds_read_tr16(p));
+        const u32x2 z = __builtin_bit_cast(u32x2, lds_read_tr16(p + 8 * RB));
+        return u32x4{y[0], y[1], z[0], z[1]};
+      }
+    };
+    // (all rows of one place see alike: masked keys are then the last one again)
+    if (masked && last > lo) special |= Special<E, FP8>::template scrub<CH>(vt, lane);
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        u32x4 A;
-        const int s16 = lane & 15, dh = (lane >> 4) & 1;
-        if constexpr (FP8) {
-          // lane pair (2 j, 2 j + 1) of 16 names the row of k-slot j
-          const int j = s16 >> 1, r = 16 * c + 4 * g + (j & 3) + 8 * (j >> 2);
-          const v2i32 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i32 *)as_lds(
-              vt + r * RB + (((2 * nb + dh) ^ vswz(r)) << 4) + 8 * (s16 & 1)));
-          const u32x2 y = widen4((uint32_t)x[0]), z = widen4((uint32_t)x[1]);
-          A = u32x4{y[0], y[1], z[0], z[1]};
-        } else {
-          const int j = s16 >> 2, r = 16 * c + 4 * g + j;
-          const uint8_t *p = vt + r * RB + (((4 * nb + 2 * dh) ^ vswz(j)) << 4) + 8 * (s16 & 3);
-          const u32x2 y = __builtin_bit_cast(u32x2, lds_read_tr16(p));
-          const u32x2 z = __builtin_bit_cast(u32x2, lds_read_tr16(p + 8 * RB));
-          A = u32x4{y[0], y[1], z[0], z[1]};
-        }
-        o[nb] = E::mfma32(as_vec8<V8>(A), as_vec8<V8>(pf[c]), o[nb]);
-      }
+      for (int nb = 0; nb < NB; ++nb)
+        o[nb] = E::mfma32(as_vec8<V8>(v_operand(c, nb)), as_vec8<V8>(pf[c]), o[nb]);
     __builtin_amdgcn_s_waitcnt(kWaitLgkm0);  // V(i) has been read
     if (later >= N) copy_v(i + N);
   }
 
+  if (__builtin_expect(special, 0))
+    add_special<E, HD, FP8>(a, it, hk, max(t0 * STEP, lo / STEP * STEP),
+                            min((t0 + ns) * STEP, it.len), pos, g, o);
   // the waves' states, merged lane by lane, NB of a row's 4 NB vectors a wave
   const float ltot = pair_sum(lsum);
   f32x4 *const box = (f32x4 *)mine + lane;
@@ -542,11 +613,7 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
     L = fmaf(wgt[k], ml[1], L);
   }
   if (lq >= rows) return;
-  const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-  auto quot = [&](float v) {
-    const float q0 = v * inv;
-    return __builtin_fmaf(__builtin_fmaf(-q0, L, v), inv, q0);
-  };
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   const int64_t t = it.row0 + tok;
   const int64_t part = ((int64_t)(it.part + it.split) * a.Hk + hk) * a.prows + lq;
 #pragma unroll
@@ -563,13 +630,13 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
       *(f32x4 *)(a.po + part * HD + d) = x;
     else
       *(u32x2 *)(a.o + t * a.os0 + (int64_t)(hk * a.group + hr) * a.os1 + d) =
-          u32x2{E::pack2(quot(x[0]), quot(x[1])), E::pack2(quot(x[2]), quot(x[3]))};
+          u32x2{E::pack2(x[0] * inv, x[1] * inv), E::pack2(x[2] * inv, x[3] * inv)};
   }
   if (w == 0 && g == 0) {
     if (it.splits > 1)
       *(f32x2 *)(a.pml + part * 2) = f32x2{M, L};
     else if (a.lse)
-      a.lse[t * a.Hq + hk * a.group + hr] = L > 0.0f ? row_lse(M, L) : -INFINITY;
+      a.lse[t * a.Hq + hk * a.group + hr] = L == 0.0f ? -INFINITY : row_lse(M, L);
   }
 }
 
@@ -586,6 +653,7 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   // K slots 0 and 1, then V slots 0 and 1; block t uses slot t & 1
   __shared__ __attribute__((aligned(16))) uint8_t smem[65536];
   __shared__ f32x2 mlbox[NT];
+  __shared__ int special[4];  // by wave: V of a masked block held infinities or NaN
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -620,6 +688,7 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
     narrow_item<E, HD, FP8>(a, it, hk, w, lane, kb0, nv, smem, mlbox);
     return;
   }
+  if (lane == 0) special[w] = 0;
   const int nkw = __builtin_amdgcn_readfirstlane(
       r0 < rows ? min(max(blocks_to(r0 + 31) - kb0, 0), nv) : 0);
   const int lo_w = __builtin_amdgcn_readfirstlane(off + quotient(min(r0, rows - 1), a.group, a.group_inv));
@@ -730,6 +799,17 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   auto put_v = [&](int t) {
     if constexpr (FP8) store8(v8, vslot(t), true);
   };
+  // the wave's own rows of a V tile, before the others read them (16-bit pools:
+  // their copy has landed; E4M3: they have been stored)
+  const int lo_tile = __builtin_amdgcn_readfirstlane(
+      off + quotient(it.tile * BM, a.group, a.group_inv));
+  auto scrub_v = [&](int t) {
+    if ((kb0 + t) * BN + BN - 1 <= lo_tile) return;
+    asm volatile("" ::: "memory");  // no read before the copy's wait
+    const bool found =
+        Special<E, false>::template scrub<CHUNKS>(vslot(t) + CHUNKS * w * 1024, lane);
+    if (found && lane == 0) special[w] = 1;
+  };
   if (nv > 0) {
     int index, rest;
     page_of(a, kb0 * (BN / 16), &index, &rest);
@@ -824,6 +904,7 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   };
 
   wait_vmem();
+  if (nv > 0) scrub_v(0);
   __syncthreads();
   if (nkw > 0) qk_from(kslot(0), k_operand(kslot(0), 0), k_operand(kslot(0), 1));
   __syncthreads();  // every wave is done with K slot 0 before it is refilled
@@ -918,7 +999,8 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
               for (int i = 0; i < 4; ++i) {
                 const float p0 = fast_exp2(fmaf(s[c >> 1][8 * (c & 1) + 2 * i], sc, nm));
                 const float p1 = fast_exp2(fmaf(s[c >> 1][8 * (c & 1) + 2 * i + 1], sc, nm));
-                pf[c][i] = E::pack2(p0 * vs[c], p1 * vs[c]);
+                // (a masked key's page may hold any scale)
+                pf[c][i] = E::pack2(p0 == 0.0f ? 0.0f : p0 * vs[c], p1 == 0.0f ? 0.0f : p1 * vs[c]);
               }
           }
         }
@@ -986,10 +1068,14 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
     if (jb + 1 < nv) put_v(jb + 1);
     if (jb + 2 < nv) put_k(jb + 2);
     wait_vmem();
+    if (jb + 1 < nv) scrub_v(jb + 1);
     __syncthreads();
   }
 
   const float ltot = pair_sum(lsum);
+  if (__builtin_expect(special[0] | special[1] | special[2] | special[3], 0))
+    add_special<E, HD, FP8>(a, it, hk, max(kb0, lo_tile / BN) * BN, min((kb0 + nv) * BN, it.len),
+                            pos, g, o);
   if (row >= rows) return;
   if (it.splits > 1) {  // this split's state, for attn_paged_combine
     const int64_t part =
@@ -1006,24 +1092,21 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
     if (g == 0) *(f32x2 *)(a.pml + part * 2) = f32x2{m, ltot};
     return;
   }
-  // O = acc / l, the correctly rounded fp32 quotient, rounded to the input type
-  const float inv = ltot > 0.0f ? 1.0f / ltot : 0.0f;
-  auto quot = [&](float v) {
-    const float q0 = v * inv;
-    return __builtin_fmaf(__builtin_fmaf(-q0, ltot, v), inv, q0);
-  };
+  // O = acc / l, rounded to the input type (by a product: 1.5 ulp of fp32 off at most,
+  // and an infinity stays one)
+  const float inv = ltot == 0.0f ? 0.0f : 1.0f / ltot;
   const int64_t t = it.row0 + tok;
   uint16_t *op = a.o + t * a.os0 + (int64_t)(hk * a.group + hr) * a.os1 + 4 * g;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int rq = 0; rq < 4; ++rq) {
-      const u32x2 pk = {E::pack2(quot(o[nb][4 * rq]), quot(o[nb][4 * rq + 1])),
-                        E::pack2(quot(o[nb][4 * rq + 2]), quot(o[nb][4 * rq + 3]))};
+      const u32x2 pk = {E::pack2(o[nb][4 * rq] * inv, o[nb][4 * rq + 1] * inv),
+                        E::pack2(o[nb][4 * rq + 2] * inv, o[nb][4 * rq + 3] * inv)};
       *(u32x2 *)(op + 32 * nb + 8 * rq) = pk;
     }
   if (g == 0 && a.lse)
-    a.lse[t * a.Hq + hk * a.group + hr] = ltot > 0.0f ? row_lse(m, ltot) : -INFINITY;
+    a.lse[t * a.Hq + hk * a.group + hr] = ltot == 0.0f ? -INFINITY : row_lse(m, ltot);
 }
 
 // Combine of the cut tiles' states: M = max m_s, l = sum 2^(m_s - M) l_s, O = sum
@@ -1086,18 +1169,14 @@ __global__ __launch_bounds__(NT) void attn_paged_combine(PagedArgs a, int take) 
         const float *o = st[threadIdx.x + i * LPR];
         join(o[0], o[1], f32x4{o[2], o[3], o[4], o[5]});
       }
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-      auto quot = [&](float v) {
-        const float q0 = v * inv;
-        return __builtin_fmaf(__builtin_fmaf(-q0, l, v), inv, q0);
-      };
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       const int row = it.tile * BM + r;
       const int tok = quotient(row, a.group, a.group_inv);
       const int h = hk * a.group + row - tok * a.group;
       const int64_t t = it.row0 + tok;
       *(u32x2 *)(a.o + t * a.os0 + h * a.os1 + d) =
-          u32x2{E::pack2(quot(acc[0]), quot(acc[1])), E::pack2(quot(acc[2]), quot(acc[3]))};
-      if (d == 0 && a.lse) a.lse[t * a.Hq + h] = l > 0.0f ? row_lse(M, l) : -INFINITY;
+          u32x2{E::pack2(acc[0] * inv, acc[1] * inv), E::pack2(acc[2] * inv, acc[3] * inv)};
+      if (d == 0 && a.lse) a.lse[t * a.Hq + h] = l == 0.0f ? -INFINITY : row_lse(M, l);
     }
     if constexpr (SG > 1) __syncthreads();  // the states are read before the next rows'
   }
@@ -1110,8 +1189,8 @@ int64_t most_tiles(const PagedAttnLaunch &L) {
 }
 
 // Whether the device may cut keys: a split takes 4 blocks at least, and one
-// sequence of at least 2 kSlots items is never cut (its mean chain is at least
-// half its longest).
+// sequence of at least 2 kSlots tiles is not cut (its mean chain is at least half
+// its longest).
 bool may_split(const PagedAttnLaunch &L) {
   if ((L.seq_kv + BN - 1) / BN < 8) return false;
   const int64_t tiles = L.tokens * (L.heads_q / L.heads_kv) / BM;
@@ -1122,38 +1201,29 @@ int64_t part_rows(const PagedAttnLaunch &L) {
   return std::min<int64_t>(BM, L.tokens * (L.heads_q / L.heads_kv));
 }
 
-// Splits of every tile of a batch whose sequences are all alike and of the
-// greatest length (make_plan, on the host)
-int likely_splits(const PagedAttnLaunch &L, int64_t tiles) {
-  const int64_t group = L.heads_q / L.heads_kv, n = (L.tokens + L.batch - 1) / L.batch;
-  const int blocks = (int)((L.seq_kv + BN - 1) / BN);
-  const uint64_t work =
-      half_blocks(tiles, (int)n, (int)L.seq_kv, blocks) * (uint64_t)(L.batch * L.heads_kv);
-  const float rows = (float)(L.tokens * group) * (float)L.heads_kv / (float)BM;
-  const int one = chain_of(work, kSlots), two = chain_of(work, 2 * kSlots);
-  const int n1 = splits_of(blocks, one, rows), n2 = splits_of(blocks, two, rows);
-  return splits_of(blocks, choose_chain(one, two, (blocks + n1 - 1) / n1, (blocks + n2 - 1) / n2),
-                   rows);
-}
-
-// Items of cut tiles per KV head that a launch has work-groups and room for:
-// those of the like batch, and kSlots over all heads at least, so that a few
-// long sequences among many short ones can be cut
-int64_t most_parts(const PagedAttnLaunch &L) {
-  if (!may_split(L)) return 0;
-  const int64_t group = L.heads_q / L.heads_kv, n = (L.tokens + L.batch - 1) / L.batch;
-  const int64_t tiles = (n * group + BM - 1) / BM;
-  const int64_t splits = likely_splits(L, tiles);
-  const int64_t likely = splits > 1 ? tiles * L.batch * (splits + 1) : 0;
-  const int64_t most = most_tiles(L) * ((L.seq_kv + BN - 1) / BN / 4);
-  return std::min(most, std::min(std::max(likely, kSlots / L.heads_kv), kParts / L.heads_kv));
+// What a launch has room for, per KV head (PagedArgs)
+struct Room {
+  int64_t items, slots, parts;
+};
+Room room_of(const PagedAttnLaunch &L) {
+  Room r;
+  const int64_t tiles = most_tiles(L);
+  r.slots = (kSlots + L.heads_kv - 1) / L.heads_kv;
+  r.items = tiles;
+  r.parts = 0;
+  if (may_split(L)) {
+    const int64_t splits = ((L.seq_kv + BN - 1) / BN + 2) / 4 + 1;  // splits_of at most
+    r.parts = std::min(tiles * splits, std::max<int64_t>(kParts / L.heads_kv, 1));
+    // work-groups without an item cost some 10 us a thousand
+    r.items = std::min(tiles * splits, std::max(tiles + r.slots / 4, r.slots * 4 / 3 + 1));
+  }
+  return r;
 }
 
 template <class E, int HD, bool FP8>
 hipError_t launch_t(const PagedArgs &a, const PagedAttnLaunch &L, hipStream_t s) {
-  const int64_t tiles = most_tiles(L);
-  hipLaunchKernelGGL((attn_paged<E, HD, FP8>), dim3((unsigned)((tiles + a.parts) * L.heads_kv)),
-                     dim3(NT), 0, s, a);
+  hipLaunchKernelGGL((attn_paged<E, HD, FP8>), dim3((unsigned)(a.items * L.heads_kv)), dim3(NT), 0,
+                     s, a);
   if (a.parts) {
     auto combine = [&](auto G) {
       constexpr int SG = decltype(G)::value;
@@ -1167,7 +1237,7 @@ hipError_t launch_t(const PagedArgs &a, const PagedAttnLaunch &L, hipStream_t s)
       hipLaunchKernelGGL((attn_paged_combine<E, HD, SG>), dim3((unsigned)(runs() * L.heads_kv)),
                          dim3(NT), 0, s, a, take);
     };
-    if (a.parts >= 8 * tiles)
+    if (a.items >= 8 * most_tiles(L))
       combine(std::integral_constant<int, 8>{});
     else
       combine(std::integral_constant<int, 1>{});
@@ -1207,7 +1277,7 @@ bool attn_paged_supported(const PagedAttnLaunch &L, const char **why) {
 }
 
 size_t attn_paged_bytes(const PagedAttnLaunch &L) {
-  const size_t parts = (size_t)most_parts(L) * L.heads_kv;
+  const size_t parts = (size_t)room_of(L).parts * L.heads_kv;
   return parts * part_rows(L) * (L.head_dim + 2) * 4;
 }
 
@@ -1240,7 +1310,10 @@ hipError_t launch_attn_paged(const PagedAttnLaunch &L, hipStream_t s) {
   a.ps16_inv = 0xffffffffu / (uint32_t)a.ps16;
   a.group_inv = 0xffffffffu / (uint32_t)a.group;
   a.Hk_inv = 0xffffffffu / (uint32_t)a.Hk;
-  a.parts = (int32_t)most_parts(L);
+  const Room room = room_of(L);
+  a.items = (int32_t)room.items;
+  a.slots = (int32_t)room.slots;
+  a.parts = (int32_t)room.parts;
   a.prows = (int32_t)part_rows(L);
   a.po = (float *)L.workspace;
   a.pml = a.po + (size_t)a.parts * L.heads_kv * a.prows * L.head_dim;

@@ -172,6 +172,43 @@ def test_strided_queries_and_outputs():
     check_attention(cache, q.cpu(), o.cpu(), lse.cpu())
 
 
+@pytest.mark.parametrize("D,qt,kt", [(64, F16, F16), (128, BF16, BF16), (64, BF16, FP8),
+                                     (128, BF16, FP8)], ids=str)
+@pytest.mark.parametrize("n,length", [(5, 5), (8, 200), (60, 100), (200, 333), (3, 2500)])
+def test_masked_places_may_hold_anything(n, length, D, qt, kt):
+    """Infinities and NaN in the keys and values of late tokens: rows before them
+    are as if they were not there, rows that see them show them."""
+    cache = Cache([(n, length)], 2, D, 32, kt, seed=n)
+    at = length - 1 - n // 3  # the first token that holds any
+    bad = [float("inf"), float("-inf"), float("nan")]
+    page, place = int(cache.table[0, at // 32]), at % 32
+    where = {}
+    for i, x in enumerate(bad):
+        x = float("nan") if kt == FP8 else x
+        cache.v[page, 0, place, 7 * i + 3] = x
+        where[7 * i + 3] = x
+    last = int(cache.table[0, (length - 1) // 32])
+    cache.k[last, 1, (length - 1) % 32, 5] = float("nan")  # the last row sees it: NaN all along
+    q = _q(cache, 4, qt)
+    o, lse = _run(cache, q)
+    seen = length - n + torch.arange(n) >= at
+    clean = Cache([(n, length)], 2, D, 32, kt, seed=n)  # the same without them
+    clean_o, clean_lse = _run(clean, q)
+    assert torch.equal(o[~seen], clean_o[~seen])
+    assert torch.equal(lse[:n - 1], clean_lse[:n - 1])
+    rows = seen.nonzero()[:, 0][:-1]  # all but the last
+    for d in range(D):
+        for h in (0, 1):
+            got = o[rows, h, d].float()
+            if d in where:
+                want = torch.full_like(got, where[d])
+                assert torch.equal(torch.isnan(got), torch.isnan(want))
+                assert torch.equal(got[~torch.isnan(got)], want[~torch.isnan(want)])
+            else:
+                assert torch.isfinite(got).all()
+    assert torch.isnan(o[n - 1, 2:]).all() and torch.isnan(lse[n - 1, 2:]).all()
+
+
 def test_scale_and_large_scores():
     """Scores of hundreds: one key takes all of a row's weight."""
     cache = Cache([(50, 400), (2, 900)], 2, 128, 64, BF16, seed=4)
