@@ -751,35 +751,50 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
       }
     }
   };
-  // E4M3 pools: 16 codes per lane and load, two rows' worth of units each
+  // E4M3 pools: 16 codes per lane and load, two 16-byte units of bf16. The rows of
+  // 16 lanes, which one cycle writes to LDS, have units of both parities: K's by
+  // its swizzle, V's by an order of rows that alternates bit 2 and a swizzle that
+  // brings that bit in (without it half the LDS cycles were conflicts)
   constexpr int LPR8 = HD / 16, ROWS8 = 64 / LPR8, N8 = 16 / ROWS8;
+  const int krow8 = lane / LPR8;
+  const int vrow8 = HD == 128 ? krow8 >> 1 | (krow8 & 1) << 2
+                              : (krow8 & 9) | (krow8 & 2) << 1 | (krow8 & 4) >> 1;
+  auto vswz8 = [](int r) { return tile_swizzle<HD, true>(r) | ((r >> 2) & 1); };
   u32x4 k8[N8], v8[N8];
-  auto load8 = [&](const char *base, int64_t tokb, int most, u32x4 *dst) {
+  auto load8 = [&](const char *base, int64_t tokb, int most, int row8, u32x4 *dst) {
 #pragma unroll
     for (int c = 0; c < N8; ++c) {
-      const int r = lane / LPR8 + ROWS8 * c;
+      const int r = row8 + ROWS8 * c;
       dst[c] = *(const u32x4 *)(base + (uint32_t)(min(r, most) * (int)tokb + (lane % LPR8) * 16));
     }
   };
+  // where a lane's first 16 bytes go in a tile; the other half of its codes is the
+  // neighbouring unit, and its second row 8 rows on (K's swizzle then differs in
+  // unit bit 3). Kept as one register each and worked out anew for every tile: the
+  // matrix products need the registers
+  auto place8 = [&](int row8, int z) {
+    return (16 * w + row8) * ROWB + (((2 * (lane % LPR8)) ^ z) << 4);
+  };
+  int kput = place8(krow8, tile_swizzle<HD, false>(16 * w + krow8));
+  int vput = place8(vrow8, vswz8(16 * w + vrow8));
   auto store8 = [&](const u32x4 *src, const uint8_t *tile, bool is_v) {
+    int at = is_v ? vput : kput;
+    asm volatile("" : "+v"(at));
 #pragma unroll
-    for (int c = 0; c < N8; ++c) {
-      const int r = 16 * w + lane / LPR8 + ROWS8 * c, u = 2 * (lane % LPR8);
-      const int z = is_v ? tile_swizzle<HD, true>(r) : tile_swizzle<HD, false>(r);
+    for (int c = 0; c < N8; ++c)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const u32x2 lo = widen4(src[c][2 * h]), hi = widen4(src[c][2 * h + 1]);
-        *(u32x4 *)(uint8_t *)(tile + r * ROWB + (((u + h) ^ z) << 4)) =
+        *(u32x4 *)(uint8_t *)(tile + ROWS8 * c * ROWB + (at ^ (16 * h) ^ (is_v ? 0 : 128 * c))) =
             u32x4{lo[0], lo[1], hi[0], hi[1]};
       }
-    }
   };
   auto load_k = [&](int t) {
     int64_t ko, vo;
     int most;
     run_at(t, &ko, &vo, &most);
     if constexpr (FP8)
-      load8(kp + ko, a.ktok, most, k8);
+      load8(kp + ko, a.ktok, most, krow8, k8);
     else
       copy(kp + ko, koff, a.ktok, most, false, kslot(t));
   };
@@ -788,7 +803,7 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
     int most;
     run_at(t, &ko, &vo, &most);
     if constexpr (FP8)
-      load8(vp + vo, a.vtok, most, v8);
+      load8(vp + vo, a.vtok, most, vrow8, v8);
     else
       copy(vp + vo, voff, a.vtok, most, true, vslot(t));
   };
@@ -798,6 +813,10 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   };
   auto put_v = [&](int t) {
     if constexpr (FP8) store8(v8, vslot(t), true);
+  };
+  auto put_next = [&](int jb) {
+    if (jb + 1 < nv) put_v(jb + 1);
+    if (jb + 2 < nv) put_k(jb + 2);
   };
   // the wave's own rows of a V tile, before the others read them (16-bit pools:
   // their copy has landed; E4M3: they have been stored)
@@ -863,7 +882,9 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
     const int s16 = lane & 15, i = s16 >> 2, q = s16 & 3, dh = (lane >> 4) & 1;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
-      va[nb] = (4 * g + i) * ROWB + (((4 * nb + 2 * dh) ^ tile_swizzle<HD, true>(i)) << 4) + 8 * q;
+      va[nb] = (4 * g + i) * ROWB +
+               (((4 * nb + 2 * dh + (q >> 1)) ^ (tile_swizzle<HD, true>(i) | (FP8 ? g : 0))) << 4) +
+               8 * (q & 1);
   }
 
   f32x16 o[NB];
@@ -881,19 +902,19 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   };
   // S^T of one key block, its first two A operands already read (k0, k1)
   auto qk_from = [&](const uint8_t *kt, const u32x4 &k0, const u32x4 &k1) {
+    // operand reads run three MFMAs ahead. The order is spelled out, not left to
+    // the scheduler, which gave up on it where registers were short: E4M3 pools
+    // then waited for every read (2000 new rows behind 6000, 32 heads of 128 over
+    // 8: 277 us against 257)
+    u32x4 next[4] = {k0, k1, k_operand(kt, 2)};
 #pragma unroll
     for (int i = 0; i < NQK; ++i) {
-      const u32x4 A = i == 0 ? k0 : i == 1 ? k1 : k_operand(kt, i);
-      s[i & 1] = E::mfma32(as_vec8<V8>(A), as_vec8<V8>(qf[i >> 1]), i < 2 ? zero16 : s[i & 1]);
+      if (i + 3 < NQK) next[(i + 3) & 3] = k_operand(kt, i + 3);
+      __builtin_amdgcn_sched_barrier(0);
+      s[i & 1] = E::mfma32(as_vec8<V8>(next[i & 3]), as_vec8<V8>(qf[i >> 1]),
+                           i < 2 ? zero16 : s[i & 1]);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    // the remaining operand reads run two MFMAs ahead
-    __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
-#pragma unroll
-    for (int i = 0; i < NQK - 4; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, 4, 1);
   };
   // The A operand of P.V step st (V^T: head_dim rows 32 nb .., keys 16 c ..)
   auto v_operand = [&](const uint8_t *vt, int st) {
@@ -911,7 +932,8 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
 
   for (int jb = 0; jb < nv; ++jb) {
     // K of block jb + 2 goes to the slot block jb's K has left, V of block
-    // jb + 1 to the slot of block jb - 1's V
+    // jb + 1 to the slot of block jb - 1's V (E4M3: in registers until the softmax
+    // is done, and written then, which the matrix products hide: 247 us against 254)
     if (jb + 1 < nv) load_v(jb + 1);
     if (jb + 2 < nv) load_k(jb + 2);
     if (jb < nkw) {
@@ -1041,33 +1063,27 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
         }
       }
       lsum += rs;
+      if constexpr (FP8) put_next(jb);
 
       // O^T += V^T P^T, then the next block's S^T, at raised issue priority
       __builtin_amdgcn_s_setprio(1);
+      // (reads run two MFMAs ahead, as above; the last are the next block's first two
+      // K operands: past the last block those are stale and dropped)
+      u32x4 next[4] = {vp0, vp1};
 #pragma unroll
       for (int st = 0; st < NPV; ++st) {
-        const u32x4 A = st == 0 ? vp0 : st == 1 ? vp1 : v_operand(vt, st);
-        o[st % NB] = E::mfma32(as_vec8<V8>(A), as_vec8<V8>(pf[st / NB]), o[st % NB]);
+        next[(st + 2) & 3] = st + 2 < NPV ? v_operand(vt, st + 2)
+                                          : k_operand(kslot(jb + 1), st + 2 - NPV);
+        __builtin_amdgcn_sched_barrier(0);
+        o[st % NB] = E::mfma32(as_vec8<V8>(next[st & 3]), as_vec8<V8>(pf[st / NB]), o[st % NB]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      // the next block's first two K operands (past the last block they are stale
-      // and dropped)
-      const u32x4 kn0 = k_operand(kslot(jb + 1), 0), kn1 = k_operand(kslot(jb + 1), 1);
-      // reads run two MFMAs ahead
-      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-      for (int i = 0; i < NPV - 4; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-      if (jb + 1 < nkw) qk_from(kslot(jb + 1), kn0, kn1);
+      if (jb + 1 < nkw) qk_from(kslot(jb + 1), next[NPV & 3], next[(NPV + 1) & 3]);
       __builtin_amdgcn_s_setprio(0);
+    } else if constexpr (FP8) {
+      put_next(jb);
     }
-    if (jb + 1 < nv) put_v(jb + 1);
-    if (jb + 2 < nv) put_k(jb + 2);
-    wait_vmem();
+    if constexpr (!FP8) wait_vmem();
     if (jb + 1 < nv) scrub_v(jb + 1);
     __syncthreads();
   }
