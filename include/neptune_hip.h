@@ -328,8 +328,9 @@ NEPTUNE_API neptune_status neptune_decode_paged_fp8(const neptune_decode_desc *d
  * operand); positions [batch, seq] int32. A position outside the tables is
  * clamped into them (the row is then meaningless). qo may be q and ko k (same
  * pointer and strides); an output that shares bytes with an input in any other
- * way is NEPTUNE_ERR_INVALID_ARGUMENT. head_dim 32, 64 or 128; 16-byte aligned
- * bases and strides of whole 16-byte units. */
+ * way, or with the other output, is NEPTUNE_ERR_INVALID_ARGUMENT (heads side by
+ * side in one buffer share none). head_dim 32, 64 or 128; 16-byte aligned bases
+ * and strides of whole 16-byte units. */
 NEPTUNE_API neptune_status neptune_qk_norm_rope(const neptune_rope_desc *desc, const void *q,
                                     const void *k, const float *q_weight,
                                     const float *k_weight, const float *cos,
@@ -346,7 +347,8 @@ NEPTUNE_API neptune_status neptune_qk_norm_rope(const neptune_rope_desc *desc, c
  * page of scale 0 takes zero codes); NULL otherwise. A row is not stored when its
  * place is negative or past its block table, or the table's entry lies outside
  * [0, num_pages); rows behind cu_seqlens[batch] are neither stored nor written to
- * qo. Two rows sent to one slot leave either. head_dim 64 or 128; 16-byte aligned
+ * qo. Two rows sent to one slot leave either. The pools and qo share no byte with
+ * each other or an input (but qo may be q). head_dim 64 or 128; 16-byte aligned
  * bases and strides of whole 16-byte units. */
 NEPTUNE_API neptune_status neptune_kv_append_paged(
     const neptune_append_desc *desc, const neptune_paged_kv_desc *pages, const void *k,

@@ -464,11 +464,13 @@ size_t span(const int64_t *sizes, const int64_t *strides, int n, int64_t row, in
 }
 
 // A strided tensor of an entry point: its rows' strides resolved (zero:
-// contiguous), its bytes
+// contiguous), their sizes, its bytes
 struct Strided {
   const char *name;
   const void *p;
-  int64_t stride[3];
+  int64_t stride[3], size[3];
+  int n;
+  int64_t dim, esize;
   size_t bytes;
 };
 
@@ -477,6 +479,10 @@ neptune_status resolve(const char *fn, const char *name, const void *p, const in
                        const int64_t *sizes, int n, int64_t dim, int64_t esize, Strided *t) {
   t->name = name;
   t->p = p;
+  t->n = n;
+  t->dim = dim;
+  t->esize = esize;
+  for (int i = 0; i < n; ++i) t->size[i] = sizes[i];
   if (!p) return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: %s must be non-NULL", fn, name);
   bool zero = true;
   for (int i = 0; i < n; ++i) zero = zero && in[i] == 0;
@@ -502,9 +508,58 @@ neptune_status resolve(const char *fn, const char *name, const void *p, const in
   return NEPTUNE_OK;
 }
 
+// Whether rows of two tensors share a byte. Their spans may cross where they do
+// not: heads of q, k and v side by side in one projection. The distance of two
+// rows is delta + sum of x_j step_j with x_j in [lo_j, hi_j] (a step that both
+// tensors take counts once); largest step first, few x_j leave one that the
+// smaller steps can still bring into (-b's row, a's row). Where strides are so
+// tangled that it takes thousands of tries, the answer is yes.
+struct Steps {
+  int n = 0, tries = 0;
+  int64_t step[6];
+  __int128 lo[6], hi[6];
+  __int128 below, above;  // the open interval
+  void add(int64_t by, int64_t first, int64_t last) {
+    int i = 0;
+    while (i < n && step[i] > by) ++i;
+    if (i == n || step[i] != by) {
+      for (int j = n++; j > i; --j) step[j] = step[j - 1], lo[j] = lo[j - 1], hi[j] = hi[j - 1];
+      step[i] = by;
+      lo[i] = hi[i] = 0;
+    }
+    lo[i] += first;
+    hi[i] += last;
+  }
+  bool reach(int j, __int128 at) {
+    if (++tries > 4096) return true;
+    if (j == n) return at > below && at < above;
+    __int128 least = 0, most = 0;  // of the smaller steps
+    for (int i = j + 1; i < n; ++i) least += lo[i] * step[i], most += hi[i] * step[i];
+    const auto floor_div = [](__int128 x, __int128 y) { return x / y - (x % y < 0); };
+    // at + x step + [least, most] meets [below + 1, above - 1]
+    const __int128 first = -floor_div(at + most - below - 1, step[j]);
+    const __int128 last = floor_div(above - 1 - least - at, step[j]);
+    for (__int128 x = first > lo[j] ? first : lo[j]; x <= last && x <= hi[j]; ++x)
+      if (reach(j + 1, at + x * step[j])) return true;
+    return false;
+  }
+};
+
+bool meet(const Strided &a, const Strided &b) {
+  if (!overlaps(a.p, a.bytes, b.p, b.bytes)) return false;
+  Steps s;
+  for (int i = 0; i < a.n; ++i)
+    if (a.size[i] > 1) s.add(a.stride[i] * a.esize, 1 - a.size[i], 0);
+  for (int i = 0; i < b.n; ++i)
+    if (b.size[i] > 1) s.add(b.stride[i] * b.esize, 0, b.size[i] - 1);
+  s.below = -(__int128)(b.dim * b.esize);
+  s.above = a.dim * a.esize;
+  return s.reach(0, (__int128)(uintptr_t)b.p - (__int128)(uintptr_t)a.p);
+}
+
 // out must share no byte with in
 neptune_status apart(const char *fn, const Strided &out, const Strided &in) {
-  if (overlaps(out.p, out.bytes, in.p, in.bytes))
+  if (meet(out, in))
     return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: %s overlaps %s", fn, out.name, in.name);
   return NEPTUNE_OK;
 }
@@ -626,15 +681,12 @@ neptune_status neptune_qk_norm_rope(const neptune_rope_desc *d, const void *q, c
       (st = resolve(fn, "qo", qo, d->qo_stride, sq, 3, d->head_dim, esize, &out[0])) != NEPTUNE_OK ||
       (st = resolve(fn, "ko", ko, d->ko_stride, sk, 3, d->head_dim, esize, &out[1])) != NEPTUNE_OK)
     return st;
-  // in place, q and k may lie head by head in one buffer; an output elsewhere
-  // may meet neither input nor the other output
-  const auto in_place = [&](int i) { return same_place(out[i], in[i], 3); };
-  if (qo == ko) return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: qo overlaps ko", fn);
   for (int i = 0; i < 2; ++i)
-    for (int j = 0; j < 2 && !in_place(i); ++j)
-      if ((st = apart(fn, out[i], in[j])) != NEPTUNE_OK) return st;
-  if (!in_place(0) && !in_place(1) && (st = apart(fn, out[0], out[1])) != NEPTUNE_OK)
-    return st;
+    for (int j = 0; j < 2; ++j)
+      if (!(i == j && same_place(out[i], in[i], 3)) &&
+          (st = apart(fn, out[i], in[j])) != NEPTUNE_OK)
+        return st;
+  if ((st = apart(fn, out[0], out[1])) != NEPTUNE_OK) return st;
   RopeLaunch L;
   L.q = q; L.k = k; L.qo = qo; L.ko = ko;
   L.q_weight = q_weight; L.k_weight = k_weight; L.cos = cos; L.sin = sin; L.positions = positions;
@@ -688,14 +740,16 @@ neptune_status neptune_kv_append_paged(const neptune_append_desc *d,
     if ((st = resolve(fn, "q", q, d->q_stride, sq, 2, d->head_dim, 2, &in[2])) != NEPTUNE_OK ||
         (st = resolve(fn, "qo", qo, d->qo_stride, sq, 2, d->head_dim, 2, &out)) != NEPTUNE_OK)
       return st;
-    for (int j = 0; j < 3 && !same_place(out, in[2], 2); ++j)
-      if ((st = apart(fn, out, in[j])) != NEPTUNE_OK) return st;
+    for (int j = 0; j < 3; ++j)
+      if (!(j == 2 && same_place(out, in[2], 2)) && (st = apart(fn, out, in[j])) != NEPTUNE_OK)
+        return st;
     for (int i = 0; i < 2; ++i)
       if ((st = apart(fn, out, pools[i])) != NEPTUNE_OK) return st;
   }
   for (int i = 0; i < 2; ++i)
     for (int j = 0; j < n_in; ++j)
       if ((st = apart(fn, pools[i], in[j])) != NEPTUNE_OK) return st;
+  if ((st = apart(fn, pools[0], pools[1])) != NEPTUNE_OK) return st;
   RopeLaunch L;
   L.append = true;
   L.fp8 = d->kv_dtype == NEPTUNE_DTYPE_FP8_E4M3;

@@ -94,10 +94,17 @@ def _require_cuda(*metas) -> None:
             raise ValueError("all tensors must be on the same device")
 
 
+def _check_not_repeated(shape, stride) -> None:
+    # all zero strides mean contiguous rows to the library, not one row repeated
+    if not any(stride[:-1]) and any(n > 1 for n in shape[:-1]):
+        raise ValueError("expected a tensor, not one row expanded to its shape")
+
+
 def _strides_bhs(meta) -> tuple[int, int, int]:
     shape, stride = meta[0], meta[1]
     if len(shape) != 4 or stride[-1] != 1:
         raise ValueError("expected a [batch, heads, seq, head_dim] tensor with unit head_dim stride")
+    _check_not_repeated(shape, stride)
     return stride[:3]
 
 
@@ -509,6 +516,7 @@ def _strides_th(name, meta, heads, head_dim, tokens, dtype) -> tuple[int, int]:
     if tuple(shape) != (tokens, heads, head_dim) or meta[2] != dtype:
         raise ValueError(f"{name} is {tuple(shape)} {meta[2]}, expected "
                          f"{(tokens, heads, head_dim)} {dtype}")
+    _check_not_repeated(shape, stride)
     return stride[:2]
 
 
@@ -649,11 +657,13 @@ def _attn_paged_plan(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, k_s
     desc.q_stride[:] = _strides_th("q", q, Hq, D, T, q[2])
     if out is not None:
         desc.o_stride[:] = _strides_th("out", out, Hq, D, T, q[2])
+    desc.scale_log2 = scale_to_log2(scale, D)
+    if scale is not None and desc.scale_log2 == 0.0:  # the library's default otherwise
+        raise ValueError("attention_paged: scale must not be 0")
     _require_cuda(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, k_scales, v_scales, out)
     desc.tokens, desc.batch, desc.heads_q, desc.heads_kv, desc.head_dim = T, B, Hq, Hk, D
     desc.seq_kv = max_seq_len if max_seq_len is not None else pk.max_pages * psize
     desc.dtype, desc.kv_dtype = _TORCH_TO_DTYPE[q[2]], kv_dtype
-    desc.scale_log2 = scale_to_log2(scale, D)
     n = ctypes.c_size_t()
     lib = load_library()
     check(lib.neptune_attn_paged_workspace_bytes(ctypes.byref(desc), ctypes.byref(n)), lib)
