@@ -365,7 +365,7 @@ NEPTUNE_API neptune_status neptune_attn_paged_workspace_bytes(
  * in the reference. lse (nullable) [tokens, heads_q] fp32, natural log. k_scales,
  * v_scales [num_pages, heads_kv] for E4M3 pools, NULL otherwise. cu_seqlens may be
  * NULL: one new token per sequence (tokens == batch). The page size must be a
- * multiple of 16. The lengths are read on the device when the work runs, and the
+ * multiple of 16, batch at most 65536. The lengths are read on the device when the work runs, and the
  * cut of the keys follows them; the workspace needs no clearing, must be 16-byte
  * aligned and is in use until the call's work is done. Table entries outside the
  * pool are clamped into it. o must share no byte with q or the pools. */

@@ -580,8 +580,7 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
         return u32x4{y[0], y[1], z[0], z[1]};
       }
     };
-    // (all rows of one place see alike: masked keys are then the last one again)
-    if (masked && last > lo) special |= Special<E, FP8>::template scrub<CH>(vt, lane);
+    if (masked) special |= Special<E, FP8>::template scrub<CH>(vt, lane);
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -945,9 +944,9 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
       // E4M3: V's scales meet P. Over a block within one page K's scale goes with
       // the score scale and V's into the exponent (lv), so they cost no operation
       // an element; the sum is then of scaled p, and unscaled by one product (iv).
-      // Across pages, or where the exponent would not hold the scale, each run's
-      // are multiplied in: K's here, before the mask (a zero scale must not meet
-      // -inf), V's with P.
+      // Across pages, or where the exponent would not hold V's scale or K's is not
+      // positive and finite, each run's are multiplied in: K's here, before the mask
+      // (such a scale must not meet -inf), V's with P.
       float vs[4] = {1.0f, 1.0f, 1.0f, 1.0f}, lv = 0.0f, iv = 1.0f;
       bool apart = false;
       if constexpr (FP8) {
@@ -964,8 +963,9 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
               float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i - sc0));
         };
         const int runs = last_key / 16 - (key0 >> 4);  // runs behind the end take the last one's
-        const float v0 = scale_at(vscv, index);
-        apart = (rest + 3 >= a.ps16 && runs > 0) || !(v0 >= 0x1p-64f && v0 <= 0x1p64f);
+        const float k0 = sc * scale_at(kscv, index), v0 = scale_at(vscv, index);
+        apart = (rest + 3 >= a.ps16 && runs > 0) || !(v0 >= 0x1p-64f && v0 <= 0x1p64f) ||
+                !(k0 > 0.0f && k0 <= 3.4e38f);
         if (apart) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -980,7 +980,7 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
           }
           sc = 1.0f;
         } else {
-          sc *= scale_at(kscv, index);
+          sc = k0;
           lv = __builtin_amdgcn_logf(v0);
           iv = 1.0f / v0;
         }
@@ -1246,9 +1246,11 @@ hipError_t launch_t(const PagedArgs &a, const PagedAttnLaunch &L, hipStream_t s)
       constexpr int ROWS = NT / (HD / 4) / SG;
       // rows of cut tiles at most; runs of them, short ones (a wait for memory
       // each) as long as the GPU holds the work-groups at once
-      const int64_t rows = std::min<int64_t>(L.tokens * a.group, (int64_t)a.parts / 2 * BM);
+      const int64_t tiles = a.parts / 2;
+      const int64_t rows = std::min<int64_t>(L.tokens * a.group, tiles * BM);
+      const int64_t ends = std::min(std::min(L.batch, tiles), rows);  // a run short of `take` each
       int take = ROWS;
-      auto runs = [&]() { return (rows + (int64_t)(take - 1) * L.batch) / take; };
+      auto runs = [&]() { return (rows + (take - 1) * ends) / take; };
       while (take < BM && runs() * L.heads_kv > 2048) take *= 2;
       hipLaunchKernelGGL((attn_paged_combine<E, HD, SG>), dim3((unsigned)(runs() * L.heads_kv)),
                          dim3(NT), 0, s, a, take);
@@ -1283,7 +1285,7 @@ bool attn_paged_supported(const PagedAttnLaunch &L, const char **why) {
     return false;
   }
   if (L.seq_kv > (int64_t)1 << 30 || L.num_pages > INT32_MAX || L.max_pages > INT32_MAX - 64 ||
-      L.page_size > (int64_t)1 << 30 || L.batch > (int64_t)1 << 24 || L.tokens > (int64_t)1 << 30 ||
+      L.page_size > (int64_t)1 << 30 || L.batch > 1 << 16 || L.tokens > (int64_t)1 << 30 ||
       L.heads_q > 1 << 20 || L.tokens * (L.heads_q / L.heads_kv) > (int64_t)1 << 30 ||
       (most_tiles(L) + kParts) * L.heads_kv * NT > (int64_t)0xffffffff) {
     *why = "shape too large for one launch";

@@ -166,3 +166,11 @@ def test_a_scale_of_zero_is_not_the_default(scale):
         ops.attention_paged(meta(10, 8, 128), meta(20, 2, 64, 128), meta(20, 2, 64, 128),
                             meta(3, 8, dtype=i32), meta(3, dtype=i32), meta(4, dtype=i32),
                             scale=scale)
+
+
+def test_batch_bound():
+    """Every work-group looks through all sequences: a launch takes 65536."""
+    w = ops.attention_paged_workspace_bytes
+    assert w(1, 1 << 16, 8, 2, 128, 2000) >= 0
+    with pytest.raises(_abi.NeptuneUnsupported, match="too large"):
+        w(1, (1 << 16) + 1, 8, 2, 128, 2000)
