@@ -340,7 +340,7 @@ NEPTUNE_API neptune_status neptune_qk_norm_rope(const neptune_rope_desc *desc, c
 /* k_pages, v_pages <- the new tokens' k (norm and rotation on the way) and v;
  * qo <- q with norm and rotation (neptune_append_desc). No counterpart in the
  * reference. cu_seqlens [batch + 1] may be NULL: one new token per sequence
- * (tokens == batch). q, qo: NULL when heads_q is 0; qo may be q. q_weight,
+ * (tokens == batch; with it, batch is at most 65536). q, qo: NULL when heads_q is 0; qo may be q. q_weight,
  * k_weight may be NULL (no norm), cos and sin NULL when rot_dim is 0. Into E4M3
  * pools a value goes as code = RNE-saturate(x / scale) under its page's and
  * head's k_scales, v_scales [num_pages, heads_kv], which the caller has set (a

@@ -402,6 +402,10 @@ bool rope_supported(const RopeLaunch &L, const char **why) {
     *why = "tables of 2^31 rows or pages and more";
     return false;
   }
+  if (L.cu_seqlens && L.sequences > 1 << 16) {  // every group of lanes looks through them
+    *why = "cu_seqlens of more than 65536 sequences";
+    return false;
+  }
   return true;
 }
 

@@ -91,10 +91,11 @@ def test_rope_large_and_tangled(lib):
                  odd, (2 * FAR, (0, 0, 0))) == INVALID
 
 
-def _append(lib, kp, vp, q=None, k=None, v=None, qo=None, tokens=10, fp8=False):
+def _append(lib, kp, vp, q=None, k=None, v=None, qo=None, tokens=10, fp8=False, batch=3,
+            cu=True):
     """Pools (address, strides); q, k, v, qo (address, strides) or apart."""
     d = _abi.AppendDesc()
-    d.tokens, d.batch, d.heads_q, d.heads_kv, d.head_dim = tokens, 3, 8, 2, 128
+    d.tokens, d.batch, d.heads_q, d.heads_kv, d.head_dim = tokens, batch, 8, 2, 128
     d.dtype, d.kv_dtype = _abi.DTYPE_BF16, _abi.DTYPE_FP8_E4M3 if fp8 else _abi.DTYPE_BF16
     for name, t in (("q", q), ("k", k), ("v", v), ("qo", qo)):
         if t:
@@ -104,6 +105,7 @@ def _append(lib, kp, vp, q=None, k=None, v=None, qo=None, tokens=10, fp8=False):
     p.num_pages, p.page_size, p.max_pages = 1000, 16, 32
     p.k_stride[:], p.v_stride[:] = kp[1], vp[1]
     far = [(40 + i) * FAR for i in range(5)]
+    far[1] = far[1] if cu else None
     return lib.neptune_kv_append_paged(
         ctypes.byref(d), ctypes.byref(p), *at[:3], None, None, None, None, *far[:3], kp[0], vp[0],
         *far[3:], at[3], None)
@@ -174,3 +176,12 @@ def test_batch_bound():
     assert w(1, 1 << 16, 8, 2, 128, 2000) >= 0
     with pytest.raises(_abi.NeptuneUnsupported, match="too large"):
         w(1, (1 << 16) + 1, 8, 2, 128, 2000)
+
+
+def test_append_batch_bound(lib):
+    """With cu_seqlens likewise; one token per sequence needs no search."""
+    pools = (6 * FAR, (4096, 2048, 128)), (7 * FAR, (4096, 2048, 128))
+    assert _append(lib, *pools, batch=1 << 16) == NO_DEVICE
+    assert _append(lib, *pools, batch=(1 << 16) + 1) == UNSUPPORTED
+    many = (1 << 16) + 1
+    assert _append(lib, *pools, batch=many, tokens=many, cu=False) == NO_DEVICE
