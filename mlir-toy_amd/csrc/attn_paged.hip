@@ -259,6 +259,23 @@ __device__ inline u32x2 widen4(uint32_t c) {
   return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
 }
 
+// The scale that V's scales are taken relative to where they meet P: that of the
+// first page looked at, in lane 0 of vscv. P is rounded to 16 bits with the ratio
+// in it, so its large values, at most 1, stay next to 1 and below, where bf16's
+// relative step is smallest, and 1 stays exact; the usual scales, amax / 448 with
+// amax near 4, lie just above 2^-7, where it is largest (a row over few keys: off by
+// 0.0027 of its norm with the bare scales, 0.0021 so; the output's rounding alone is
+// 0.0017). Within 2^+-16, so that no ratio leaves the range of an ordinary float.
+__device__ inline float scale_unit(float vscv) {
+  const float v = __builtin_bit_cast(
+      float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vscv), 0));
+  return v >= 0x1p-16f && v <= 0x1p16f ? v : 1.0f;
+}
+// (v_rcp_f32 inverts it: 1 ulp)
+__device__ inline float scalar(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
+
 // Infinities and NaN of V behind the mask. A masked key's p is 0, but 0 times them
 // is NaN, and a matrix product cannot leave a key out for some of its rows. So in
 // blocks that any row of a tile does not see whole, V is looked over in LDS before
@@ -416,6 +433,7 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
   }
   settle(kscv);
   settle(vscv);
+  const float unit = FP8 ? scale_unit(vscv) : 1.0f, unit_inv = FP8 ? scalar(__builtin_amdgcn_rcpf(unit)) : 1.0f;
 #pragma unroll
   for (int st = 0; st < NST; ++st) settle(qf[st]);
   settle(tabv);
@@ -517,7 +535,7 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
         }
         const float ks = a.scale2 * __builtin_bit_cast(
             float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, kscv), index - sc0));
-        vs[h] = __builtin_bit_cast(
+        vs[h] = unit_inv * __builtin_bit_cast(
             float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vscv), index - sc0));
 #pragma unroll
         for (int r = 0; r < 8; ++r) s[8 * h + r] *= ks;
@@ -593,6 +611,10 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
   if (__builtin_expect(special, 0))
     add_special<E, HD, FP8>(a, it, hk, max(t0 * STEP, lo / STEP * STEP),
                             min((t0 + ns) * STEP, it.len), pos, g, o);
+  if constexpr (FP8) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) o[nb] *= unit;
+  }
   // the waves' states, merged lane by lane, NB of a row's 4 NB vectors a wave
   const float ltot = pair_sum(lsum);
   f32x4 *const box = (f32x4 *)mine + lane;
@@ -858,6 +880,7 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
     settle(kscv);
     settle(vscv);
   }
+  const float unit = FP8 ? scale_unit(vscv) : 1.0f, unit_inv = FP8 ? scalar(__builtin_amdgcn_rcpf(unit)) : 1.0f;
   // Q and the table land before the first copy is issued
 #pragma unroll
   for (int st = 0; st < NST; ++st) settle(qf[st]);
@@ -941,7 +964,7 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
       const u32x4 vp0 = v_operand(vt, 0), vp1 = v_operand(vt, 1);
       const int key0 = (kb0 + jb) * BN;
       float sc = a.scale2;
-      // E4M3: V's scales meet P. Over a block within one page K's scale goes with
+      // E4M3: V's scales (over scale_unit) meet P. Over a block within one page K's scale goes with
       // the score scale and V's into the exponent (lv), so they cost no operation
       // an element; the sum is then of scaled p, and unscaled by one product (iv).
       // Across pages, or where the exponent would not hold V's scale or K's is not
@@ -963,14 +986,14 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
               float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i - sc0));
         };
         const int runs = last_key / 16 - (key0 >> 4);  // runs behind the end take the last one's
-        const float k0 = sc * scale_at(kscv, index), v0 = scale_at(vscv, index);
+        const float k0 = sc * scale_at(kscv, index), v0 = unit_inv * scale_at(vscv, index);
         apart = (rest + 3 >= a.ps16 && runs > 0) || !(v0 >= 0x1p-64f && v0 <= 0x1p64f) ||
                 !(k0 > 0.0f && k0 <= 3.4e38f);
         if (apart) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const float ks = sc * scale_at(kscv, index);
-            vs[c] = scale_at(vscv, index);
+            vs[c] = unit_inv * scale_at(vscv, index);
 #pragma unroll
             for (int r = 0; r < 8; ++r) s[c >> 1][8 * (c & 1) + r] *= ks;
             if (c < runs && ++rest == a.ps16) {
@@ -982,7 +1005,7 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
         } else {
           sc = k0;
           lv = __builtin_amdgcn_logf(v0);
-          iv = 1.0f / v0;
+          iv = __builtin_amdgcn_rcpf(v0);
         }
       }
       if (key0 + BN - 1 > lo_w) {
@@ -1088,6 +1111,10 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
     __syncthreads();
   }
 
+  if constexpr (FP8) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) o[nb] *= unit;
+  }
   const float ltot = pair_sum(lsum);
   if (__builtin_expect(special[0] | special[1] | special[2] | special[3], 0))
     add_special<E, HD, FP8>(a, it, hk, max(kb0, lo_tile / BN) * BN, min((kb0 + nv) * BN, it.len),

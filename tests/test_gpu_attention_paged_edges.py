@@ -123,3 +123,29 @@ def test_many_sequences_without_tokens():
     o, lse = ops.attention_paged(q.cuda(), small.k.cuda(), small.v.cuda(), table.cuda(),
                                  lens.cuda(), cu.cuda(), return_lse=True, max_seq_len=1500)
     check_attention(small, q, o.cpu(), lse.cpu())
+
+
+@pytest.mark.parametrize("n,D", [(1, 64), (1, 128), (9, 128), (40, 64), (40, 128)])
+def test_scales_cost_no_rounding_of_their_own(n, D):
+    """E4M3 rows whose keys' weight lies on one key come out rounded once: half a step of
+    bf16, 2^-9 of the next power of two above, so 2^-8 of the value at most, and 2^-12 of
+    that for the fp32 products. A second rounding, of the probability with the scale,
+    would be off by as much again."""
+    cache = Cache([(n, n)], 2, D, 16, FP8, seed=n)
+    used = ~torch.isnan(cache.k_scales[:, 0])
+    cache.v_scales[used] = 1.03 / 128.0  # between two steps of bf16
+    cache.k = torch.full_like(cache.k.float(), 0.0).to(FP8)
+    for t in range(n):  # key t points along its own direction
+        page, place = int(cache.table[0, t // 16]), t % 16
+        row = torch.zeros(D)
+        row[t] = 448.0
+        cache.k[page, :, place] = row.to(FP8)
+    cache.k_scales[used] = 1.0
+    q = torch.zeros(n, 8, D)
+    for t in range(n):
+        q[t, :, t] = 8.0  # a row's score of its own key passes all others by hundreds
+    o, _ = _run(cache, q.to(BF16))
+    want = cache.values(0, "v").permute(1, 0, 2).repeat_interleave(4, dim=1)
+    assert ((o.double() - want).abs() <= 2.0**-8 * (1 + 2.0**-12) * want.abs()).all()
+    step = torch.exp2(torch.floor(torch.log2(want.abs().clamp_min(1e-30))) - 8)  # half a step
+    assert ((o.double() - want).abs() <= step * (1 + 2.0**-10)).all()
