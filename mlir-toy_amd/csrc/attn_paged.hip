@@ -23,7 +23,15 @@
 // block-table entries, so no load waits on a load. E4M3 codes pass through
 // registers and are widened to bf16 (exact) on their way to LDS, once for the
 // work-group's four waves; the K scale meets the scores, the V scale P before
-// its rounding.
+// its rounding. Tiles of at most 32 rows take the narrow form (narrow_item).
+//
+// Bound: chunks by the matrix cores beside softmax VALU and copies, as that kernel;
+// tiles of few rows by HBM; small launches by the chain lengths - table - K and V -
+// states, at 0.7 us a link, and the second launch. Measured (us, in a replayed graph;
+// 32 heads of 128 over 8 unless said): 4 x 4096 causal 520-540, 1000 over 30000 460-478
+// (1050 TFLOP/s; a bf16 GEMM of 8192^3 1344), 2000 over 6000 E4M3 250 (bf16 225),
+// 32 x 1 over 8000 164 (6.4 TB/s), E4M3 95, 16 x 1-4 over 8000 69, 1 over 32768 29,
+// 1 over 64 6.1.
 #include <algorithm>
 #include <type_traits>
 
@@ -35,7 +43,10 @@ namespace {
 
 constexpr int kSlots = 512;         // two work-groups on each of 256 CUs
 constexpr int kParts = 2 * kSlots;  // items of cut tiles in a launch at most (make_plan)
-constexpr int NARROW = 32;          // rows up to which a tile takes the narrow form
+// Rows up to which a tile takes the narrow form. Measured (us, narrow / wide for such
+// tiles): 32 x 1 over 8000 164 / 182, E4M3 95 / 154, 16 x 1-4 over 8000 69 / 79, 1 over
+// 2000 12.6 / 13.7; a tile of more rows than one wave's 32 needs the wide one's waves.
+constexpr int NARROW = 32;
 
 struct PagedArgs {
   const uint16_t *q;
@@ -402,7 +413,9 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
   const char *kp = a.k + hk * a.kps1, *vp = a.v + hk * a.vps1;
   const int32_t *tab = a.btab + (int64_t)it.b * a.maxp;
   const int last_run = (it.len - 1) >> 4;
-  const bool once = it.tiles == 1;  // no other work-group reads these keys
+  // no other work-group reads these keys: their copies pass the caches by (32 x 1 over
+  // 8000 164 us, with them kept 187; E4M3 95, 109)
+  const bool once = it.tiles == 1;
   int tab0 = 0, tabv = 0, sc0 = 0;
   float kscv = 0.0f, vscv = 0.0f;
   auto load_tab = [&](int first) {
@@ -1256,9 +1269,11 @@ Room room_of(const PagedAttnLaunch &L) {
   r.parts = 0;
   if (may_split(L)) {
     const int64_t splits = ((L.seq_kv + BN - 1) / BN + 2) / 4 + 1;  // splits_of at most
-    r.parts = std::min(tiles * splits, std::max<int64_t>(kParts / L.heads_kv, 1));
+    r.parts = std::min(tiles * splits, (int64_t)kParts / L.heads_kv);
+    if (r.parts < 2) r.parts = 0;  // heads enough without
     // work-groups without an item cost some 10 us a thousand
-    r.items = std::min(tiles * splits, std::max(tiles + r.slots / 4, r.slots * 4 / 3 + 1));
+    if (r.parts)
+      r.items = std::min(tiles * splits, std::max(tiles + r.slots / 4, r.slots * 4 / 3 + 1));
   }
   return r;
 }
@@ -1282,6 +1297,9 @@ hipError_t launch_t(const PagedArgs &a, const PagedAttnLaunch &L, hipStream_t s)
       hipLaunchKernelGGL((attn_paged_combine<E, HD, SG>), dim3((unsigned)(runs() * L.heads_kv)),
                          dim3(NT), 0, s, a, take);
     };
+    // eight groups a row where a tile may have that many splits (1 over 32768 29.4 us,
+    // one group 38.6), else one (16 x 8 over 8000 90, eight 96; chunks of 130 head_dim-64
+    // rows over 1500 19.6, 25.9)
     if (a.items >= 8 * most_tiles(L))
       combine(std::integral_constant<int, 8>{});
     else

@@ -149,3 +149,13 @@ def test_scales_cost_no_rounding_of_their_own(n, D):
     assert ((o.double() - want).abs() <= 2.0**-8 * (1 + 2.0**-12) * want.abs()).all()
     step = torch.exp2(torch.floor(torch.log2(want.abs().clamp_min(1e-30))) - 8)  # half a step
     assert ((o.double() - want).abs() <= step * (1 + 2.0**-10)).all()
+
+
+@pytest.mark.parametrize("Hk", [257, 512, 513, 700])
+def test_more_kv_heads_than_work_groups(Hk):
+    """Heads by the hundred fill the GPU: no keys are cut from 513 on."""
+    cache = Cache([(1, 600), (3, 530)], Hk, 64, 16, BF16, seed=2)
+    q = _q(cache, Hk, BF16)
+    check_attention(cache, q, *_run(cache, q))
+    need = ops.attention_paged_workspace_bytes(4, 2, Hk, Hk, 64, 600)
+    assert (need == 0) == (Hk > 512)
