@@ -159,3 +159,24 @@ def test_more_kv_heads_than_work_groups(Hk):
     check_attention(cache, q, *_run(cache, q))
     need = ops.attention_paged_workspace_bytes(4, 2, Hk, Hk, 64, 600)
     assert (need == 0) == (Hk > 512)
+
+
+def test_overlapping_sequences_stay_within_the_buffers():
+    """cu_seqlens that run back name rows twice, more than the launch has room for:
+    nothing outside the outputs and the workspace is touched, and the call ends."""
+    cache = Cache([(64, 900)], 2, 64, 16, BF16, seed=6)
+    q = _q(cache, 8, BF16)
+    B = 40
+    cu = torch.tensor([0, 64] * (B // 2) + [64], dtype=torch.int32)
+    lens = torch.full((B,), 900, dtype=torch.int32)
+    table = cache.table[:1].repeat(B, 1)
+    need = ops.attention_paged_workspace_bytes(64, B, 8, 2, 64, 900)
+    guard = 1 << 16
+    ws = torch.full((need + 2 * guard,), 77, dtype=torch.uint8, device="cuda")
+    out = torch.full((64 + 64, 8, 64), 5.0, dtype=BF16, device="cuda")
+    ops.attention_paged(q.cuda(), cache.k.cuda(), cache.v.cuda(), table.cuda(), lens.cuda(),
+                        cu.cuda(), max_seq_len=900, out=out[32:96],
+                        workspace=ws[guard:guard + need])
+    torch.cuda.synchronize()
+    assert (out[:32] == 5.0).all() and (out[96:] == 5.0).all()
+    assert (ws[:guard] == 77).all() and (ws[guard + need:] == 77).all()
