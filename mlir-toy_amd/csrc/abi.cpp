@@ -453,14 +453,14 @@ bool is_float(int32_t dtype, bool f32) {
 }
 
 // Bytes from the first element to past the last of a [sizes.., row] tensor;
-// 0 where that passes 2^62
+// 0 where that passes 2^60
 size_t span(const int64_t *sizes, const int64_t *strides, int n, int64_t row, int64_t esize) {
   int64_t at = row, step;
   for (int i = 0; i < n; ++i)
     if (__builtin_mul_overflow(sizes[i] - 1, strides[i], &step) ||
         __builtin_add_overflow(at, step, &at))
       return 0;
-  return at > ((int64_t)1 << 62) / esize ? 0 : (size_t)(at * esize);
+  return at > ((int64_t)1 << 60) / esize ? 0 : (size_t)(at * esize);
 }
 
 // A strided tensor of an entry point: its rows' strides resolved (zero:
@@ -513,12 +513,12 @@ neptune_status resolve(const char *fn, const char *name, const void *p, const in
 // rows is delta + sum of x_j step_j with x_j in [lo_j, hi_j] (a step that both
 // tensors take counts once); largest step first, few x_j leave one that the
 // smaller steps can still bring into (-b's row, a's row). Where strides are so
-// tangled that it takes thousands of tries, the answer is yes.
+// tangled that it takes thousands of tries, the answer is yes. (Both span at most
+// 2^60 bytes and cross, so 64 bits hold every sum.)
 struct Steps {
   int n = 0, tries = 0;
-  int64_t step[6];
-  __int128 lo[6], hi[6];
-  __int128 below, above;  // the open interval
+  int64_t step[6], lo[6], hi[6];
+  int64_t below, above;  // the open interval
   void add(int64_t by, int64_t first, int64_t last) {
     int i = 0;
     while (i < n && step[i] > by) ++i;
@@ -530,16 +530,16 @@ struct Steps {
     lo[i] += first;
     hi[i] += last;
   }
-  bool reach(int j, __int128 at) {
+  bool reach(int j, int64_t at) {
     if (++tries > 4096) return true;
     if (j == n) return at > below && at < above;
-    __int128 least = 0, most = 0;  // of the smaller steps
+    int64_t least = 0, most = 0;  // of the smaller steps
     for (int i = j + 1; i < n; ++i) least += lo[i] * step[i], most += hi[i] * step[i];
-    const auto floor_div = [](__int128 x, __int128 y) { return x / y - (x % y < 0); };
+    const auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
     // at + x step + [least, most] meets [below + 1, above - 1]
-    const __int128 first = -floor_div(at + most - below - 1, step[j]);
-    const __int128 last = floor_div(above - 1 - least - at, step[j]);
-    for (__int128 x = first > lo[j] ? first : lo[j]; x <= last && x <= hi[j]; ++x)
+    const int64_t first = -floor_div(at + most - below - 1, step[j]);
+    const int64_t last = floor_div(above - 1 - least - at, step[j]);
+    for (int64_t x = first > lo[j] ? first : lo[j]; x <= last && x <= hi[j]; ++x)
       if (reach(j + 1, at + x * step[j])) return true;
     return false;
   }
@@ -552,9 +552,9 @@ bool meet(const Strided &a, const Strided &b) {
     if (a.size[i] > 1) s.add(a.stride[i] * a.esize, 1 - a.size[i], 0);
   for (int i = 0; i < b.n; ++i)
     if (b.size[i] > 1) s.add(b.stride[i] * b.esize, 0, b.size[i] - 1);
-  s.below = -(__int128)(b.dim * b.esize);
+  s.below = -(b.dim * b.esize);
   s.above = a.dim * a.esize;
-  return s.reach(0, (__int128)(uintptr_t)b.p - (__int128)(uintptr_t)a.p);
+  return s.reach(0, (int64_t)((uintptr_t)b.p - (uintptr_t)a.p));
 }
 
 // out must share no byte with in
