@@ -139,7 +139,9 @@ __device__ inline Seq sequence(const PagedArgs &a, int b) {
 // rows_inv: 62 / rows. The quotient blocks / chain is cut to a whole number (a
 // quarter block keeps whole ones whole), but for a tile of few rows rounded to
 // one: those wait for memory, and more of them side by side help (24 x 12 heads,
-// 1 over 7300: 185 / 214 us).
+// 1 over 7300: 185 / 214 us). Few rows' states are small, but the combine still joins
+// them one after the other: kFewRows more rows of them (3 x 1 over 20000, one KV head
+// 16.8 / 19.6 us).
 // (Uncontracted, so that every wave of both kernels rounds alike.)
 __device__ inline int splits_of(int blocks, bool few, float chain_inv, float rows, float rows_inv) {
 #pragma clang fp contract(off)
@@ -152,13 +154,21 @@ __device__ inline int splits_of(int blocks, bool few, float chain_inv, float row
 }
 
 struct Plan {
-  float chain_inv, rows, rows_inv;  // of splits_of
-  Seq first;                        // of the wave's lane as sequence 0 .. 63
+  float chain_inv, rows[2], rows_inv[2];  // of splits_of; [1]: tiles of few rows
+  Seq first;                              // of the wave's lane as sequence 0 .. 63
 };
+constexpr float kFewRows = 1.5f;
+
+__device__ inline int splits_of(const PagedArgs &a, const Plan &p, const Seq &s) {
+  const bool few = s.n * a.group <= NARROW;
+  return splits_of(s.blocks, few, p.chain_inv, few ? p.rows[1] : p.rows[0],
+                   few ? p.rows_inv[1] : p.rows_inv[0]);
+}
 
 // The plan of a launch, by every wave for itself, one sequence per lane. The chain
 // starts at the launch's blocks (a tile's taken as the mean of its sequence's first
-// and last tile's) over kSlots work-groups and grows until the items fit: into one
+// and last tile's) over kSlots work-groups, two blocks at least (of four: 1 over 3000
+// 11.8 / 13.0 us, 100 over 600 15.3 / 17.5), and grows until the items fit: into one
 // round of the GPU where the tiles themselves do, else into the launch's
 // work-groups, and in any case into the room for states. One round of items that
 // differ by up to a factor of two in length did better than two of half as long
@@ -171,7 +181,7 @@ __device__ inline Plan make_plan(const PagedArgs &a, int lane) {
 #pragma clang fp contract(off)
   Plan p;
   p.first = sequence(a, lane);
-  p.chain_inv = p.rows = p.rows_inv = 0.0f;
+  p.chain_inv = p.rows[0] = p.rows[1] = p.rows_inv[0] = p.rows_inv[1] = 0.0f;
   if (!a.parts) return p;
   uint64_t work = 0;  // half blocks
   int rows = 0, tiles = 0;
@@ -189,18 +199,18 @@ __device__ inline Plan make_plan(const PagedArgs &a, int lane) {
                          ((uint64_t)wave_total((int)(work >> 42)) << 42);
   tiles = wave_total(tiles);
   if (tiles > a.items) return p;  // sequences that overlap: not all of it is done, nothing is cut
-  p.rows = (float)wave_total(rows) * (float)a.Hk * (1.0f / BM);
-  p.rows_inv = 62.0f * __builtin_amdgcn_rcpf(p.rows);
+  p.rows[0] = (float)wave_total(rows) * (float)a.Hk * (1.0f / BM);
+  p.rows[1] = p.rows[0] + kFewRows;
+  for (int i = 0; i < 2; ++i) p.rows_inv[i] = 62.0f * __builtin_amdgcn_rcpf(p.rows[i]);
   const uint64_t even = (total * (uint32_t)a.Hk + 2 * kSlots - 1) / (2 * kSlots);
-  const int chain0 = (int)min(max(even, (uint64_t)4), (uint64_t)1 << 25);
+  const int chain0 = (int)min(max(even, (uint64_t)2), (uint64_t)1 << 25);
   int chain = chain0;
   bool fits = false, first_fits = false;
   while (true) {
     p.chain_inv = __builtin_amdgcn_rcpf((float)chain);
     int items = 0, parts = 0;
     auto count = [&](const Seq &s) {
-      const int sp =
-          splits_of(s.blocks, s.n * a.group <= NARROW, p.chain_inv, p.rows, p.rows_inv);
+      const int sp = splits_of(a, p, s);
       items += s.tiles * sp;
       parts += sp > 1 ? s.tiles * sp : 0;
     };
@@ -230,8 +240,7 @@ __device__ inline bool find_item(const PagedArgs &a, const Plan &p, int lane, in
   int base = 0, parts = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const Seq s = b0 ? sequence(a, b0 + lane) : p.first;
-    const int sp = a.parts ? splits_of(s.blocks, s.n * a.group <= NARROW, p.chain_inv, p.rows, p.rows_inv)
-                           : 1;
+    const int sp = a.parts ? splits_of(a, p, s) : 1;
     const int mparts = sp > 1 ? s.tiles * sp : 0;
     const int mine = take ? (sp > 1 ? (s.n * a.group + take - 1) / take : 0) : s.tiles * sp;
     const int sum = wave_scan(mine), psum = a.parts ? wave_scan(mparts) : 0;
@@ -1245,7 +1254,7 @@ int64_t most_tiles(const PagedAttnLaunch &L) {
   return std::min((rows + (BM - 1) * L.batch) / BM, rows);
 }
 
-// Whether the device may cut keys: a split takes 4 blocks at least, and one
+// Whether the device may cut keys: not those of fewer than eight blocks, and one
 // sequence of at least 2 kSlots tiles is not cut (its mean chain is at least half
 // its longest).
 bool may_split(const PagedAttnLaunch &L) {
@@ -1269,7 +1278,7 @@ Room room_of(const PagedAttnLaunch &L) {
   r.items = tiles;
   r.parts = 0;
   if (may_split(L)) {
-    const int64_t splits = ((L.seq_kv + BN - 1) / BN + 2) / 4 + 1;  // splits_of at most
+    const int64_t splits = ((L.seq_kv + BN - 1) / BN + 2) / 2 + 1;  // splits_of at most
     r.parts = std::min(tiles * splits, (int64_t)kParts / L.heads_kv);
     if (r.parts < 2) r.parts = 0;  // heads enough without
     // work-groups without an item cost some 10 us a thousand
@@ -1298,10 +1307,10 @@ hipError_t launch_t(const PagedArgs &a, const PagedAttnLaunch &L, hipStream_t s)
       hipLaunchKernelGGL((attn_paged_combine<E, HD, SG>), dim3((unsigned)(runs() * L.heads_kv)),
                          dim3(NT), 0, s, a, take);
     };
-    // eight groups a row where a tile may have that many splits (1 over 32768 29.4 us,
-    // one group 38.6), else one (16 x 8 over 8000 90, eight 96; chunks of 130 head_dim-64
-    // rows over 1500 19.6, 25.9)
-    if (a.items >= 8 * most_tiles(L))
+    // eight groups a row where the rows are few and a tile may have that many splits (1
+    // over 32768 29.4 us, one group 38.6), else one (16 x 8 over 8000 90, eight 96; 6 x
+    // 32-130 head_dim-64 tokens over 1500 20, 26; 200 over 8000 45, 53)
+    if (L.tokens * L.heads_q <= 512 && a.items >= 8 * most_tiles(L))
       combine(std::integral_constant<int, 8>{});
     else
       combine(std::integral_constant<int, 1>{});
