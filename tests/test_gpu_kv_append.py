@@ -136,6 +136,18 @@ def test_many_sequences(n):
     _append(cache, 4, BF16, rot=64)
 
 
+@pytest.mark.parametrize("n", [700, 4096, 4097])
+def test_sequences_by_the_thousand(n):
+    """More than a lane has one of, and than 64 lanes have 64 of; most of them empty
+    in long runs, some with several tokens."""
+    g = torch.Generator().manual_seed(n)
+    new = torch.randint(0, 4, (n,), generator=g) * (torch.rand(n, generator=g) < 0.2)
+    new[n // 3:n // 2] = 0
+    new[0] = new[-1] = 1
+    cache = Cache([(int(x), int(x) + i % 20) for i, x in enumerate(new)], 1, 64, 16, BF16)
+    _append(cache, 2, BF16, rot=64)
+
+
 def test_many_tokens():
     """Enough groups for the form that takes several heads a group."""
     cache = Cache([(1100, 1100), (700, 950)], 4, 64, 64, BF16)
