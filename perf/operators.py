@@ -16,7 +16,6 @@ Activations are N(0, 1), as projections after a norm give; norm weights are
 1 + 0.1 N(0, 1); pages lie in the pool in random order.
 """
 
-import functools
 import math
 import random
 import sys
@@ -32,7 +31,6 @@ _BYTES = {"f32": 4, "f16": 2, "bf16": 2, "fp8": 1}
 _EPS = 1e-6
 
 
-@functools.lru_cache(maxsize=None)
 def _ops():
     package = str(Path(__file__).resolve().parents[1] / "mlir-toy_amd")
     if package not in sys.path:
