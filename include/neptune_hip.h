@@ -342,8 +342,8 @@ NEPTUNE_API neptune_status neptune_qk_norm_rope(const neptune_rope_desc *desc, c
  * reference. cu_seqlens [batch + 1] may be NULL: one new token per sequence
  * (tokens == batch; with it, batch is at most 65536). q, qo: NULL when heads_q is 0; qo may be q. q_weight,
  * k_weight may be NULL (no norm), cos and sin NULL when rot_dim is 0. Into E4M3
- * pools a value goes as code = RNE-saturate(x / scale) under its page's and
- * head's k_scales, v_scales [num_pages, heads_kv], which the caller has set (a
+ * pools a value goes as code = RNE-saturate(x / scale), the quotient rounded to
+ * fp32 first, under its page's and head's k_scales, v_scales [num_pages, heads_kv], which the caller has set (a
  * page of scale 0 takes zero codes); NULL otherwise. A row is not stored when its
  * place is negative or past its block table, or the table's entry lies outside
  * [0, num_pages); rows behind cu_seqlens[batch] are neither stored nor written to
