@@ -117,6 +117,13 @@ __device__ inline float group_sum(float x) {
   return x;
 }
 
+// 1 / sqrt(x) by v_rsq_f32 (1 ulp), which reads subnormal numbers as 0: those, the mean
+// squares of rows near 2^-64 with an eps as small, are scaled up first
+__device__ inline float inverse_root(float x) {
+  const bool small = x < 0x1p-100f;
+  return __builtin_amdgcn_rsqf(small ? x * 0x1p100f : x) * (small ? 0x1p50f : 1.0f);
+}
+
 // Eight E4M3 codes of the fp32 quotients x / scale: nearest even, saturated (the
 // instruction turns what passes 448 into NaN, so it is cut off first). The product
 // with 1 / scale is off by up to 1.5 steps of fp32, which moves quotients from the
@@ -306,8 +313,7 @@ __device__ inline void rows(const RopeArgs &a) {
         float ss = 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) ss = fmaf(ya[j], ya[j], fmaf(yb[j], yb[j], ss));
-        // v_rsq_f32: 1 ulp
-        r = __builtin_amdgcn_rsqf(fmaf(group_sum<LPR>(ss), a.inv_dim, a.eps));
+        r = inverse_root(fmaf(group_sum<LPR>(ss), a.inv_dim, a.eps));
       }
       f32x4 za, zb;
 #pragma unroll
