@@ -495,6 +495,9 @@ def qk_norm_rope(
     x * w / sqrt(mean(x^2) + eps). ``out`` = (q_out, k_out) may be (q, k).
     Returns (q_out, k_out), by default new contiguous tensors.
     """
+    if out is not None and not (isinstance(out, (tuple, list)) and len(out) == 2 and
+                                all(isinstance(t, torch.Tensor) for t in out)):
+        raise ValueError("out must be a pair of tensors (q_out, k_out)")
     q_out, k_out = (None, None) if out is None else out
     desc = _rope_plan(_meta(q), _meta(k), _meta(cos), _meta(sin), _meta(positions),
                       _meta(q_weight), _meta(k_weight), _meta(q_out), _meta(k_out), float(eps),
