@@ -170,7 +170,8 @@ def attention(
 ):
     """softmax(q k^T * scale) v with the HTile numeric policy.
 
-    q [B, Hq, Sq, D], k/v [B, Hkv, Skv, D] in float32, float16 or bfloat16;
+    q [B, Hq, Sq, D], k/v [B, Hkv, Skv, D] in float32, float16 or bfloat16
+    (any strides with D contiguous, but not one row expanded to all of them);
     returns out [B, Hq, Sq, D] (and lse [B, Hq, Sq] fp32 if asked).
     ``scale_log2`` gives the score scale already in the exp2 domain (the
     HTile program's own constant, HTile:24), in place of ``scale``.

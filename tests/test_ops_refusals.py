@@ -25,3 +25,24 @@ def test_rope_takes_both_outputs_or_none(out):
     with pytest.raises(ValueError, match="q_out, k_out"):
         ops.qk_norm_rope(meta(2, 8, 5, 128), meta(2, 2, 5, 128), meta(100, 64, dtype=f32),
                          meta(100, 64, dtype=f32), meta(2, 5, dtype=i32), out=out)
+
+
+def _device_meta(t):
+    """What a plan knows of such a tensor on a GPU."""
+    return t.shape, t.stride(), t.dtype, torch.device("cuda", 0)
+
+
+@pytest.mark.parametrize("at", ["q", "k", "v", "out"])
+def test_expanded_rows_are_refused_by_attention(at):
+    """All strides zero would read as contiguous, far past the row."""
+    shapes = dict(q=(2, 8, 5, 128), k=(2, 2, 9, 128), v=(2, 2, 9, 128), out=(2, 8, 5, 128))
+    tensors = {n: _device_meta(_row(*s) if n == at else meta(*s)) for n, s in shapes.items()}
+    with pytest.raises(ValueError, match="one row expanded"):
+        ops._attn_plan(*tensors.values(), None, False, None, None, 0, 0)
+
+
+def test_a_single_row_may_have_any_strides():
+    """Where no step is taken, strides of zero mean nothing."""
+    row = _device_meta(_row(1, 1, 1, 128))
+    desc, _, shape = ops._attn_plan(row, row, row, None, None, False, None, None, 0, 0)
+    assert shape == (1, 1, 1)
