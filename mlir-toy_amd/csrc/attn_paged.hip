@@ -1068,10 +1068,7 @@ hipError_t launch_t(const PagedArgs &a, const PagedAttnLaunch &L, hipStream_t s)
       hipLaunchKernelGGL((attn_paged_combine<E, HD, SG>), dim3((unsigned)(runs() * L.heads_kv)),
                          dim3(NT), 0, s, a, take);
     };
-    // eight groups a row where the rows are few and a tile may have that many splits (1
-    // over 32768 29.4 us, one group 38.6), else one (16 x 8 over 8000 90, eight 96; 6 x
-    // 32-130 head_dim-64 tokens over 1500 20, 26; 200 over 8000 45, 53)
-    if (L.tokens * L.heads_q <= 512 && a.items >= 8 * most_tiles(L))
+    if (combine_groups(L, room_of(L)) == 8)
       combine(std::integral_constant<int, 8>{});
     else
       combine(std::integral_constant<int, 1>{});

@@ -270,5 +270,13 @@ Room room_of(const PagedAttnLaunch &L) {
   return r;
 }
 
+// Groups of lanes that join a row's states in the combine: eight where the rows are few
+// and a tile may have that many splits (1 over 32768 29.4 us, one group 38.6), else one
+// (16 x 8 over 8000 90, eight 96; 6 x 32-130 head_dim-64 tokens over 1500 20, 26; 200
+// over 8000 45, 53)
+int combine_groups(const PagedAttnLaunch &L, const Room &r) {
+  return L.tokens * L.heads_q <= 512 && r.items >= 8 * most_tiles(L) ? 8 : 1;
+}
+
 }  // namespace
 }  // namespace neptune

@@ -1,8 +1,8 @@
 // Runs attn_plan.h on the CPU: 64 lanes as coroutines that meet at every ballot,
 // lane read and sum, as a wave does. stdin: tokens batch heads_q heads_kv head_dim
 // seq_kv, whether cu_seqlens follows, its batch + 1 numbers, batch lengths, then the
-// asked items as "count index..". stdout: "items slots parts part_rows", then for
-// each asked index "-" or "b n row0 len tile tiles split splits part".
+// asked items as "count index..". stdout: "items slots parts part_rows combine_groups",
+// then for each asked index "-" or "b n row0 len tile tiles split splits part".
 #include <math.h>
 #include <stdint.h>
 #include <stdio.h>
@@ -138,7 +138,8 @@ int main() {
       live = live || turn[i] >= 0;
     }
   }
-  printf("%ld %ld %ld %ld\n", room.items, room.slots, room.parts, part_rows(L));
+  printf("%ld %ld %ld %ld %d\n", room.items, room.slots, room.parts, part_rows(L),
+         combine_groups(L, room));
   for (size_t i = 0; i < asked.size(); ++i) {
     const Item &t = found[i];
     if (!there[i])

@@ -8,6 +8,8 @@ from pathlib import Path
 
 import pytest
 
+from test_gpu_attention_paged_cuts import CUTS
+
 ROOT = Path(__file__).resolve().parents[1]
 BM = 128
 
@@ -37,7 +39,7 @@ def _check(lanes, batch, Hq, Hk, D, seq_kv):
     """Items of a launch of sequences [(new, length)], each once, states apart."""
     cu = [sum(n for n, _ in batch[:b]) for b in range(len(batch) + 1)]
     lens = [n for _, n in batch]
-    (items, _, parts, rows), _ = lanes(cu[-1], Hq, Hk, D, seq_kv, cu, lens, [])
+    (items, _, parts, *_), _ = lanes(cu[-1], Hq, Hk, D, seq_kv, cu, lens, [])
     _, found = lanes(cu[-1], Hq, Hk, D, seq_kv, cu, lens, range(items))
     want = {(b, t) for b, (n, _) in enumerate(batch) for t in range(-(-n * (Hq // Hk) // BM))}
     got, states, cut = {}, set(), 0
@@ -80,6 +82,15 @@ def test_items(lanes, batch, Hq, Hk, D, seq_kv, cut):
     assert (_check(lanes, batch, Hq, Hk, D, seq_kv) > 0) == cut
 
 
+@pytest.mark.parametrize("batch,Hq,Hk,D,page,qt,kt,cut,groups", CUTS, ids=lambda x: str(x)[:24])
+def test_what_the_gpu_tests_mean_to_cut(lanes, batch, Hq, Hk, D, page, qt, kt, cut, groups):
+    longest = max(n for _, n in batch)
+    assert (_check(lanes, batch, Hq, Hk, D, longest) > 0) == cut
+    (_, _, parts, _, by), _ = lanes(sum(n for n, _ in batch), Hq, Hk, D, longest, None,
+                                    [n for _, n in batch], [])
+    assert parts > 0 and by == groups
+
+
 def test_items_of_random_batches(lanes):
     rng = random.Random(11)
     for _ in range(60):
@@ -105,7 +116,7 @@ def test_states_of_sequences_that_overlap_stay_within_the_room(lanes, B, tokens,
     in 64 bits."""
     cu = [0, tokens] * (B // 2) + [tokens]
     lens = [length] * B
-    (items, _, parts, _), _ = lanes(tokens, Hq, Hk, 64, 6000, cu, lens, [])
+    (items, _, parts, *_), _ = lanes(tokens, Hq, Hk, 64, 6000, cu, lens, [])
     assert parts > 0, "keys could be cut"
     asked = sorted({0, 1, 2, parts - 1, parts, parts + 1, items // 2, items - 2, items - 1})
     _, found = lanes(tokens, Hq, Hk, 64, 6000, cu, lens, [i for i in asked if 0 <= i < items])
@@ -124,7 +135,7 @@ def test_more_tiles_than_the_launch_has_items_for_are_not_cut(lanes, B, rows, gr
     tokens = rows // group + 1
     cu = [0] + [1, tokens] * (B // 2)
     lens = [100000] + [0] * (B - 1)
-    (items, _, parts, _), found = lanes(tokens, group, 1, 64, 100000, cu, lens, [0, 1, 2])
+    (items, _, parts, *_), found = lanes(tokens, group, 1, 64, 100000, cu, lens, [0, 1, 2])
     assert parts > 0, "keys could be cut"
     assert [it[7] for it in found] == [1, 1, 1]
     # and it is, by itself
