@@ -347,7 +347,9 @@ NEPTUNE_API neptune_status neptune_qk_norm_rope(const neptune_rope_desc *desc, c
  * page of scale 0 takes zero codes); NULL otherwise. A row is not stored when its
  * place is negative or past its block table, or the table's entry lies outside
  * [0, num_pages); rows behind cu_seqlens[batch] are neither stored nor written to
- * qo. Two rows sent to one slot leave either. The pools and qo share no byte with
+ * qo. A place outside cos and sin is clamped into them, as in neptune_qk_norm_rope:
+ * such a key is stored, turned by the last row's angles, so the tables must cover the
+ * longest sequence. Two rows sent to one slot leave either. The pools and qo share no byte with
  * each other or an input (but qo may be q). head_dim 64 or 128; 16-byte aligned
  * bases and strides of whole 16-byte units. */
 NEPTUNE_API neptune_status neptune_kv_append_paged(

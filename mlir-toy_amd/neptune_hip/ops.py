@@ -630,8 +630,9 @@ def kv_append_paged(
     ``q`` [T, Hq, D] the queries too, and [T, Hq, D] is returned (``out``, which
     may be q, or a new tensor; None without q). A row without a slot (a
     negative place, one past its table, a table entry outside the pool) is not
-    stored; rows behind the last sequence are left out of the cache and of the
-    result.
+    stored. ``cos`` and ``sin`` must reach the longest sequence: a place past
+    their last row is turned by that row's angles and stored all the same. Rows
+    behind the last sequence are left out of the cache and of the result.
     """
     desc, pk = _append_plan(
         _meta(k), _meta(v), _meta(k_pages), _meta(v_pages), _meta(block_table), _meta(seq_lens),
