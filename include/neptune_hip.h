@@ -201,7 +201,7 @@ typedef struct neptune_append_desc {
  * [tokens, heads_q, head_dim] with (token, head) strides in elements (zero:
  * contiguous). A row sees its sequence's tokens up to its own place; one whose
  * place is negative sees none: O = 0, lse = -inf. Rows of no sequence (behind
- * cu_seqlens[batch]) are left as they were. */
+ * cu_seqlens[batch]) are left as they were, in o and in lse. */
 typedef struct neptune_attn_paged_desc {
   int64_t tokens, batch, heads_q, heads_kv, head_dim;
   int64_t seq_kv; /* the longest sequence; longer ones are cut to it           */

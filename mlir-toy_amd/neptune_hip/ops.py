@@ -632,7 +632,9 @@ def kv_append_paged(
     negative place, one past its table, a table entry outside the pool) is not
     stored. ``cos`` and ``sin`` must reach the longest sequence: a place past
     their last row is turned by that row's angles and stored all the same. Rows
-    behind the last sequence are left out of the cache and of the result.
+    behind the last sequence are left out of the cache and of the result: they
+    stay as they were in ``out``, and in a new tensor hold whatever its memory
+    held, so a padded step gives its own ``out``.
     """
     desc, pk = _append_plan(
         _meta(k), _meta(v), _meta(k_pages), _meta(v_pages), _meta(block_table), _meta(seq_lens),
@@ -701,8 +703,14 @@ def attention_paged(
     bfloat16 q; page sizes that are multiples of 16; D 64 or 128).
     ``max_seq_len`` (default max_pages * page_size) bounds the lengths. A row
     sees its sequence up to its own place; one with a negative place sees
-    nothing: output 0, log-sum-exp -inf. Rows behind the last sequence are left
-    as they were. Returns o [T, Hq, D] (and lse [T, Hq] fp32 if asked).
+    nothing: output 0, log-sum-exp -inf. Rows behind the last sequence are not
+    written: they stay as they were in ``out``, and in a new tensor, lse among
+    them, hold whatever its memory held (a padded step gives its own ``out``,
+    and reads no lse there). Returns o [T, Hq, D] (and lse [T, Hq] fp32 if
+    asked).
+
+    The workspace is for the calls of the sizes it was asked for: fewer tokens
+    may need a larger one, since keys are cut where tiles are few.
     """
     desc, pk, need = _attn_paged_plan(
         _meta(q), _meta(k_pages), _meta(v_pages), _meta(block_table), _meta(seq_lens),

@@ -46,3 +46,10 @@ def test_a_single_row_may_have_any_strides():
     row = _device_meta(_row(1, 1, 1, 128))
     desc, _, shape = ops._attn_plan(row, row, row, None, None, False, None, None, 0, 0)
     assert shape == (1, 1, 1)
+
+
+def test_a_workspace_is_for_its_own_sizes():
+    """Cutting keys needs room where tiles are few; one sequence of many is not cut."""
+    few, many = (ops.attention_paged_workspace_bytes(n, 1, 32, 8, 128, 100000)
+                 for n in (4000, 40000))
+    assert few > 0 and many == 0
