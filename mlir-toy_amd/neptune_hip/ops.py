@@ -622,7 +622,9 @@ def kv_append_paged(
     (without ``cu_seqlens`` one row each), and seq_lens[b] counts its tokens
     with them, so that its last row lands at seq_lens[b] - 1. k_pages / v_pages
     [num_pages, Hkv, page_size, D] views as in ``decode_paged``, of k's dtype or
-    E4M3 codes under the given k_scales / v_scales [num_pages, Hkv]; block_table
+    E4M3 codes under the given k_scales / v_scales [num_pages, Hkv] (of either
+    dtype's values: ``attention_paged`` and ``decode_paged`` read codes with
+    bfloat16 queries, a float16 model casts its own); block_table
     [B, max_pages], seq_lens [B], cu_seqlens [B + 1] int32 on the device.
 
     Keys are normalised (``k_weight``) and rotated (``cos``, ``sin``,
