@@ -25,6 +25,13 @@
 // work-group's four waves; the K scale meets the scores, the V scale P before
 // its rounding. Tiles of at most 32 rows take the narrow form (narrow_item).
 //
+// One rounding is not the plain form's: P goes to 16 bits for P.V, the operands that
+// the matrix instructions take (as a sum of two 16-bit numbers it would cost twice the
+// products). The sums l and O are fp32, l of p before the rounding. The result is then
+// off by 0.0021-0.0024 of its norm (f16 0.00027) where rounding the output alone gives
+// 0.0017 (0.00021). A maximum that lags (kSlack) changes none of it: p's relative
+// rounding is the same at 2^8 as at 1, and f16 holds both.
+//
 // Bound: chunks by the matrix cores beside softmax VALU and copies, as that kernel;
 // tiles of few rows by HBM; small launches by the chain lengths - table - K and V -
 // states, at 0.7 us a link, and the second launch. Measured (us, in a replayed graph;
@@ -399,7 +406,7 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
       for (int j = 0; j < 4; ++j) {
         const float p0 = fast_exp2(s[8 * c + 2 * j] - m), p1 = fast_exp2(s[8 * c + 2 * j + 1] - m);
         lsum += p0 + p1;
-        // (a masked key's page may hold any scale)
+        // rounded to 16 bits (above), V's scale with it; a masked key's page may hold any
         pf[c][j] = FP8 ? E::pack2(p0 == 0.0f ? 0.0f : p0 * vs[c], p1 == 0.0f ? 0.0f : p1 * vs[c])
                        : E::pack2(p0, p1);
       }
@@ -602,7 +609,8 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   // E4M3 pools: 16 codes per lane and load, two 16-byte units of bf16. The rows of
   // 16 lanes, which one cycle writes to LDS, have units of both parities: K's by
   // its swizzle, V's by an order of rows that alternates bit 2 and a swizzle that
-  // brings that bit in (without it half the LDS cycles were conflicts)
+  // brings that bit in (without it half the LDS cycles were conflicts; counted, a
+  // quarter of them still are, none with 16-bit pools)
   constexpr int LPR8 = HD / 16, ROWS8 = 64 / LPR8, N8 = 16 / ROWS8;
   const int krow8 = lane / LPR8;
   const int vrow8 = HD == 128 ? krow8 >> 1 | (krow8 & 1) << 2
@@ -859,7 +867,7 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
             const float p1 = fast_exp2(fmaf(s[kb][8 * hh + 2 * i + 1], sc, nm));
             rs = c + i == 0 ? p0 : rs + p0;
             rs += p1;
-            pf[c][i] = E::pack2(p0, p1);
+            pf[c][i] = E::pack2(p0, p1);  // 16 bits, for P.V alone
           }
         }
         if constexpr (FP8) {
