@@ -36,7 +36,7 @@
 // tiles of few rows by HBM; small launches by the chain lengths - table - K and V -
 // states, at 0.7 us a link, and the second launch. Measured (us, in a replayed graph;
 // 32 heads of 128 over 8 unless said): 4 x 4096 causal 520-540, 1000 over 30000 460-478
-// (1050-1080 TFLOP/s; a bf16 GEMM of 8192^3 1344-1433 by box), 2000 over 6000 E4M3 244
+// (1050-1080 TFLOP/s; a bf16 GEMM of 8192^3 1344-1433), 2000 over 6000 E4M3 244
 // (bf16 222; head_dim 64 179 and 150; pages of 16 291), 32 x 1 over 8000 164-169 (6.2-6.4
 // TB/s), E4M3 96, 16 x 1-4 over 8000 69-71, 1 over 32768 29, 1 over 64 6.1-6.5.
 #include <algorithm>
