@@ -337,21 +337,23 @@ NEPTUNE_API neptune_status neptune_qk_norm_rope(const neptune_rope_desc *desc, c
                                     const float *sin, const int32_t *positions,
                                     void *qo, void *ko, void *stream);
 
-/* k_pages, v_pages <- the new tokens' k (norm and rotation on the way) and v;
- * qo <- q with norm and rotation (neptune_append_desc). No counterpart in the
+/* k_pages, v_pages <- the new tokens' k (norm and rotation on the way) and v; qo
+ * <- q with norm and rotation (neptune_append_desc). No counterpart in the
  * reference. cu_seqlens [batch + 1] may be NULL: one new token per sequence
- * (tokens == batch; with it, batch is at most 65536). q, qo: NULL when heads_q is 0; qo may be q. q_weight,
- * k_weight may be NULL (no norm), cos and sin NULL when rot_dim is 0. Into E4M3
- * pools a value goes as code = RNE-saturate(x / scale), the quotient rounded to
- * fp32 first, under its page's and head's k_scales, v_scales [num_pages, heads_kv], which the caller has set (a
- * page of scale 0 takes zero codes); NULL otherwise. A row is not stored when its
- * place is negative or past its block table, or the table's entry lies outside
- * [0, num_pages); rows behind cu_seqlens[batch] are neither stored nor written to
- * qo. A place outside cos and sin is clamped into them, as in neptune_qk_norm_rope:
- * such a key is stored, turned by the last row's angles, so the tables must cover the
- * longest sequence. Two rows sent to one slot leave either. The pools and qo share no byte with
- * each other or an input (but qo may be q). head_dim 64 or 128; 16-byte aligned
- * bases and strides of whole 16-byte units. */
+ * (tokens == batch; with it, batch is at most 65536). q, qo: NULL when heads_q
+ * is 0; qo may be q. q_weight, k_weight may be NULL (no norm), cos and sin NULL
+ * when rot_dim is 0. Into E4M3 pools a value goes as code = RNE-saturate(x /
+ * scale), the quotient rounded to fp32 first, under its page's and head's
+ * k_scales, v_scales [num_pages, heads_kv], which the caller has set (a page of
+ * scale 0 takes zero codes); NULL otherwise. A row is not stored when its place
+ * is negative or past its block table, or the table's entry lies outside [0,
+ * num_pages); rows behind cu_seqlens[batch] are neither stored nor written to
+ * qo. A place outside cos and sin is clamped into them, as in
+ * neptune_qk_norm_rope: such a key is stored, turned by the last row's angles,
+ * so the tables must cover the longest sequence. Two rows sent to one slot leave
+ * either. The pools and qo share no byte with each other or an input (but qo may
+ * be q). head_dim 64 or 128; 16-byte aligned bases and strides of whole 16-byte
+ * units. */
 NEPTUNE_API neptune_status neptune_kv_append_paged(
     const neptune_append_desc *desc, const neptune_paged_kv_desc *pages, const void *k,
     const void *v, const void *q, const float *q_weight, const float *k_weight,
