@@ -55,7 +55,8 @@ typedef enum neptune_dtype {
   NEPTUNE_DTYPE_F32 = 0,
   NEPTUNE_DTYPE_F16 = 1,
   NEPTUNE_DTYPE_BF16 = 2,
-  NEPTUNE_DTYPE_FP8_E4M3 = 3 /* OCP E4M3FN: bias 7, max 448, no infinities */
+  NEPTUNE_DTYPE_FP8_E4M3 = 3, /* OCP E4M3FN: bias 7, max 448, no infinities */
+  NEPTUNE_DTYPE_MXFP4 = 4     /* OCP MXFP4: neptune_mx_desc; paged pools only */
 } neptune_dtype;
 
 /* Versioned info record, the same discovery pattern as MLIR's
@@ -140,6 +141,20 @@ typedef struct neptune_paged_kv_desc {
   int64_t v_stride[3];
 } neptune_paged_kv_desc;
 
+/* MXFP4 pools (kv_dtype NEPTUNE_DTYPE_MXFP4 of the paged entry points that take this
+ * descriptor). A head row of head_dim elements is head_dim / 2 bytes of E2M1 codes
+ * (sign, two bits of exponent, one of mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6), element 2i
+ * in the low half of byte i and 2i + 1 in the high one, and head_dim / 32 bytes e of
+ * scales: a code of elements 32 j .. 32 j + 31 stands for its value times 2^(e - 127), e
+ * byte j; e = 255 makes the 32 of them NaN. neptune_paged_kv_desc's strides are in bytes
+ * (of codes) then, multiples of 16. The scales are pools of their own: byte j of (page,
+ * kv head, position) is at page * k_stride[0] + head * k_stride[1] + position *
+ * k_stride[2] + j here (the same for V), bases and strides multiples of head_dim / 32.
+ * Products smaller than 2^-126 (float16 tensors: 2^-24) may be rounded to 0. */
+typedef struct neptune_mx_desc {
+  int64_t k_stride[3], v_stride[3]; /* bytes: page, kv head, position */
+} neptune_mx_desc;
+
 /* Mamba-1 selective scan (Gu & Dao 2023, selective_scan_fn semantics):
  *   delta = softplus(delta_raw + delta_bias[d])   (if delta_softplus)
  *   x_n  <- exp(delta * A[d,n]) x_n + delta * B[b,n,l] * u[b,d,l]
@@ -211,6 +226,27 @@ typedef struct neptune_attn_paged_desc {
   float scale_log2; /* 0 => log2(e)/sqrt(head_dim)                             */
   int32_t reserved;
 } neptune_attn_paged_desc;
+
+/* Tokens of a paged cache as rows (rows, sequences and places as in
+ * neptune_append_desc, which writes what this reads). ko, vo [tokens, heads_kv,
+ * head_dim] in dtype, (token, head) strides in elements (zero: contiguous). */
+typedef struct neptune_kv_read_desc {
+  int64_t tokens, batch, heads_kv, head_dim;
+  int64_t ko_stride[2], vo_stride[2];
+  int32_t dtype;    /* F32, F16 or BF16: ko and vo                             */
+  int32_t kv_dtype; /* the pools': F16, BF16, FP8_E4M3 or MXFP4                */
+} neptune_kv_read_desc;
+
+/* Scores that are not plain products. With x = q . k scale, a row at place p and a
+ * key at place j of its sequence, head h:
+ *   s = softcap tanh(x / softcap)       (softcap > 0; x otherwise)
+ *   s += slopes[h] (j - p)              (slopes given)
+ * and the row sees keys max(0, p - window + 1) .. p (window > 0; 0 .. p otherwise). */
+typedef struct neptune_score_desc {
+  int64_t window;  /* keys a row sees at most, its own among them; 0: all     */
+  float softcap;   /* 0: none                                                 */
+  int32_t reserved;
+} neptune_score_desc;
 
 /* ---- discovery and errors ------------------------------------------- */
 
@@ -361,7 +397,39 @@ NEPTUNE_API neptune_status neptune_kv_append_paged(
     const int32_t *cu_seqlens, const int32_t *seq_lens, void *k_pages, void *v_pages,
     const float *k_scales, const float *v_scales, void *qo, void *stream);
 
-/* Workspace of neptune_attn_paged in bytes (0: none is needed). */
+/* neptune_kv_append_paged into MXFP4 pools (desc->kv_dtype MXFP4). No counterpart in
+ * the reference. A block of 32 elements of a key (normed and rotated, in fp32) or value is
+ * quantised as it is written: its scale's byte e is the exponent of the block's largest
+ * magnitude, rounded to two significant bits, less 2 (so the largest is at most 6 scales,
+ * or cut to that from less than 7), a code the nearest of x / 2^(e - 127), halves to the
+ * even one. e is 252 at most; a block whose largest magnitude is below 2^-123 is held as
+ * zeros (e = 0), one with an infinity or NaN as NaN (e = 255). k_scales and v_scales are
+ * written where the codes are; they share no byte with each other, the pools, qo or an
+ * input. The rest is neptune_kv_append_paged's. */
+NEPTUNE_API neptune_status neptune_kv_append_paged_mx(
+    const neptune_append_desc *desc, const neptune_paged_kv_desc *pages,
+    const neptune_mx_desc *mx, const void *k, const void *v, const void *q,
+    const float *q_weight, const float *k_weight, const float *cos, const float *sin,
+    const int32_t *block_table, const int32_t *cu_seqlens, const int32_t *seq_lens,
+    void *k_pages, void *v_pages, uint8_t *k_scales, uint8_t *v_scales, void *qo, void *stream);
+
+/* ko, vo <- the tokens' keys and values as the cache holds them (neptune_kv_read_desc):
+ * 16-bit elements, code * scale otherwise, formed in fp32 and rounded once to dtype. No
+ * counterpart in the reference. k_scales, v_scales: float [num_pages, heads_kv] for E4M3
+ * pools, bytes for MXFP4 pools (mx, NULL otherwise), NULL for 16-bit ones. cu_seqlens may
+ * be NULL: one token per sequence, its last (tokens == batch; with it, batch is at most
+ * 65536). A row without a slot (a negative place, one past its block table, an entry
+ * outside [0, num_pages)) is zeros; rows behind cu_seqlens[batch] are left as they were.
+ * ko and vo share no byte with each other, the pools or their scales. head_dim 64 or 128;
+ * any page size; 16-byte aligned bases and strides of whole 16-byte units. */
+NEPTUNE_API neptune_status neptune_kv_read_paged(
+    const neptune_kv_read_desc *desc, const neptune_paged_kv_desc *pages,
+    const neptune_mx_desc *mx, const void *k_pages, const void *v_pages, const void *k_scales,
+    const void *v_scales, const int32_t *block_table, const int32_t *cu_seqlens,
+    const int32_t *seq_lens, void *ko, void *vo, void *stream);
+
+/* Workspace of neptune_attn_paged and neptune_attn_paged_ext in bytes (0: none is
+ * needed). */
 NEPTUNE_API neptune_status neptune_attn_paged_workspace_bytes(
     const neptune_attn_paged_desc *desc, size_t *bytes);
 
@@ -378,6 +446,19 @@ NEPTUNE_API neptune_status neptune_attn_paged(
     const void *k_pages, const void *v_pages, const float *k_scales, const float *v_scales,
     const int32_t *block_table, const int32_t *cu_seqlens, const int32_t *seq_lens, void *o,
     float *lse, void *workspace, size_t workspace_bytes, void *stream);
+
+/* neptune_attn_paged over pools of any kind (desc->kv_dtype dtype, FP8_E4M3 or MXFP4; mx
+ * and bytes for scales with MXFP4, dtype F16 or BF16), and with scores as in
+ * neptune_score_desc (score NULL: plain). No counterpart in the reference. slopes
+ * (nullable) [heads_q] fp32. Under the cap a score is off by some 2^-23 of itself, or of
+ * the cap where it passes half of that. The rest is neptune_attn_paged's. */
+NEPTUNE_API neptune_status neptune_attn_paged_ext(
+    const neptune_attn_paged_desc *desc, const neptune_paged_kv_desc *pages,
+    const neptune_mx_desc *mx, const neptune_score_desc *score, const void *q,
+    const void *k_pages, const void *v_pages, const void *k_scales, const void *v_scales,
+    const float *slopes, const int32_t *block_table, const int32_t *cu_seqlens,
+    const int32_t *seq_lens, void *o, float *lse, void *workspace, size_t workspace_bytes,
+    void *stream);
 
 /* ---- selective scan ---------------------------------------------------- */
 

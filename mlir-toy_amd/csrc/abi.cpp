@@ -590,11 +590,13 @@ neptune_status rope_check(const char *fn, int64_t head_dim, int64_t rot_dim, int
 }
 
 // the pools of a ragged batch's entry points
+// (mx, scales: entry points that take MXFP4 pools)
 neptune_status pools_check(const char *fn, const neptune_paged_kv_desc *pk, const void *k_pages,
-                           const void *v_pages, const float *k_scales, const float *v_scales,
+                           const void *v_pages, const void *k_scales, const void *v_scales,
                            const int32_t *block_table, const int32_t *cu_seqlens,
                            const int32_t *seq_lens, int64_t tokens, int64_t batch,
-                           int64_t heads_kv, int64_t head_dim, int32_t kv_dtype, Strided pools[2]) {
+                           int64_t heads_kv, int64_t head_dim, int32_t kv_dtype, Strided pools[2],
+                           const neptune_mx_desc *mx = nullptr, Strided *scales = nullptr) {
   if (!pk) return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: pages desc is NULL", fn);
   if (!block_table || !seq_lens)
     return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: block_table and seq_lens must be non-NULL", fn);
@@ -605,9 +607,13 @@ neptune_status pools_check(const char *fn, const neptune_paged_kv_desc *pk, cons
     return fail(NEPTUNE_ERR_INVALID_ARGUMENT,
                 "%s: without cu_seqlens a sequence has one new token: tokens %lld, batch %lld", fn,
                 (long long)tokens, (long long)batch);
-  const bool fp8 = kv_dtype == NEPTUNE_DTYPE_FP8_E4M3;
+  const bool fp8 = kv_dtype == NEPTUNE_DTYPE_FP8_E4M3, mx4 = kv_dtype == NEPTUNE_DTYPE_MXFP4;
   if (fp8 && (!k_scales || !v_scales))
     return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: E4M3 pools need k_scales and v_scales", fn);
+  if (mx4 && (!mx || !k_scales || !v_scales))
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: MXFP4 pools need mx, k_scales and v_scales", fn);
+  if (mx4 && head_dim % 32)
+    return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: MXFP4 pools need a head_dim of whole 32s", fn);
   const int64_t sizes[3] = {pk->num_pages, heads_kv, pk->page_size};
   const struct { const char *name; const void *p; const int64_t *stride; } in[2] = {
       {"k_pages", k_pages, pk->k_stride}, {"v_pages", v_pages, pk->v_stride}};
@@ -615,11 +621,34 @@ neptune_status pools_check(const char *fn, const neptune_paged_kv_desc *pk, cons
     for (int j = 0; j < 3; ++j)
       if (in[i].stride[j] <= 0)
         return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: pool strides must be positive", fn);
-    neptune_status st = resolve(fn, in[i].name, in[i].p, in[i].stride, sizes, 3, head_dim,
-                                fp8 ? 1 : 2, &pools[i]);
+    neptune_status st = resolve(fn, in[i].name, in[i].p, in[i].stride, sizes, 3,
+                                mx4 ? head_dim / 2 : head_dim, fp8 || mx4 ? 1 : 2, &pools[i]);
     if (st != NEPTUNE_OK) return st;
   }
+  if (!mx4) return NEPTUNE_OK;
+  // the scales' pools: whole rows of head_dim / 32 bytes
+  const int64_t row = head_dim / 32;
+  for (int i = 0; i < 2; ++i) {
+    Strided &t = scales[i];
+    const int64_t *stride = i ? mx->v_stride : mx->k_stride;
+    t = {i ? "v_scales" : "k_scales", i ? v_scales : k_scales, {}, {}, 3, row, 1, 0};
+    for (int j = 0; j < 3; ++j) {
+      t.size[j] = sizes[j];
+      t.stride[j] = sizes[j] == 1 ? row : stride[j];  // no step is taken along it
+      if (t.stride[j] <= 0)
+        return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: the scales' strides must be positive", fn);
+      if (t.stride[j] % row || (uintptr_t)t.p % row)
+        return fail(NEPTUNE_ERR_UNSUPPORTED,
+                    "%s: %s: base and strides must be multiples of head_dim / 32 bytes", fn, t.name);
+    }
+    t.bytes = span(t.size, t.stride, 3, row, 1);
+    if (!t.bytes) return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: %s is too large", fn, t.name);
+  }
   return NEPTUNE_OK;
+}
+
+Pool pool_of(int32_t kv_dtype) {
+  return kv_dtype == NEPTUNE_DTYPE_MXFP4 ? MXFP4 : kv_dtype == NEPTUNE_DTYPE_FP8_E4M3 ? E4M3 : WIDE;
 }
 
 // the checks of an attn_paged descriptor, and the launch it describes (no tensors)
@@ -637,14 +666,14 @@ neptune_status attn_paged_resolve(const neptune_attn_paged_desc *d, PagedAttnLau
                 (long long)d->heads_q, (long long)d->heads_kv);
   if (!is_float(d->dtype, false))
     return fail(NEPTUNE_ERR_UNSUPPORTED, "attn_paged: dtype must be F16 or BF16");
-  if (d->kv_dtype != d->dtype && d->kv_dtype != NEPTUNE_DTYPE_FP8_E4M3)
-    return fail(NEPTUNE_ERR_UNSUPPORTED, "attn_paged: kv_dtype must be dtype or FP8_E4M3");
+  if (d->kv_dtype != d->dtype && pool_of(d->kv_dtype) == WIDE)
+    return fail(NEPTUNE_ERR_UNSUPPORTED, "attn_paged: kv_dtype must be dtype, FP8_E4M3 or MXFP4");
   if (!(d->scale_log2 >= 0.0f) || !std::isfinite(d->scale_log2))
     return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "attn_paged: scale_log2 must be finite and >= 0");
   *L = PagedAttnLaunch();
   L->tokens = d->tokens; L->batch = d->batch; L->heads_q = d->heads_q; L->heads_kv = d->heads_kv;
   L->head_dim = d->head_dim; L->seq_kv = d->seq_kv; L->dtype = d->dtype;
-  L->fp8 = d->kv_dtype == NEPTUNE_DTYPE_FP8_E4M3;
+  L->pool = pool_of(d->kv_dtype);
   L->page_size = 16;
   L->scale_log2 = d->scale_log2 != 0.0f
                       ? d->scale_log2
@@ -704,15 +733,15 @@ neptune_status neptune_qk_norm_rope(const neptune_rope_desc *d, const void *q, c
   return hip_result(launch_rope(L, (hipStream_t)stream), "qk_norm_rope launch");
 }
 
-neptune_status neptune_kv_append_paged(const neptune_append_desc *d,
-                                       const neptune_paged_kv_desc *pk, const void *k,
-                                       const void *v, const void *q, const float *q_weight,
-                                       const float *k_weight, const float *cos, const float *sin,
-                                       const int32_t *block_table, const int32_t *cu_seqlens,
-                                       const int32_t *seq_lens, void *k_pages, void *v_pages,
-                                       const float *k_scales, const float *v_scales, void *qo,
-                                       void *stream) {
-  const char *fn = "kv_append_paged";
+namespace {
+// both append entry points (mx: into MXFP4 pools, whose scales are written)
+neptune_status append_run(const char *fn, const neptune_append_desc *d,
+                          const neptune_paged_kv_desc *pk, bool to_mx, const neptune_mx_desc *mx,
+                          const void *k, const void *v, const void *q, const float *q_weight,
+                          const float *k_weight, const float *cos, const float *sin,
+                          const int32_t *block_table, const int32_t *cu_seqlens,
+                          const int32_t *seq_lens, void *k_pages, void *v_pages,
+                          const void *k_scales, const void *v_scales, void *qo, void *stream) {
   if (!d) return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: desc is NULL", fn);
   if (d->tokens <= 0 || d->batch <= 0 || d->heads_q < 0 || d->heads_kv <= 0 || d->head_dim <= 0)
     return fail(NEPTUNE_ERR_INVALID_ARGUMENT,
@@ -722,14 +751,17 @@ neptune_status neptune_kv_append_paged(const neptune_append_desc *d,
                 (long long)d->heads_kv, (long long)d->head_dim);
   if (!is_float(d->dtype, false))
     return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: dtype must be F16 or BF16", fn);
-  if (d->kv_dtype != d->dtype && d->kv_dtype != NEPTUNE_DTYPE_FP8_E4M3)
-    return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: kv_dtype must be dtype or FP8_E4M3", fn);
+  if (to_mx ? d->kv_dtype != NEPTUNE_DTYPE_MXFP4
+            : d->kv_dtype != d->dtype && d->kv_dtype != NEPTUNE_DTYPE_FP8_E4M3)
+    return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: kv_dtype must be %s", fn,
+                to_mx ? "MXFP4" : "dtype or FP8_E4M3 (MXFP4: neptune_kv_append_paged_mx)");
   neptune_status st = rope_check(fn, d->head_dim, d->rot_dim, d->table_len, cos, sin, q_weight,
                                  k_weight, d->interleaved, d->eps);
   if (st != NEPTUNE_OK) return st;
-  Strided pools[2], in[3], out;
+  Strided pools[4], in[3], out;  // pools: K, V, and MXFP4's scales
+  const int n_pools = to_mx ? 4 : 2;
   st = pools_check(fn, pk, k_pages, v_pages, k_scales, v_scales, block_table, cu_seqlens, seq_lens,
-                   d->tokens, d->batch, d->heads_kv, d->head_dim, d->kv_dtype, pools);
+                   d->tokens, d->batch, d->heads_kv, d->head_dim, d->kv_dtype, pools, mx, pools + 2);
   if (st != NEPTUNE_OK) return st;
   const int64_t sq[2] = {d->tokens, d->heads_q}, sk[2] = {d->tokens, d->heads_kv};
   const int n_in = d->heads_q ? 3 : 2;
@@ -743,20 +775,28 @@ neptune_status neptune_kv_append_paged(const neptune_append_desc *d,
     for (int j = 0; j < 3; ++j)
       if (!(j == 2 && same_place(out, in[2], 2)) && (st = apart(fn, out, in[j])) != NEPTUNE_OK)
         return st;
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < n_pools; ++i)
       if ((st = apart(fn, out, pools[i])) != NEPTUNE_OK) return st;
   }
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < n_pools; ++i) {
     for (int j = 0; j < n_in; ++j)
       if ((st = apart(fn, pools[i], in[j])) != NEPTUNE_OK) return st;
-  if ((st = apart(fn, pools[0], pools[1])) != NEPTUNE_OK) return st;
+    for (int j = 0; j < i; ++j)
+      if ((st = apart(fn, pools[j], pools[i])) != NEPTUNE_OK) return st;
+  }
   RopeLaunch L;
   L.append = true;
-  L.fp8 = d->kv_dtype == NEPTUNE_DTYPE_FP8_E4M3;
+  L.pool = pool_of(d->kv_dtype);
   L.q = q; L.k = k; L.v = v; L.qo = qo; L.ko = k_pages; L.vo = v_pages;
   L.q_weight = q_weight; L.k_weight = k_weight; L.cos = cos; L.sin = sin;
   L.cu_seqlens = cu_seqlens; L.seq_lens = seq_lens; L.block_table = block_table;
-  L.k_scales = k_scales; L.v_scales = v_scales;
+  if (to_mx) {
+    L.k_bytes = (uint8_t *)k_scales;
+    L.v_bytes = (uint8_t *)v_scales;
+  } else {
+    L.k_scales = (const float *)k_scales;
+    L.v_scales = (const float *)v_scales;
+  }
   L.batch = 1; L.seq = d->tokens; L.heads_q = d->heads_q; L.heads_kv = d->heads_kv;
   L.head_dim = d->head_dim; L.rot_dim = d->rot_dim; L.table_len = d->table_len;
   L.sequences = d->batch; L.page_size = pk->page_size; L.max_pages = pk->max_pages;
@@ -776,6 +816,10 @@ neptune_status neptune_kv_append_paged(const neptune_append_desc *d,
   for (int i = 0; i < 3; ++i) {
     L.kos[i] = pools[0].stride[i];
     L.vos[i] = pools[1].stride[i];
+    if (to_mx) {
+      L.kss[i] = pools[2].stride[i];
+      L.vss[i] = pools[3].stride[i];
+    }
   }
   L.dtype = d->dtype; L.interleaved = d->interleaved; L.eps = d->eps;
   const char *why = "";
@@ -783,6 +827,98 @@ neptune_status neptune_kv_append_paged(const neptune_append_desc *d,
   st = device_ready();
   if (st != NEPTUNE_OK) return st;
   return hip_result(launch_rope(L, (hipStream_t)stream), "kv_append_paged launch");
+}
+}  // namespace
+
+neptune_status neptune_kv_append_paged(const neptune_append_desc *d,
+                                       const neptune_paged_kv_desc *pk, const void *k,
+                                       const void *v, const void *q, const float *q_weight,
+                                       const float *k_weight, const float *cos, const float *sin,
+                                       const int32_t *block_table, const int32_t *cu_seqlens,
+                                       const int32_t *seq_lens, void *k_pages, void *v_pages,
+                                       const float *k_scales, const float *v_scales, void *qo,
+                                       void *stream) {
+  return append_run("kv_append_paged", d, pk, false, nullptr, k, v, q, q_weight, k_weight, cos, sin,
+                    block_table, cu_seqlens, seq_lens, k_pages, v_pages, k_scales, v_scales, qo,
+                    stream);
+}
+
+neptune_status neptune_kv_append_paged_mx(const neptune_append_desc *d,
+                                          const neptune_paged_kv_desc *pk,
+                                          const neptune_mx_desc *mx, const void *k, const void *v,
+                                          const void *q, const float *q_weight,
+                                          const float *k_weight, const float *cos, const float *sin,
+                                          const int32_t *block_table, const int32_t *cu_seqlens,
+                                          const int32_t *seq_lens, void *k_pages, void *v_pages,
+                                          uint8_t *k_scales, uint8_t *v_scales, void *qo,
+                                          void *stream) {
+  return append_run("kv_append_paged_mx", d, pk, true, mx, k, v, q, q_weight, k_weight, cos, sin,
+                    block_table, cu_seqlens, seq_lens, k_pages, v_pages, k_scales, v_scales, qo,
+                    stream);
+}
+
+neptune_status neptune_kv_read_paged(const neptune_kv_read_desc *d, const neptune_paged_kv_desc *pk,
+                                     const neptune_mx_desc *mx, const void *k_pages,
+                                     const void *v_pages, const void *k_scales,
+                                     const void *v_scales, const int32_t *block_table,
+                                     const int32_t *cu_seqlens, const int32_t *seq_lens, void *ko,
+                                     void *vo, void *stream) {
+  const char *fn = "kv_read_paged";
+  if (!d) return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: desc is NULL", fn);
+  if (d->tokens <= 0 || d->batch <= 0 || d->heads_kv <= 0 || d->head_dim <= 0)
+    return fail(NEPTUNE_ERR_INVALID_ARGUMENT,
+                "%s: sizes must be positive (tokens=%lld batch=%lld heads_kv=%lld head_dim=%lld)",
+                fn, (long long)d->tokens, (long long)d->batch, (long long)d->heads_kv,
+                (long long)d->head_dim);
+  if (!is_float(d->dtype, true))
+    return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: dtype must be F32, F16 or BF16", fn);
+  if (!is_float(d->kv_dtype, false) && pool_of(d->kv_dtype) == WIDE)
+    return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: kv_dtype must be F16, BF16, FP8_E4M3 or MXFP4", fn);
+  Strided pools[4], out[2];
+  const Pool pool = pool_of(d->kv_dtype);
+  neptune_status st = pools_check(fn, pk, k_pages, v_pages, k_scales, v_scales, block_table,
+                                  cu_seqlens, seq_lens, d->tokens, d->batch, d->heads_kv,
+                                  d->head_dim, d->kv_dtype, pools, mx, pools + 2);
+  if (st != NEPTUNE_OK) return st;
+  const int64_t sizes[2] = {d->tokens, d->heads_kv};
+  const int64_t esize = d->dtype == NEPTUNE_DTYPE_F32 ? 4 : 2;
+  if ((st = resolve(fn, "ko", ko, d->ko_stride, sizes, 2, d->head_dim, esize, &out[0])) != NEPTUNE_OK ||
+      (st = resolve(fn, "vo", vo, d->vo_stride, sizes, 2, d->head_dim, esize, &out[1])) != NEPTUNE_OK ||
+      (st = apart(fn, out[0], out[1])) != NEPTUNE_OK)
+    return st;
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < (pool == MXFP4 ? 4 : 2); ++j)
+      if ((st = apart(fn, out[i], pools[j])) != NEPTUNE_OK) return st;
+  if (pool == E4M3) {
+    const size_t n = (size_t)pk->num_pages * (size_t)d->heads_kv * 4;
+    for (int i = 0; i < 2; ++i)
+      if (overlaps(out[i].p, out[i].bytes, k_scales, n) || overlaps(out[i].p, out[i].bytes, v_scales, n))
+        return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: %s overlaps the scales", fn, out[i].name);
+  }
+  ReadLaunch L = {};
+  L.k = k_pages; L.v = v_pages; L.k_scales = k_scales; L.v_scales = v_scales;
+  L.block_table = block_table; L.cu_seqlens = cu_seqlens; L.seq_lens = seq_lens;
+  L.ko = ko; L.vo = vo;
+  L.tokens = d->tokens; L.sequences = d->batch; L.heads_kv = d->heads_kv; L.head_dim = d->head_dim;
+  L.page_size = pk->page_size; L.max_pages = pk->max_pages; L.num_pages = pk->num_pages;
+  for (int i = 0; i < 3; ++i) {
+    L.kps[i] = pools[0].stride[i];
+    L.vps[i] = pools[1].stride[i];
+    if (pool == MXFP4) {
+      L.kss[i] = pools[2].stride[i];
+      L.vss[i] = pools[3].stride[i];
+    }
+  }
+  for (int i = 0; i < 2; ++i) {
+    L.kos[i] = out[0].stride[i];
+    L.vos[i] = out[1].stride[i];
+  }
+  L.dtype = d->dtype; L.kv_dtype = d->kv_dtype; L.pool = pool;
+  const char *why = "";
+  if (!kv_read_supported(L, &why)) return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: %s", fn, why);
+  st = device_ready();
+  if (st != NEPTUNE_OK) return st;
+  return hip_result(launch_kv_read(L, (hipStream_t)stream), "kv_read_paged launch");
 }
 
 neptune_status neptune_attn_paged_workspace_bytes(const neptune_attn_paged_desc *d,
@@ -798,20 +934,33 @@ neptune_status neptune_attn_paged_workspace_bytes(const neptune_attn_paged_desc 
   return ok();
 }
 
-neptune_status neptune_attn_paged(const neptune_attn_paged_desc *d,
-                                  const neptune_paged_kv_desc *pk, const void *q,
-                                  const void *k_pages, const void *v_pages, const float *k_scales,
-                                  const float *v_scales, const int32_t *block_table,
-                                  const int32_t *cu_seqlens, const int32_t *seq_lens, void *o,
-                                  float *lse, void *workspace, size_t workspace_bytes,
-                                  void *stream) {
-  const char *fn = "attn_paged";
+namespace {
+// both entry points; the extended one takes mx, score and slopes
+neptune_status attn_paged_run(const char *fn, const neptune_attn_paged_desc *d,
+                              const neptune_paged_kv_desc *pk, const neptune_mx_desc *mx,
+                              const neptune_score_desc *score, const void *q, const void *k_pages,
+                              const void *v_pages, const void *k_scales, const void *v_scales,
+                              const float *slopes, const int32_t *block_table,
+                              const int32_t *cu_seqlens, const int32_t *seq_lens, void *o,
+                              float *lse, void *workspace, size_t workspace_bytes, void *stream) {
   PagedAttnLaunch L;
   neptune_status st = attn_paged_resolve(d, &L);
   if (st != NEPTUNE_OK) return st;
-  Strided pools[2], tq, to;
+  if (score) {
+    if (!(score->softcap >= 0.0f) || !std::isfinite(score->softcap))
+      return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: softcap must be finite and >= 0", fn);
+    // (its inverse and products with it stay ordinary numbers)
+    if (score->softcap != 0.0f && (score->softcap < 0x1p-60f || score->softcap > 0x1p60f))
+      return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: softcap must lie between 2^-60 and 2^60", fn);
+    if (score->window < 0)
+      return fail(NEPTUNE_ERR_INVALID_ARGUMENT, "%s: window must be >= 0", fn);
+    L.softcap = score->softcap;
+    L.window = score->window;
+  }
+  L.slopes = slopes;
+  Strided pools[4], tq, to;
   st = pools_check(fn, pk, k_pages, v_pages, k_scales, v_scales, block_table, cu_seqlens, seq_lens,
-                   d->tokens, d->batch, d->heads_kv, d->head_dim, d->kv_dtype, pools);
+                   d->tokens, d->batch, d->heads_kv, d->head_dim, d->kv_dtype, pools, mx, pools + 2);
   if (st != NEPTUNE_OK) return st;
   if (pk->max_pages < cdiv(d->seq_kv, pk->page_size))
     return fail(NEPTUNE_ERR_INVALID_ARGUMENT,
@@ -824,6 +973,9 @@ neptune_status neptune_attn_paged(const neptune_attn_paged_desc *d,
       (st = apart(fn, to, pools[0])) != NEPTUNE_OK ||
       (st = apart(fn, to, pools[1])) != NEPTUNE_OK)
     return st;
+  if (L.pool == MXFP4)
+    for (int i = 2; i < 4; ++i)
+      if ((st = apart(fn, to, pools[i])) != NEPTUNE_OK) return st;
   L.q = q; L.k = k_pages; L.v = v_pages; L.k_scales = k_scales; L.v_scales = v_scales;
   L.block_table = block_table; L.cu_seqlens = cu_seqlens; L.seq_lens = seq_lens;
   L.o = o; L.lse = lse; L.workspace = workspace;
@@ -835,6 +987,10 @@ neptune_status neptune_attn_paged(const neptune_attn_paged_desc *d,
   for (int i = 0; i < 3; ++i) {
     L.kps[i] = pools[0].stride[i];
     L.vps[i] = pools[1].stride[i];
+    if (L.pool == MXFP4) {
+      L.kss[i] = pools[2].stride[i];
+      L.vss[i] = pools[3].stride[i];
+    }
   }
   const char *why = "";
   if (!attn_paged_supported(L, &why)) return fail(NEPTUNE_ERR_UNSUPPORTED, "%s: %s", fn, why);
@@ -850,6 +1006,36 @@ neptune_status neptune_attn_paged(const neptune_attn_paged_desc *d,
   if (st != NEPTUNE_OK) return st;
   return hip_result(launch_attn_paged(L, (hipStream_t)stream), "attn_paged launch");
 }
+}  // namespace
+
+neptune_status neptune_attn_paged(const neptune_attn_paged_desc *d,
+                                  const neptune_paged_kv_desc *pk, const void *q,
+                                  const void *k_pages, const void *v_pages, const float *k_scales,
+                                  const float *v_scales, const int32_t *block_table,
+                                  const int32_t *cu_seqlens, const int32_t *seq_lens, void *o,
+                                  float *lse, void *workspace, size_t workspace_bytes,
+                                  void *stream) {
+  if (d && d->kv_dtype == NEPTUNE_DTYPE_MXFP4)
+    return fail(NEPTUNE_ERR_UNSUPPORTED, "attn_paged: MXFP4 pools: neptune_attn_paged_ext");
+  return attn_paged_run("attn_paged", d, pk, nullptr, nullptr, q, k_pages, v_pages, k_scales,
+                        v_scales, nullptr, block_table, cu_seqlens, seq_lens, o, lse, workspace,
+                        workspace_bytes, stream);
+}
+
+neptune_status neptune_attn_paged_ext(const neptune_attn_paged_desc *d,
+                                      const neptune_paged_kv_desc *pk, const neptune_mx_desc *mx,
+                                      const neptune_score_desc *score, const void *q,
+                                      const void *k_pages, const void *v_pages,
+                                      const void *k_scales, const void *v_scales,
+                                      const float *slopes, const int32_t *block_table,
+                                      const int32_t *cu_seqlens, const int32_t *seq_lens, void *o,
+                                      float *lse, void *workspace, size_t workspace_bytes,
+                                      void *stream) {
+  return attn_paged_run("attn_paged_ext", d, pk, mx, score, q, k_pages, v_pages, k_scales, v_scales,
+                        slopes, block_table, cu_seqlens, seq_lens, o, lse, workspace,
+                        workspace_bytes, stream);
+}
+
 
 neptune_status neptune_selective_scan_fwd(const neptune_scan_desc *d, const void *u,
                                           const void *delta_raw, const float *A, const void *B,

@@ -36,6 +36,15 @@ struct PagedArgs {
                                   // cut tiles at most (0: no keys are cut)
   int32_t prows;                  // rows of a split item's states
   float scale2;
+  // MXFP4 pools: the scales' bytes, (page, head) and place strides
+  const uint8_t *kmx, *vmx;
+  int64_t kss0, kss1, kstok, vss0, vss1, vstok;
+  // scores that are not plain products
+  const float *slopes;            // [Hq], nullable
+  int32_t window;                 // keys a row sees at most; 0: all
+  uint32_t blocks_1;              // blocks that a tile's windows span at most, plus 1; 0: all
+  float cap2, cap_inv, capp[5];   // the cap in log2 units (0: none), its inverse, tanh(y) / y
+                                  // times the cap as a polynomial of y^2
 };
 
 // floor(x / d), inv = floor((2^32 - 1) / d): the estimate is that or one less
@@ -79,7 +88,8 @@ __device__ inline Seq sequence(const PagedArgs &a, int b) {
   s.row0 = lo;
   s.len = b < a.B ? min(max(len, 0), a.Lmax) : 0;
   s.tiles = (s.n * a.group + BM - 1) / BM;
-  s.blocks = (s.len + BN - 1) / BN;
+  // those that count for the cut (0 - 1: no bound)
+  s.blocks = (int)min((uint32_t)((s.len + BN - 1) / BN), a.blocks_1 - 1u);
   return s;
 }
 

@@ -63,6 +63,11 @@ struct ScanLaunch {
   int32_t delta_softplus;
 };
 
+// What a paged cache's pools hold: 16-bit elements, E4M3 codes under a float for each
+// page and head, or MXFP4: E2M1 codes (two to a byte, strides in bytes) under a byte for
+// each 32 elements of a row, 2^(byte - 127) or NaN (255).
+enum Pool : int32_t { WIDE = 0, E4M3 = 1, MXFP4 = 2 };
+
 // qk_norm_rope, and (append) kv_append_paged: tokens as one batch of `seq` rows,
 // ko and vo the pools, kos and vos their (page, head, place) strides.
 struct RopeLaunch {
@@ -72,20 +77,36 @@ struct RopeLaunch {
   const int32_t *positions = nullptr;                                  // qk_norm_rope
   const int32_t *cu_seqlens = nullptr, *seq_lens = nullptr, *block_table = nullptr;  // append
   const float *k_scales = nullptr, *v_scales = nullptr;                // E4M3 pools
+  uint8_t *k_bytes = nullptr, *v_bytes = nullptr;                      // MXFP4 pools' scales
   int64_t batch = 0, heads_q = 0, heads_kv = 0, seq = 0, head_dim = 0;
   int64_t rot_dim = 0, table_len = 0;
   int64_t sequences = 0, page_size = 1, max_pages = 0, num_pages = 0;
   // (batch, head, seq) strides, elements
   int64_t qs[3] = {}, ks[3] = {}, vs[3] = {}, qos[3] = {}, kos[3] = {}, vos[3] = {};
+  int64_t kss[3] = {}, vss[3] = {};  // MXFP4: the scales' (page, head, place) strides, bytes
   int32_t dtype = 0, interleaved = 0;
   float eps = 0.0f;
-  bool append = false, fp8 = false;
+  bool append = false;
+  Pool pool = WIDE;
+};
+
+// kv_read_paged: tokens out of a paged cache, as rows
+struct ReadLaunch {
+  const void *k, *v, *k_scales, *v_scales;
+  const int32_t *block_table, *cu_seqlens, *seq_lens;  // cu_seqlens nullable
+  void *ko, *vo;
+  int64_t tokens, sequences, heads_kv, head_dim;
+  int64_t page_size, max_pages, num_pages;
+  int64_t kps[3], vps[3], kss[3], vss[3];  // (page, head, place), elements; scales: bytes
+  int64_t kos[2], vos[2];                  // (token, head), elements
+  int32_t dtype, kv_dtype;                 // kv_dtype: of 16-bit pools
+  Pool pool;
 };
 
 // Attention of a ragged batch of new tokens over a paged cache.
 struct PagedAttnLaunch {
   const void *q, *k, *v;
-  const float *k_scales, *v_scales;  // E4M3 pools
+  const void *k_scales, *v_scales;  // E4M3: floats by page and head; MXFP4: bytes by block
   const int32_t *block_table, *cu_seqlens, *seq_lens;  // cu_seqlens nullable
   void *o;
   float *lse;  // nullable
@@ -93,10 +114,15 @@ struct PagedAttnLaunch {
   int64_t tokens, batch, heads_q, heads_kv, seq_kv, head_dim;
   int64_t qs[2], os[2];          // (token, head) strides, elements
   int64_t kps[3], vps[3];        // (page, head, place) strides, elements
+  int64_t kss[3], vss[3];        // MXFP4: the scales' (page, head, place) strides, bytes
   int64_t page_size, max_pages, num_pages;
   int32_t dtype;
-  bool fp8;
+  Pool pool;
   float scale_log2;
+  // scores that are not plain products
+  const float *slopes;  // [heads_q], nullable
+  float softcap;        // 0: none
+  int64_t window;       // 0: none
 };
 
 // Bytes of the static device scratch behind neptune_decode_splitk_noalloc
@@ -116,7 +142,11 @@ hipError_t launch_decode(const DecodeLaunch &a, hipStream_t s);
 hipError_t launch_kv_quantize(const QuantLaunch &a, hipStream_t s);
 hipError_t launch_selective_scan(const ScanLaunch &a, hipStream_t s);
 hipError_t launch_rope(const RopeLaunch &a, hipStream_t s);
+hipError_t launch_kv_read(const ReadLaunch &a, hipStream_t s);
 hipError_t launch_attn_paged(const PagedAttnLaunch &a, hipStream_t s);
+// (its part over MXFP4 pools, and of capped, biased or windowed scores over others)
+hipError_t launch_attn_paged_mx(const PagedAttnLaunch &a, hipStream_t s);
+hipError_t launch_attn_paged_shaped(const PagedAttnLaunch &a, hipStream_t s);
 
 // Workspace of a launch for the states of split keys (0: it splits none).
 size_t attn_paged_bytes(const PagedAttnLaunch &a);
@@ -130,6 +160,7 @@ bool attn_supported(const AttnLaunch &a, const char **why);
 bool decode_supported(const DecodeLaunch &a, const char **why);
 bool scan_supported(const ScanLaunch &a, const char **why);
 bool rope_supported(const RopeLaunch &a, const char **why);
+bool kv_read_supported(const ReadLaunch &a, const char **why);
 bool attn_paged_supported(const PagedAttnLaunch &a, const char **why);
 
 }  // namespace neptune

@@ -30,6 +30,7 @@
 
 #include "device_common.h"
 #include "kernels.h"
+#include "paged_rows.h"
 
 namespace neptune {
 namespace {
@@ -78,6 +79,8 @@ struct RopeSide {
   const char *in;
   char *out;
   const float *w, *scales;  // norm weight; scales of an E4M3 pool (nullable)
+  uint8_t *bytes;           // scales of an MXFP4 pool
+  int64_t ss[3];            // their strides (page, head, place), bytes
   int64_t is[3], os[3];     // byte strides (batch, head, token); pool (page, head, place)
   int32_t heads, runs;      // runs: groups of lanes per token
   uint32_t runs_inv;
@@ -95,12 +98,6 @@ struct RopeArgs {
   int32_t B, ps, maxp, npages;
   float eps, inv_dim;
 };
-
-// floor(x / d), inv = floor((2^32 - 1) / d): the estimate is that or one less
-__device__ inline uint32_t divide(uint32_t x, uint32_t d, uint32_t inv) {
-  const uint32_t q = __umulhi(x, inv);
-  return x - q * d >= d ? q + 1 : q;
-}
 
 // sum over aligned groups of N (4, 8 or 16) lanes, in every lane: DPP moves
 template <int N>
@@ -169,12 +166,46 @@ __device__ inline u32x2 codes8(f32x4 a, f32x4 b, float scale) {
   return c;
 }
 
+// max over aligned groups of four lanes, in every lane
+__device__ inline uint32_t quad_max(uint32_t x) {
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xb1, 0xf, 0xf, true));
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4e, 0xf, 0xf, true));
+}
+
+// Eight E2M1 codes of a lane's values and the scale's byte of its block, four lanes'. The
+// scale is 2^(e - 2), e the exponent of the block's largest magnitude rounded to the two
+// significant bits that a code has: below 7 / 4 of its power of two the largest is 6
+// scales and less, or passes 6 by less than a sixth and becomes 6; from 7 / 4 on, the
+// next scale, it is 3.5 and more. (Without that rounding magnitudes up to 8 scales would
+// become 6.) A block below 2^-123 is held as zeros, one with an infinity or NaN as NaN.
+__device__ inline uint32_t mx8(f32x4 a, f32x4 b, uint32_t *byte) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    top = max(top, __float_as_uint(a[i]) & 0x7fffffffu);
+    top = max(top, __float_as_uint(b[i]) & 0x7fffffffu);
+  }
+  top = quad_max(top);
+  const uint32_t e = top >= 0x7f800000u  ? 255u
+                     : top < 0x02000000u ? 0u
+                                         : min(((top + 0x200000u) >> 23) - 2u, 252u);
+  const float s = __uint_as_float(e << 23);
+  uint32_t c = 0;  // nearest, halves to even, saturated
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, a[0], a[1], s, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, a[2], a[3], s, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, b[0], b[1], s, 2);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, b[2], b[3], s, 3);
+  *byte = e;
+  return e == 0u || e == 255u ? 0u : c;
+}
+
 // KIND: 0 queries, 1 keys, 2 values
-template <class E, int D, bool APPEND, bool FP8, int HPG, int KIND>
+template <class E, int D, bool APPEND, int POOL, int HPG, int KIND>
 __device__ inline void rows(const RopeArgs &a) {
   typedef typename E::raw raw;
   constexpr int LPR = D / 8;
   constexpr bool TO_POOL = APPEND && KIND > 0;
+  constexpr bool FP8 = POOL == E4M3, MX = POOL == MXFP4 && TO_POOL;
   const int lane = threadIdx.x & 63, l = threadIdx.x % LPR;
   const RopeSide &x = a.side[KIND];
   const uint32_t gid = (blockIdx.x - x.first) * (NT / LPR) + threadIdx.x / LPR;
@@ -188,14 +219,29 @@ __device__ inline void rows(const RopeArgs &a) {
   // tokens, one head a group.)
   const int t0 = APPEND ? 0 : (int)divide(tok, a.S, a.S_inv), t1 = APPEND ? tok : tok - t0 * a.S;
   int t, page = -1, place = 0, end = 0x7fffffff;
-  const int chunk = (a.B + 63) >> 6;  // sequences a lane stands for in the search
   if constexpr (APPEND)
-    if (a.cu && lane * chunk < a.B) end = a.cu[min((lane + 1) * chunk, a.B)];
+    if (a.cu) end = chunk_end(a.cu, a.B, lane);
 
   // this lane's two runs of four elements, the rotated ones' pairs 4l ..; flat: all
   // lanes' runs are neighbours
-  const bool flat = KIND == 2 || a.interleaved || a.half == 0;
+  const bool flat = KIND == 2 || a.interleaved || a.half == 0 || MX;
   const bool turns = KIND < 2 && 4 * l < a.half;
+  // MXFP4: a block's 32 elements are four lanes', so keys keep their order here, and a
+  // run's partners (half-split pairs) are loaded beside it: run i of the lane, its
+  // element e, has its partner at e + half or e - half
+  const bool beside = MX && KIND == 1 && !a.interleaved && a.half > 0;
+  int poff[2] = {}, pair[2] = {};
+  bool pairs[2] = {}, upper[2] = {};
+  if constexpr (MX && KIND == 1) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int e = 8 * l + 4 * i;
+      pairs[i] = beside && e < 2 * a.half;
+      upper[i] = e >= a.half;
+      pair[i] = pairs[i] ? (upper[i] ? e - a.half : e) : 0;
+      poff[i] = !pairs[i] ? e : upper[i] ? e - a.half : e + a.half;
+    }
+  }
   const int offa = turns && !flat ? 4 * l : 8 * l;
   const int offb = turns && !flat ? 4 * l + a.half : 8 * l + 4;
   const char *src = x.in + (APPEND ? 0 : t0 * x.is[0]) + t1 * x.is[2];
@@ -212,35 +258,23 @@ __device__ inline void rows(const RopeArgs &a) {
     }
   }
 
+  raw ua[MX ? HPG : 1], ub[MX ? HPG : 1];  // the partners' runs
+  if constexpr (MX && KIND == 1) {
+    if (beside) {
+#pragma unroll
+      for (int i = 0; i < HPG; ++i) {
+        ua[i] = *(const raw *)(row_in(i) + poff[0] * E::SIZE);
+        ub[i] = *(const raw *)(row_in(i) + poff[1] * E::SIZE);
+      }
+    }
+  }
+
   float scale[HPG];
   if constexpr (!APPEND) t = a.pos[tok];
   if constexpr (APPEND) {
     int b = tok, left = 1;
     if (a.cu) {
-      // the sequence: as many ends lie at or before the row. Among 64 ends of whole
-      // chunks, then among those of the chunk that the row is in (1024
-      // single tokens 6.9 us, 2048 10.6; with a step per 64 sequences 9.7 and 19.3)
-      constexpr int GROUPS = 64 / LPR;
-      int row[GROUPS], at[GROUPS];
-      b = 0;
-#pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        row[g] = __builtin_amdgcn_readlane(tok, g * LPR);
-        at[g] = chunk * __builtin_popcountll(__ballot(end <= row[g]));
-        if (lane / LPR == g) b = at[g];
-      }
-      if (chunk > 1)
-        for (int j = lane; j - lane < chunk; j += 64) {
-          int ends[GROUPS];
-#pragma unroll
-          for (int g = 0; g < GROUPS; ++g)
-            ends[g] = j < chunk && at[g] + j < a.B ? a.cu[at[g] + j + 1] : 0x7fffffff;
-#pragma unroll
-          for (int g = 0; g < GROUPS; ++g) {
-            const int n = __builtin_popcountll(__ballot(ends[g] <= row[g]));
-            if (lane / LPR == g) b += n;
-          }
-        }
+      b = sequence_of<LPR>(a.cu, a.B, lane, tok, end);
       live = live && b < a.B && a.cu[0] <= tok;  // rows behind the last sequence stay as they were
       b = min(b, a.B - 1);
       left = a.cu[b + 1] - tok;
@@ -252,7 +286,7 @@ __device__ inline void rows(const RopeArgs &a) {
       if (t >= 0 && index < a.maxp) page = a.btab[(int64_t)b * a.maxp + index];
       // a key or value without a slot is not stored
       live = live && page >= 0 && page < a.npages;
-      if constexpr (FP8)
+      if constexpr (FP8 && TO_POOL)
 #pragma unroll
         for (int i = 0; i < HPG; ++i)
           scale[i] = live ? x.scales[(int64_t)page * x.heads + min(run + i * x.runs, x.heads - 1)]
@@ -266,17 +300,38 @@ __device__ inline void rows(const RopeArgs &a) {
   if constexpr (KIND < 2) {
     // all four loads are in flight before the first is waited for
     f32x4 c = pa, s = qa;
-    if (a.half) {
+    if (beside) {
+      const int64_t row = (int64_t)min(max(t, 0), a.P - 1) * a.half;
+      f32x4 cb = *(const f32x4 *)(a.cos + row + pair[1]), sb = *(const f32x4 *)(a.sin + row + pair[1]);
+      c = *(const f32x4 *)(a.cos + row + pair[0]);
+      s = *(const f32x4 *)(a.sin + row + pair[0]);
+      qa = qb = f32x4{1, 1, 1, 1};
+      if (x.w) {
+        pa = *(const f32x4 *)(x.w + offa);
+        pb = *(const f32x4 *)(x.w + offb);
+        qa = *(const f32x4 *)(x.w + poff[0]);
+        qb = *(const f32x4 *)(x.w + poff[1]);
+      }
+      asm volatile("" : "+v"(c), "+v"(s), "+v"(cb), "+v"(sb), "+v"(pa), "+v"(pb), "+v"(qa), "+v"(qb));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        pa[j] *= pairs[0] ? c[j] : 1.0f;
+        pb[j] *= pairs[1] ? cb[j] : 1.0f;
+        qa[j] *= upper[0] ? s[j] : -s[j];
+        qb[j] *= upper[1] ? sb[j] : -sb[j];
+      }
+    }
+    if (!beside && a.half) {
       const int64_t row = (int64_t)min(max(t, 0), a.P - 1) * a.half + min(4 * l, a.half - 4);
       c = *(const f32x4 *)(a.cos + row);
       s = *(const f32x4 *)(a.sin + row);
     }
-    if (x.w) {
+    if (!beside && x.w) {
       pa = *(const f32x4 *)(x.w + offa);
       pb = *(const f32x4 *)(x.w + offb);
     }
     asm volatile("" : "+v"(c), "+v"(s), "+v"(pa), "+v"(pb));
-    if (turns) {
+    if (turns && !beside) {
       if (a.interleaved) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -322,7 +377,13 @@ __device__ inline void rows(const RopeArgs &a) {
         const float oa = a.interleaved ? ya[j ^ 1] : yb[j], ob = a.interleaved ? yb[j ^ 1] : ya[j];
         za[j] = ya[j] * pa[j];
         zb[j] = yb[j] * pb[j];
-        if (turns) {
+        if (beside) {
+          if constexpr (MX) {
+            const f32x4 oa = E::load(ua[i]), ob = E::load(ub[i]);
+            if (pairs[0]) za[j] = fmaf(oa[j], qa[j], za[j]);
+            if (pairs[1]) zb[j] = fmaf(ob[j], qb[j], zb[j]);
+          }
+        } else if (turns) {
           za[j] = fmaf(oa, qa[j], za[j]);
           zb[j] = fmaf(ob, qb[j], zb[j]);
         }
@@ -330,9 +391,30 @@ __device__ inline void rows(const RopeArgs &a) {
       ya = za * r;
       yb = zb * r;
     }
+    uint32_t codes = 0, bytes = 0;
+    if constexpr (MX) {
+      codes = mx8(ya, yb, &bytes);
+      // the row's scales, a byte for each four lanes
+      bytes <<= 8 * (l >> 2);
+      if constexpr (LPR == 16) {
+        bytes |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)bytes, 0x124, 0xf, 0xf, true);  // row_ror 4
+        bytes |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)bytes, 0x128, 0xf, 0xf, true);  // row_ror 8
+      } else {
+        bytes |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)bytes, 0x141, 0xf, 0xf, true);  // row_half_mirror
+      }
+    }
     if (!live || h >= x.heads) continue;
     char *p = dst + h * x.os[1];
-    if constexpr (FP8 && TO_POOL) {
+    if constexpr (MX) {
+      *(uint32_t *)(p + 4 * l) = codes;
+      uint8_t *to = x.bytes + page * x.ss[0] + place * x.ss[2] + h * x.ss[1];
+      if (l == 0) {
+        if constexpr (LPR == 16)
+          *(uint32_t *)to = bytes;
+        else
+          *(uint16_t *)to = (uint16_t)bytes;
+      }
+    } else if constexpr (FP8 && TO_POOL) {
       const u32x2 c = codes8(ya, yb, scale[i]);
       if (flat) {
         *(u32x2 *)(p + 8 * l) = c;
@@ -351,17 +433,17 @@ __device__ inline void rows(const RopeArgs &a) {
   }
 }
 
-template <class E, int D, bool APPEND, bool FP8, int HPG>
+template <class E, int D, bool APPEND, int POOL, int HPG>
 __global__ __launch_bounds__(NT) void norm_rope(RopeArgs a) {
   if (blockIdx.x < a.side[1].first)
-    rows<E, D, APPEND, FP8, HPG, 0>(a);
+    rows<E, D, APPEND, POOL, HPG, 0>(a);
   else if (!APPEND || blockIdx.x < a.side[2].first)
-    rows<E, D, APPEND, FP8, HPG, 1>(a);
+    rows<E, D, APPEND, POOL, HPG, 1>(a);
   else if constexpr (APPEND)
-    rows<E, D, APPEND, FP8, HPG, 2>(a);
+    rows<E, D, APPEND, POOL, HPG, 2>(a);
 }
 
-template <class E, int D, bool APPEND, bool FP8>
+template <class E, int D, bool APPEND, int POOL>
 hipError_t launch_hpg(RopeArgs a, hipStream_t s) {
   constexpr int GPB = NT / (D / 8);  // groups of lanes per work-group
   auto go = [&](auto H) {
@@ -375,7 +457,7 @@ hipError_t launch_hpg(RopeArgs a, hipStream_t s) {
       x.runs_inv = 0xffffffffu / (uint32_t)x.runs;
       blocks += (uint32_t)(((int64_t)a.tokens * x.runs + GPB - 1) / GPB);
     }
-    hipLaunchKernelGGL((norm_rope<E, D, APPEND, FP8, HPG>), dim3(blocks), dim3(NT), 0, s, a);
+    hipLaunchKernelGGL((norm_rope<E, D, APPEND, POOL, HPG>), dim3(blocks), dim3(NT), 0, s, a);
   };
   // Several heads a group spare it most of its instructions, but leave fewer
   // work-groups: from 8 for every CU on. Measured (us, 1 / 2 / 4 / 8 heads): 16384
@@ -392,19 +474,22 @@ hipError_t launch_hpg(RopeArgs a, hipStream_t s) {
 }
 
 template <class E, int D>
-hipError_t launch_d(const RopeArgs &a, bool append, bool fp8, hipStream_t s) {
+hipError_t launch_d(const RopeArgs &a, bool append, Pool pool, hipStream_t s) {
   if constexpr (E::SIZE == 2 && D >= 64) {
-    if (append) return fp8 ? launch_hpg<E, D, true, true>(a, s) : launch_hpg<E, D, true, false>(a, s);
+    if (append)
+      return pool == MXFP4  ? launch_hpg<E, D, true, MXFP4>(a, s)
+             : pool == E4M3 ? launch_hpg<E, D, true, E4M3>(a, s)
+                            : launch_hpg<E, D, true, WIDE>(a, s);
   }
-  return launch_hpg<E, D, false, false>(a, s);
+  return launch_hpg<E, D, false, WIDE>(a, s);
 }
 
 template <class E>
-hipError_t launch_e(const RopeArgs &a, int64_t head_dim, bool append, bool fp8, hipStream_t s) {
+hipError_t launch_e(const RopeArgs &a, int64_t head_dim, bool append, Pool pool, hipStream_t s) {
   switch (head_dim) {
-    case 32: return launch_d<E, 32>(a, append, fp8, s);
-    case 64: return launch_d<E, 64>(a, append, fp8, s);
-    default: return launch_d<E, 128>(a, append, fp8, s);
+    case 32: return launch_d<E, 32>(a, append, pool, s);
+    case 64: return launch_d<E, 64>(a, append, pool, s);
+    default: return launch_d<E, 128>(a, append, pool, s);
   }
 }
 
@@ -446,10 +531,16 @@ bool rope_supported(const RopeLaunch &L, const char **why) {
 
 hipError_t launch_rope(const RopeLaunch &L, hipStream_t s) {
   RopeArgs a = {};
-  const int64_t size = L.dtype == 0 ? 4 : 2, kv = L.fp8 ? 1 : size;
+  const int64_t size = L.dtype == 0 ? 4 : 2, kv = L.pool == WIDE ? size : 1;
   a.side[0] = {(const char *)L.q, (char *)L.qo, L.q_weight, nullptr};
   a.side[1] = {(const char *)L.k, (char *)L.ko, L.k_weight, L.k_scales};
   a.side[2] = {(const char *)L.v, (char *)L.vo, nullptr, L.v_scales};
+  a.side[1].bytes = L.k_bytes;
+  a.side[2].bytes = L.v_bytes;
+  for (int j = 0; j < 3; ++j) {
+    a.side[1].ss[j] = L.kss[j];
+    a.side[2].ss[j] = L.vss[j];
+  }
   const int64_t *const in[3] = {L.qs, L.ks, L.vs}, *const out[3] = {L.qos, L.kos, L.vos};
   for (int i = 0; i < 3; ++i) {
     a.side[i].heads = (int32_t)(i ? L.heads_kv : L.heads_q);
@@ -472,9 +563,9 @@ hipError_t launch_rope(const RopeLaunch &L, hipStream_t s) {
   a.npages = (int32_t)L.num_pages;
   a.eps = L.eps;
   a.inv_dim = 1.0f / (float)L.head_dim;
-  if (L.dtype == 0) return launch_e<F32Elem>(a, L.head_dim, false, false, s);
-  if (L.dtype == 1) return launch_e<Elem16<F16Tag>>(a, L.head_dim, L.append, L.fp8, s);
-  return launch_e<Elem16<Bf16Tag>>(a, L.head_dim, L.append, L.fp8, s);
+  if (L.dtype == 0) return launch_e<F32Elem>(a, L.head_dim, false, WIDE, s);
+  if (L.dtype == 1) return launch_e<Elem16<F16Tag>>(a, L.head_dim, L.append, L.pool, s);
+  return launch_e<Elem16<Bf16Tag>>(a, L.head_dim, L.append, L.pool, s);
 }
 
 }  // namespace neptune

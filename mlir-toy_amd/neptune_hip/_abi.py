@@ -33,6 +33,7 @@ DTYPE_F32 = 0
 DTYPE_F16 = 1
 DTYPE_BF16 = 2
 DTYPE_FP8_E4M3 = 3
+DTYPE_MXFP4 = 4
 
 # every entry point the header declares (checked by the CPU test suite)
 EXPORTED_SYMBOLS = (
@@ -50,8 +51,11 @@ EXPORTED_SYMBOLS = (
     "neptune_kv_quantize_fp8",
     "neptune_qk_norm_rope",
     "neptune_kv_append_paged",
+    "neptune_kv_append_paged_mx",
+    "neptune_kv_read_paged",
     "neptune_attn_paged_workspace_bytes",
     "neptune_attn_paged",
+    "neptune_attn_paged_ext",
     "neptune_selective_scan_fwd",
 )
 
@@ -172,6 +176,40 @@ class AttnPagedDesc(ctypes.Structure):
         ("dtype", ctypes.c_int32),
         ("kv_dtype", ctypes.c_int32),
         ("scale_log2", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class MxDesc(ctypes.Structure):
+    """include/neptune_hip.h: neptune_mx_desc"""
+
+    _fields_ = [
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
+    ]
+
+
+class KvReadDesc(ctypes.Structure):
+    """include/neptune_hip.h: neptune_kv_read_desc"""
+
+    _fields_ = [
+        ("tokens", ctypes.c_int64),
+        ("batch", ctypes.c_int64),
+        ("heads_kv", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("ko_stride", ctypes.c_int64 * 2),
+        ("vo_stride", ctypes.c_int64 * 2),
+        ("dtype", ctypes.c_int32),
+        ("kv_dtype", ctypes.c_int32),
+    ]
+
+
+class ScoreDesc(ctypes.Structure):
+    """include/neptune_hip.h: neptune_score_desc"""
+
+    _fields_ = [
+        ("window", ctypes.c_int64),
+        ("softcap", ctypes.c_float),
         ("reserved", ctypes.c_int32),
     ]
 
@@ -304,6 +342,19 @@ def _declare(lib: ctypes.CDLL) -> None:
         ctypes.POINTER(AttnPagedDesc), ctypes.POINTER(PagedKvDesc),
     ] + [vp] * 11 + [ctypes.c_size_t, vp]
     lib.neptune_attn_paged.restype = i32
+    lib.neptune_kv_append_paged_mx.argtypes = [
+        ctypes.POINTER(AppendDesc), ctypes.POINTER(PagedKvDesc), ctypes.POINTER(MxDesc),
+    ] + [vp] * 16
+    lib.neptune_kv_append_paged_mx.restype = i32
+    lib.neptune_kv_read_paged.argtypes = [
+        ctypes.POINTER(KvReadDesc), ctypes.POINTER(PagedKvDesc), ctypes.POINTER(MxDesc),
+    ] + [vp] * 10
+    lib.neptune_kv_read_paged.restype = i32
+    lib.neptune_attn_paged_ext.argtypes = [
+        ctypes.POINTER(AttnPagedDesc), ctypes.POINTER(PagedKvDesc), ctypes.POINTER(MxDesc),
+        ctypes.POINTER(ScoreDesc),
+    ] + [vp] * 12 + [ctypes.c_size_t, vp]
+    lib.neptune_attn_paged_ext.restype = i32
     lib.neptune_selective_scan_fwd.argtypes = [
         ctypes.POINTER(ScanDesc), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp,
     ]

@@ -524,18 +524,46 @@ def _strides_th(name, meta, heads, head_dim, tokens, dtype) -> tuple[int, int]:
     return stride[:2]
 
 
+_E2M1 = getattr(torch, "float4_e2m1fn_x2", None)
+_E8M0 = getattr(torch, "float8_e8m0fnu", None)
+
+
+def _is_mx(k_pages, k_scales) -> bool:
+    """MXFP4 pools: bytes of codes whose scales are bytes too, or torch's types."""
+    if _E2M1 is not None and k_pages[2] == _E2M1:
+        return True
+    return k_pages[2] == torch.uint8 and k_scales is not None and \
+        k_scales[2] in (torch.uint8, _E8M0)
+
+
+def _mx_plan(name, k_pages, v_pages, k_scales, v_scales) -> _abi.MxDesc:
+    """The scales' descriptor, checked with the pools'."""
+    npages, Hk, psize, half = k_pages[0]
+    want = (npages, Hk, psize, half // 16)
+    for what, m in (("k_scales", k_scales), ("v_scales", v_scales)):
+        if m is None or m[2] not in (torch.uint8, _E8M0) or tuple(m[0]) != want or m[1][-1] != 1:
+            raise ValueError(f"{name}: MXFP4 pools need {what}: a uint8 view {list(want)}, the last "
+                             "axis contiguous")
+    mx = _abi.MxDesc()
+    mx.k_stride[:] = k_scales[1][:3]
+    mx.v_stride[:] = v_scales[1][:3]
+    return mx
+
+
 def _pool_plan(name, dtype, tokens, k_pages, v_pages, block_table, seq_lens, cu_seqlens,
                k_scales, v_scales):
-    """(page descriptor, neptune dtype of the pools, batch) of a ragged batch."""
-    fp8 = k_pages[2] in (torch.uint8, torch.float8_e4m3fn)
+    """(page descriptor, neptune dtype of the pools, batch, head_dim, MXFP4 descriptor or
+    None) of a ragged batch."""
+    mx = _is_mx(k_pages, k_scales)
+    fp8 = not mx and k_pages[2] in (torch.uint8, torch.float8_e4m3fn)
     if dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"{name} takes float16 or bfloat16 tensors")
-    if k_pages[2] != v_pages[2] or not (fp8 or k_pages[2] == dtype):
-        raise ValueError(f"{name}: the pools must be {dtype} or E4M3, both alike")
+    if k_pages[2] != v_pages[2] or not (fp8 or mx or k_pages[2] == dtype):
+        raise ValueError(f"{name}: the pools must be {dtype}, E4M3 or MXFP4, both alike")
     if len(k_pages[0]) != 4 or k_pages[0] != v_pages[0] or k_pages[1][-1] != 1 or \
             v_pages[1][-1] != 1:
         raise ValueError("k_pages / v_pages: matching [pages, Hkv, page_size, D] views, D contiguous")
-    npages, Hk, psize, _ = k_pages[0]
+    npages, Hk, psize, width = k_pages[0]
     if len(block_table[0]) != 2:
         raise ValueError("block_table must be [B, max_pages]")
     B, max_pages = block_table[0]
@@ -556,23 +584,26 @@ def _pool_plan(name, dtype, tokens, k_pages, v_pages, block_table, seq_lens, cu_
             if m is None or m[2] != torch.float32 or not _contiguous(m) or \
                     tuple(m[0]) != (npages, Hk):
                 raise ValueError(f"fp8 pages need {what}: contiguous float32 [num_pages, Hkv]")
-    elif k_scales is not None or v_scales is not None:
-        raise ValueError("k_scales / v_scales apply to E4M3 pools only")
+    elif not mx and (k_scales is not None or v_scales is not None):
+        raise ValueError("k_scales / v_scales apply to MXFP4 and E4M3 pools only")
     pk = _abi.PagedKvDesc()
     pk.num_pages, pk.page_size, pk.max_pages = npages, psize, max_pages
     pk.k_stride[:] = k_pages[1][:3]
     pk.v_stride[:] = v_pages[1][:3]
-    return pk, _abi.DTYPE_FP8_E4M3 if fp8 else _TORCH_TO_DTYPE[dtype], B
+    if mx:
+        return (pk, _abi.DTYPE_MXFP4, B, 2 * width,
+                _mx_plan(name, k_pages, v_pages, k_scales, v_scales))
+    return pk, _abi.DTYPE_FP8_E4M3 if fp8 else _TORCH_TO_DTYPE[dtype], B, width, None
 
 
 @functools.lru_cache(maxsize=_PLANS, typed=True)
 def _append_plan(k, v, k_pages, v_pages, block_table, seq_lens, cu_seqlens, q, cos, sin, q_weight,
                  k_weight, k_scales, v_scales, out, eps, interleaved):
-    """(descriptor, page descriptor)."""
+    """(descriptor, page descriptor, MXFP4 descriptor or None)."""
     T = k[0][0] if len(k[0]) == 3 else 0
-    pk, kv_dtype, B = _pool_plan("kv_append_paged", k[2], T, k_pages, v_pages, block_table,
-                                 seq_lens, cu_seqlens, k_scales, v_scales)
-    _, Hk, _, D = k_pages[0]
+    pk, kv_dtype, B, D, mx = _pool_plan("kv_append_paged", k[2], T, k_pages, v_pages, block_table,
+                                        seq_lens, cu_seqlens, k_scales, v_scales)
+    Hk = k_pages[0][1]
     desc = _abi.AppendDesc()
     desc.k_stride[:] = _strides_th("k", k, Hk, D, T, k[2])
     desc.v_stride[:] = _strides_th("v", v, Hk, D, T, k[2])
@@ -592,7 +623,7 @@ def _append_plan(k, v, k_pages, v_pages, block_table, seq_lens, cu_seqlens, q, c
     desc.rot_dim, desc.table_len = rot, rows
     desc.dtype, desc.kv_dtype = _TORCH_TO_DTYPE[k[2]], kv_dtype
     desc.interleaved, desc.eps = interleaved, eps
-    return ctypes.byref(desc), ctypes.byref(pk)
+    return ctypes.byref(desc), ctypes.byref(pk), None if mx is None else ctypes.byref(mx)
 
 
 def kv_append_paged(
@@ -624,8 +655,16 @@ def kv_append_paged(
     [num_pages, Hkv, page_size, D] views as in ``decode_paged``, of k's dtype or
     E4M3 codes under the given k_scales / v_scales [num_pages, Hkv] (of either
     dtype's values: ``attention_paged`` and ``decode_paged`` read codes with
-    bfloat16 queries, a float16 model casts its own); block_table
+    bfloat16 queries, a float16 model casts its own), or MXFP4; block_table
     [B, max_pages], seq_lens [B], cu_seqlens [B + 1] int32 on the device.
+
+    MXFP4 pools hold four bits an element: k_pages / v_pages [num_pages, Hkv,
+    page_size, D / 2] of bytes (uint8, or torch.float4_e2m1fn_x2), two E2M1 codes each,
+    the even element's in the low half, and k_scales / v_scales [num_pages, Hkv,
+    page_size, D / 32] of bytes (uint8, or torch.float8_e8m0fnu), the scale 2^(e - 127)
+    of 32 elements each (255: NaN), views of any page/head/position strides alike. The
+    scales are outputs here: each block of 32 is quantised as it is written, by its
+    largest magnitude, to the nearest codes.
 
     Keys are normalised (``k_weight``) and rotated (``cos``, ``sin``,
     ``interleaved``) at their positions on the way, as in ``qk_norm_rope``; with
@@ -638,14 +677,16 @@ def kv_append_paged(
     stay as they were in ``out``, and in a new tensor hold whatever its memory
     held, so a padded step gives its own ``out``.
     """
-    desc, pk = _append_plan(
+    desc, pk, mx = _append_plan(
         _meta(k), _meta(v), _meta(k_pages), _meta(v_pages), _meta(block_table), _meta(seq_lens),
         _meta(cu_seqlens), _meta(q), _meta(cos), _meta(sin), _meta(q_weight), _meta(k_weight),
         _meta(k_scales), _meta(v_scales), _meta(out), float(eps), 1 if interleaved else 0)
     if q is not None and out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lib = load_library()
-    _launch(lib, k.device, lib.neptune_kv_append_paged, desc, pk, k.data_ptr(), v.data_ptr(),
+    entry = (lib.neptune_kv_append_paged, desc, pk) if mx is None else \
+        (lib.neptune_kv_append_paged_mx, desc, pk, mx)
+    _launch(lib, k.device, *entry, k.data_ptr(), v.data_ptr(),
             _ptr(q), _ptr(q_weight), _ptr(k_weight), _ptr(cos), _ptr(sin), block_table.data_ptr(),
             _ptr(cu_seqlens), seq_lens.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
             _ptr(k_scales), _ptr(v_scales), _ptr(out))
@@ -653,15 +694,87 @@ def kv_append_paged(
 
 
 @functools.lru_cache(maxsize=_PLANS, typed=True)
+def _read_plan(k_pages, v_pages, block_table, seq_lens, cu_seqlens, k_scales, v_scales, k_out,
+               v_out, tokens, dtype):
+    """(descriptor, page descriptor, MXFP4 descriptor or None, rows' shape, their dtype)."""
+    if tokens is None:
+        if k_out is None and cu_seqlens is not None:
+            raise ValueError("kv_read_paged: give tokens (or out) with cu_seqlens")
+        tokens = k_out[0][0] if k_out is not None and len(k_out[0]) == 3 else seq_lens[0][0]
+    pool = k_pages[2] if k_pages[2] in (torch.float16, torch.bfloat16) else torch.bfloat16
+    pk, kv_dtype, B, D, mx = _pool_plan("kv_read_paged", pool, tokens, k_pages, v_pages,
+                                        block_table, seq_lens, cu_seqlens, k_scales, v_scales)
+    if dtype is None:
+        dtype = pool if k_out is None else k_out[2]
+    if dtype not in _TORCH_TO_DTYPE:
+        raise ValueError(f"dtype must be one of {list(_TORCH_TO_DTYPE)}")
+    shape = (tokens, k_pages[0][1], D)
+    desc = _abi.KvReadDesc()
+    if k_out is not None:
+        desc.ko_stride[:] = _strides_th("k_out", k_out, shape[1], D, tokens, dtype)
+        desc.vo_stride[:] = _strides_th("v_out", v_out, shape[1], D, tokens, dtype)
+    _require_cuda(k_pages, v_pages, block_table, seq_lens, cu_seqlens, k_scales, v_scales, k_out,
+                  v_out)
+    desc.tokens, desc.batch, desc.heads_kv, desc.head_dim = tokens, B, shape[1], D
+    desc.dtype, desc.kv_dtype = _TORCH_TO_DTYPE[dtype], kv_dtype
+    return (ctypes.byref(desc), ctypes.byref(pk), None if mx is None else ctypes.byref(mx), shape,
+            dtype)
+
+
+def kv_read_paged(
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    cu_seqlens: torch.Tensor | None = None,
+    *,
+    tokens: int | None = None,
+    dtype: torch.dtype | None = None,
+    k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None,
+    out: tuple[torch.Tensor, torch.Tensor] | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Cached keys and values as rows: what ``kv_append_paged`` wrote, read back.
+
+    Pools, tables and lengths as there (16-bit, E4M3 or MXFP4 pools): row r of
+    sequence b, cu_seqlens[b] <= r < cu_seqlens[b + 1], is the token at place
+    seq_lens[b] - (cu_seqlens[b + 1] - r), so that cu_seqlens of whole lengths reads
+    whole sequences, and the step's own the rows just appended; without it, each
+    sequence's last token. ``tokens`` is the number of rows (cu_seqlens[B], known to
+    the caller; the device's is not waited for). Returns (k, v) [tokens, Hkv, D] in
+    ``dtype`` float32, float16 or bfloat16 (default: the pools', bfloat16 for codes),
+    new or ``out`` = (k_out, v_out). A row without a slot is zeros; rows behind the last
+    sequence stay as they were in ``out``, and in new tensors hold whatever their memory
+    held.
+    """
+    if out is not None and not (isinstance(out, (tuple, list)) and len(out) == 2 and
+                                all(isinstance(t, torch.Tensor) for t in out)):
+        raise ValueError("out must be a pair of tensors (k_out, v_out)")
+    k_out, v_out = (None, None) if out is None else out
+    desc, pk, mx, shape, dtype = _read_plan(
+        _meta(k_pages), _meta(v_pages), _meta(block_table), _meta(seq_lens), _meta(cu_seqlens),
+        _meta(k_scales), _meta(v_scales), _meta(k_out), _meta(v_out),
+        None if tokens is None else int(tokens), dtype)
+    if out is None:
+        k_out, v_out = (torch.empty(shape, dtype=dtype, device=k_pages.device) for _ in range(2))
+    lib = load_library()
+    _launch(lib, k_pages.device, lib.neptune_kv_read_paged, desc, pk, mx, k_pages.data_ptr(),
+            v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales), block_table.data_ptr(),
+            _ptr(cu_seqlens), seq_lens.data_ptr(), k_out.data_ptr(), v_out.data_ptr())
+    return k_out, v_out
+
+
+@functools.lru_cache(maxsize=_PLANS, typed=True)
 def _attn_paged_plan(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, k_scales, v_scales,
-                     out, max_seq_len, scale):
-    """(descriptor, page descriptor, workspace bytes)."""
+                     out, max_seq_len, scale, softcap, slopes, window):
+    """(descriptor, page descriptor, workspace bytes, None or the MXFP4 and the scores'
+    descriptors, either of them None)."""
     if len(q[0]) != 3:
         raise ValueError("attention_paged takes q [tokens, Hq, D]")
     T, Hq, _ = q[0]
-    pk, kv_dtype, B = _pool_plan("attention_paged", q[2], T, k_pages, v_pages, block_table,
-                                 seq_lens, cu_seqlens, k_scales, v_scales)
-    _, Hk, psize, D = k_pages[0]
+    pk, kv_dtype, B, D, mx = _pool_plan("attention_paged", q[2], T, k_pages, v_pages, block_table,
+                                        seq_lens, cu_seqlens, k_scales, v_scales)
+    _, Hk, psize, _ = k_pages[0]
     desc = _abi.AttnPagedDesc()
     desc.q_stride[:] = _strides_th("q", q, Hq, D, T, q[2])
     if out is not None:
@@ -669,14 +782,29 @@ def _attn_paged_plan(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, k_s
     desc.scale_log2 = scale_to_log2(scale, D)
     if scale is not None and desc.scale_log2 == 0.0:  # the library's default otherwise
         raise ValueError("attention_paged: scale must not be 0")
-    _require_cuda(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, k_scales, v_scales, out)
+    score = None
+    if softcap is not None or window is not None:
+        if softcap is not None and not softcap > 0.0:
+            raise ValueError("attention_paged: softcap must be positive")
+        if window is not None and window < 1:
+            raise ValueError("attention_paged: window must be at least 1")
+        score = _abi.ScoreDesc(window or 0, softcap or 0.0, 0)
+    if slopes is not None and (slopes[2] != torch.float32 or tuple(slopes[0]) != (Hq,) or
+                               not _contiguous(slopes)):
+        raise ValueError(f"attention_paged: slopes must be a contiguous float32 [{Hq}] tensor")
+    _require_cuda(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, k_scales, v_scales, out,
+                  slopes)
     desc.tokens, desc.batch, desc.heads_q, desc.heads_kv, desc.head_dim = T, B, Hq, Hk, D
     desc.seq_kv = max_seq_len if max_seq_len is not None else pk.max_pages * psize
     desc.dtype, desc.kv_dtype = _TORCH_TO_DTYPE[q[2]], kv_dtype
     n = ctypes.c_size_t()
     lib = load_library()
     check(lib.neptune_attn_paged_workspace_bytes(ctypes.byref(desc), ctypes.byref(n)), lib)
-    return ctypes.byref(desc), ctypes.byref(pk), n.value
+    ext = None
+    if mx is not None or score is not None or slopes is not None:
+        ext = (None if mx is None else ctypes.byref(mx),
+               None if score is None else ctypes.byref(score))
+    return ctypes.byref(desc), ctypes.byref(pk), n.value, ext
 
 
 def attention_paged(
@@ -694,6 +822,9 @@ def attention_paged(
     workspace: torch.Tensor | None = None,
     k_scales: torch.Tensor | None = None,
     v_scales: torch.Tensor | None = None,
+    softcap: float | None = None,
+    slopes: torch.Tensor | None = None,
+    window: int | None = None,
 ):
     """Causal attention of new tokens over a paged cache that holds them.
 
@@ -702,7 +833,8 @@ def attention_paged(
     single token, none (``cu_seqlens`` and ``seq_lens`` as in
     ``kv_append_paged``, called before). k_pages / v_pages, block_table,
     k_scales / v_scales as in ``decode_paged`` (pools of q's dtype, or E4M3 with
-    bfloat16 q; page sizes that are multiples of 16; D 64 or 128).
+    bfloat16 q), or MXFP4 pools as ``kv_append_paged`` writes them; page sizes that
+    are multiples of 16; D 64 or 128.
     ``max_seq_len`` (default max_pages * page_size) bounds the lengths. A row
     sees its sequence up to its own place; one with a negative place sees
     nothing: output 0, log-sum-exp -inf. Rows behind the last sequence are not
@@ -711,13 +843,20 @@ def attention_paged(
     and reads no lse there). Returns o [T, Hq, D] (and lse [T, Hq] fp32 if
     asked).
 
+    Scores x = q . k * scale become softcap * tanh(x / softcap) with ``softcap``; with
+    ``slopes`` float32 [Hq], slopes[h] * (j - p) is added for a key at place j and a
+    row at place p; with ``window`` a row sees that many keys at most, its own the last
+    of them. Any of them together, over pools of any kind.
+
     The workspace is for the calls of the sizes it was asked for: fewer tokens
     may need a larger one, since keys are cut where tiles are few.
     """
-    desc, pk, need = _attn_paged_plan(
+    desc, pk, need, ext = _attn_paged_plan(
         _meta(q), _meta(k_pages), _meta(v_pages), _meta(block_table), _meta(seq_lens),
         _meta(cu_seqlens), _meta(k_scales), _meta(v_scales), _meta(out),
-        None if max_seq_len is None else int(max_seq_len), None if scale is None else float(scale))
+        None if max_seq_len is None else int(max_seq_len), None if scale is None else float(scale),
+        None if softcap is None else float(softcap), _meta(slopes),
+        None if window is None else int(window))
     _check_workspace(workspace, q.device)
     if workspace is None and need:
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
@@ -725,10 +864,16 @@ def attention_paged(
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
     lib = load_library()
-    _launch(lib, q.device, lib.neptune_attn_paged, desc, pk, q.data_ptr(), k_pages.data_ptr(),
-            v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales), block_table.data_ptr(),
-            _ptr(cu_seqlens), seq_lens.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(workspace),
+    tail = (block_table.data_ptr(), _ptr(cu_seqlens), seq_lens.data_ptr(), out.data_ptr(),
+            _ptr(lse), _ptr(workspace),
             0 if workspace is None else workspace.numel() * workspace.element_size())
+    if ext is None:
+        _launch(lib, q.device, lib.neptune_attn_paged, desc, pk, q.data_ptr(), k_pages.data_ptr(),
+                v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales), *tail)
+    else:
+        _launch(lib, q.device, lib.neptune_attn_paged_ext, desc, pk, *ext, q.data_ptr(),
+                k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales),
+                _ptr(slopes), *tail)
     return (out, lse) if return_lse else out
 
 
@@ -736,7 +881,8 @@ def attention_paged_workspace_bytes(
     tokens: int, batch: int, heads_q: int, heads_kv: int, head_dim: int, max_seq_len: int,
     *, dtype: torch.dtype = torch.bfloat16, fp8: bool = False,
 ) -> int:
-    """Bytes of ``attention_paged``'s workspace for such a call (0: none)."""
+    """Bytes of ``attention_paged``'s workspace for such a call (0: none); MXFP4 pools, a
+    cap, slopes and a window change none of it."""
     desc = _abi.AttnPagedDesc()
     desc.tokens, desc.batch, desc.heads_q, desc.heads_kv = tokens, batch, heads_q, heads_kv
     desc.head_dim, desc.seq_kv = head_dim, max_seq_len
