@@ -24,6 +24,13 @@ bool attn_paged_supported(const PagedAttnLaunch &L, const char **why) {
     *why = "token strides must be below 2^31 / 15 bytes";
     return false;
   }
+  if (L.pool == MXFP4)
+    for (const int64_t *t : {L.kps, L.vps, L.kss, L.vss})
+      // (pages beyond the pool's are not looked at; factors below 2^31, as checked next)
+      if (t[0] > INT32_MAX || t[2] > INT32_MAX / std::max<int64_t>(L.page_size, 1)) {
+        *why = "MXFP4 pools' pages must lie less than 2 GiB apart, and their tokens within as much";
+        return false;
+      }
   if (L.seq_kv > (int64_t)1 << 30 || L.num_pages > INT32_MAX || L.max_pages > INT32_MAX - 64 ||
       L.page_size > (int64_t)1 << 30 || L.batch > 1 << 16 || L.tokens > (int64_t)1 << 30 ||
       L.heads_q > 1 << 20 || L.tokens * (L.heads_q / L.heads_kv) > (int64_t)1 << 30 ||

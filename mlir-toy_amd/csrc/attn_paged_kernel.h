@@ -110,48 +110,99 @@ __device__ inline u32x4 widen8(uint32_t c, float scale) {
 }
 // byte i of x as such a scale
 __device__ inline float scale_byte(uint32_t x, int i) {
-  return __builtin_bit_cast(float, ((x >> (8 * i)) & 0xffu) << 23);
+  return __builtin_bit_cast(float, __builtin_amdgcn_ubfe(x, 8 * i, 8) << 23);
+}
+// The kernel's argument, read again: scalars kept from its first lines on pass what a
+// wave has registers for, and were fetched out of vector lanes in the loops (66 of 330
+// vector instructions a step of narrow_mx)
+__device__ inline const PagedArgs &arguments() {
+  auto p = (const __attribute__((address_space(4))) PagedArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const PagedArgs *)p;
+}
+// base + page * stride + place * tok of an MXFP4 pool: a page's offset is a product of 32
+// by 32 bits, a place's within it fits 32 (attn_paged_supported), four scalar
+// instructions where 64-bit strides take ten
+__device__ inline const char *mx_at(const char *base, int page, int64_t stride, int place,
+                                    int64_t tok) {
+  return base + (uint64_t)(uint32_t)page * (uint32_t)stride + (uint32_t)place * (uint32_t)tok;
+}
+// x, at its use: loads in flight round a loop are carried whole. (Carried element by
+// element they were copied at the loop's end, and so waited for.)
+template <class T>
+__device__ inline T whole(T x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+// x, a lane's 32-bit offset from a scalar base, at its use: widened ahead of a loop it
+// takes two registers, and the loads 64-bit sums
+__device__ inline uint32_t offset(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+// A row's scales as a load brings them, all of a row at once: 32 bits for four, for two
+// 16 that are not an integer to the compiler (it carries a small integer round a loop
+// widened, and so waits at the loop's end for what is in flight)
+template <int HD>
+using row_scales = typename std::conditional<HD == 128, uint32_t, _Float16>::type;
+// scale i of them
+template <class T>
+__device__ inline float scale_of(T x, int i) {
+  uint32_t bytes;
+  if constexpr (sizeof(T) == 4)
+    bytes = whole(x);
+  else
+    bytes = __builtin_bit_cast(uint16_t, whole(x));
+  return scale_byte(bytes, i);
+}
+// a number of the lane's bits: bit i of it is the lane's bit (bits >> 4 i) & 15
+__device__ inline int lane_bits(int lane, int bits) {
+  int x = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < 2 || bits >> 8) x |= ((lane >> ((bits >> (4 * i)) & 15)) & 1) << i;
+  return x;
 }
 
 // Scores that are not plain products, in log2 units: cap tanh(x / cap) with x = s sc,
 // then slope (key - place). Element r is key c0 + 8 (r >> 2) + (r & 3) after the lane's
 // first, which lies d0 after the row's place.
 //
-// Up to |y| = 1/2, y = x / cap, tanh(y) is y times a polynomial of y^2 (fitted at
-// Chebyshev nodes: off by 1.1e-7, 3e-8 rms), beyond it 1 - 2 / (e^2y + 1), whose
-// cancellation would cost a small score its last bits. Scores of ordinary heads keep
-// within a cap of 20 and more, so a wave forms the second for blocks that need it only.
-__device__ inline void shape(const PagedArgs &a, float slope2, float sc, float d0, int c0,
-                             f32x16 &s) {
+// Up to |y| = 3/8, y = x / cap, tanh(y) is y times a polynomial of y^2 (fitted at
+// Chebyshev nodes: off by 6e-8, in fp32 1.5e-7, 5e-8 rms), beyond it 1 - 2 / (e^2y + 1),
+// whose cancellation would cost a small score its last bits. Scores of ordinary heads
+// keep to an eighth of such caps as 30 and 50, so a wave forms the second only for blocks
+// that need it.
+template <int N, class V>
+__device__ inline void shape(const PagedArgs &a, float slope2, float sc, float d0, int c0, V &s) {
   if (a.cap2 != 0.0f) {
     const float u = sc * a.cap_inv;
     float big = 0.0f;
-    f32x16 y;
+    V y;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
+    for (int r = 0; r < N; ++r) {
       y[r] = s[r] * u;
       big = fmaxf(big, fabsf(y[r]));
       const float w = y[r] * y[r];
-      float p = fmaf(w, a.capp[4], a.capp[3]);
-      p = fmaf(w, p, a.capp[2]);
+      float p = fmaf(w, a.capp[3], a.capp[2]);
       p = fmaf(w, p, a.capp[1]);
       s[r] = y[r] * fmaf(w, p, a.capp[0]);
     }
-    if (__any(big > 0.5f)) {
+    if (__any(big > kCapPoly)) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
+      for (int r = 0; r < N; ++r) {
         const float e = fast_exp2(y[r] * (2.0f * kLog2e));
         const float t = fmaf(-2.0f * a.cap2, __builtin_amdgcn_rcpf(e + 1.0f), a.cap2);
-        s[r] = fabsf(y[r]) > 0.5f ? t : s[r];
+        s[r] = fabsf(y[r]) > kCapPoly ? t : s[r];
       }
     }
   } else {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] *= sc;
+    for (int r = 0; r < N; ++r) s[r] *= sc;
   }
   if (a.slopes) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
+    for (int r = 0; r < N; ++r)
       s[r] = fmaf(slope2, d0 + (float)(c0 + 8 * (r >> 2) + (r & 3)), s[r]);
   }
 }
@@ -217,11 +268,11 @@ struct Special {
   }
 };
 
-// o (element 4 rq + e of o[nb]: head_dim 32 nb + 8 rq + 4 g + e) += the special
-// values of V's keys lo .. hi - 1 up to the row's place
-template <class E, int HD, int POOL>
+// add(i, e, x) for the special values x of V's keys lo .. hi - 1 that the row at pos sees,
+// elements e of the lane's runs of four: head_dim RUN i + 4 g + e
+template <class E, int HD, int POOL, int RUN, int VECTORS, class O>
 __device__ inline void add_special(const PagedArgs &a, const Item &it, int hk, int lo, int hi,
-                                   int pos, int g, f32x16 (&o)[HD / 32]) {
+                                   int pos, int g, O add) {
   const int from = a.window ? pos - a.window : -1;  // the last key before the row's
   const int32_t *tab = a.btab + (int64_t)it.b * a.maxp;
 #pragma unroll 1
@@ -235,27 +286,33 @@ __device__ inline void add_special(const PagedArgs &a, const Item &it, int hk, i
                             ? a.vmx + hk * a.vss1 + page * a.vss0 + (int64_t)place * a.vstok
                             : nullptr;
 #pragma unroll
-    for (int nb = 0; nb < HD / 32; ++nb)
+    for (int i = 0; i < VECTORS; ++i) {
+      const int d = RUN * i + 4 * g;
+      u32x4 four;
+      if constexpr (POOL == MXFP4)
+        four = widen8<E>(*(const uint16_t *)(v + d / 2), scale_byte(vs[d / 32], 0));
 #pragma unroll
-      for (int rq = 0; rq < 4; ++rq) {
-        const int d = 32 * nb + 8 * rq + 4 * g;
-        u32x4 four;
+      for (int e = 0; e < 4; ++e) {
+        float x;
         if constexpr (POOL == MXFP4)
-          four = widen8<E>(*(const uint16_t *)(v + d / 2), scale_byte(vs[nb], 0));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x;
-          if constexpr (POOL == MXFP4)
-            x = E::to_f32((uint16_t)(four[e >> 1] >> (16 * (e & 1))));
-          else if constexpr (POOL == E4M3)
-            x = (((const uint8_t *)v)[d + e] & 0x7f) == 0x7f ? __builtin_nanf("") : 0.0f;
-          else
-            x = E::to_f32(((const uint16_t *)v)[d + e]);
-          if (j <= pos && j > from && !(fabsf(x) <= 3.4e38f)) o[nb][4 * rq + e] += x;
-        }
-        __builtin_amdgcn_sched_barrier(0);  // few registers at a time
+          x = E::to_f32((uint16_t)(four[e >> 1] >> (16 * (e & 1))));
+        else if constexpr (POOL == E4M3)
+          x = (((const uint8_t *)v)[d + e] & 0x7f) == 0x7f ? __builtin_nanf("") : 0.0f;
+        else
+          x = E::to_f32(((const uint16_t *)v)[d + e]);
+        if (j <= pos && j > from && !(fabsf(x) <= 3.4e38f)) add(i, e, x);
       }
+      __builtin_amdgcn_sched_barrier(0);  // few registers at a time
+    }
   }
+}
+// (o of the 32-row forms: element 4 rq + e of o[nb] is head_dim 32 nb + 8 rq + 4 g + e)
+template <class E, int HD, int POOL>
+__device__ inline void add_special(const PagedArgs &a, const Item &it, int hk, int lo, int hi,
+                                   int pos, int g, f32x16 (&o)[HD / 32]) {
+  add_special<E, HD, POOL, 8, HD / 8>(a, it, hk, lo, hi, pos, g, [&](int i, int e, float x) {
+    o[i >> 2][4 * (i & 3) + e] += x;
+  });
 }
 
 // A tile of at most 32 rows (generated or guessed tokens, a chunk's last few): the
@@ -265,17 +322,14 @@ __device__ inline void add_special(const PagedArgs &a, const Item &it, int hk, i
 // with no barrier: K of step i + N is issued once step i's scores are formed, V
 // once its P.V is (N slots per operand: 1 for 16-bit head_dim 128, 2 or 4 for
 // smaller rows), so a wave has copies in flight at all times. E4M3 codes stay codes in
-// LDS and are widened as operands are read; E2M1 codes come in registers, DEPTH steps
-// ahead: a lane takes whole blocks of 32 elements of K's rows, one scale each, as the
-// products' operands (which element a product's k-slot holds is free, as long as Q's
-// agree), and V goes through LDS widened. The running max moves with every
+// LDS and are widened as operands are read. The running max moves with every
 // step, so a row's largest p is 1. At the end the waves' states merge in LDS, a
 // quarter of the head_dim each.
 template <class E, int HD, int POOL, bool MOD>
 __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, int w, int lane,
                                    int kb0, int nv, const uint8_t *smem, f32x2 *mlbox) {
   typedef typename E::vec8 V8;
-  constexpr bool FP8 = POOL == E4M3, MX = POOL == MXFP4;
+  constexpr bool FP8 = POOL == E4M3;
   constexpr int STEP = 32;
   constexpr int RB = HD * (FP8 ? 1 : 2);        // bytes of a row
   constexpr int TILE = STEP * RB;
@@ -294,7 +348,7 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
   };
   auto vswz = [](int r) {
     return FP8 ? (UNITS == 8 ? (r >> 1) & 7 : (r >> 2) & 3)
-               : (UNITS == 16 ? (r & 3) << 2 : ((r >> 1) & 1) << 2) | (MX ? (r >> 2) & 3 : 0);
+               : (UNITS == 16 ? (r & 3) << 2 : ((r >> 1) & 1) << 2);
   };
 
   const int off = it.len - it.n, base_row = it.tile * BM;
@@ -343,11 +397,10 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
   u32x4 qf[NST];
   {
     const uint16_t *qp = a.q + (int64_t)(it.row0 + tok) * a.qs0 +
-                         (int64_t)(hk * a.group + hr) * a.qs1 + (MX ? 32 : 8) * g;
+                         (int64_t)(hk * a.group + hr) * a.qs1 + 8 * g;
 #pragma unroll
     for (int st = 0; st < NST; ++st)
-      qf[st] = lq < rows ? *(const u32x4 *)(qp + (MX ? 64 * (st >> 2) + 8 * (st & 3) : 16 * st))
-                         : u32x4{0, 0, 0, 0};
+      qf[st] = lq < rows ? *(const u32x4 *)(qp + 16 * st) : u32x4{0, 0, 0, 0};
   }
   float slope2 = 0.0f;
   if constexpr (MOD)
@@ -397,76 +450,18 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
   auto copy_k = [&](int i) { copy(i, std::false_type{}, kslot(i)); };
   auto copy_v = [&](int i) { copy(i, std::true_type{}, vslot(i)); };
 
-  // MXFP4: a step's codes and scales in registers. K: lane (lq, g) has blocks g and
-  // g + 2 (head_dim 64: block g) of row lq. V: two lanes a row, in an order of rows whose
-  // bits 0, 2 and 3 differ among the 16 lanes that one cycle writes to LDS: with the
-  // swizzle they fill its banks evenly.
-  constexpr int DEPTH = MX ? 2 : 1, MU = MX ? HD / 64 : 1;
-  u32x4 kc[DEPTH][MU], vc[DEPTH][MU];
-  uint32_t ksb[DEPTH], vsb[DEPTH];
-  const int l5 = lane >> 1;
-  const int vrow = (l5 & 1) | (l5 & 2) << 1 | (l5 & 4) << 1 | (l5 & 8) >> 2 | (l5 & 16);
-  const int vblk = MU * (lane & 1);
-  const int vput = vrow * RB + (((4 * vblk) ^ vswz(vrow)) << 4);
-  const int vget0 = 4 * g + ((lane & 15) >> 2);  // the row of V's first operand
-  const int vgetb = vget0 * RB + ((((lane >> 3) & 2) + ((lane >> 1) & 1) ^ vswz(vget0)) << 4) + 8 * (lane & 1);
-  typedef typename std::conditional<HD == 128, uint32_t, uint16_t>::type krow_t;
-  auto fetch = [&](int i, auto slot) __attribute__((always_inline)) {
-    constexpr int S = decltype(slot)::value;
-    const char *kb[2], *vb[2];
-    const uint8_t *kx[2], *vx[2];
-    int most[2];
-    const int step = min(i, ns - 1);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int run = min(2 * (t0 + step) + h, last_run);
-      int index, rest;
-      page_of(a, run, &index, &rest);
-      if (index - tab0 >= 64) {
-        load_tab(max(index - 1, 0));  // the step's first run may lie a page before
-        settle(tabv);
-      }
-      int page = __builtin_amdgcn_readlane(tabv, index - tab0);
-      page = min(max(page, 0), a.npages - 1);
-      const int64_t place = rest * 16;
-      kb[h] = kp + page * a.kps0 + place * a.ktok;
-      vb[h] = vp + page * a.vps0 + place * a.vtok;
-      kx[h] = a.kmx + hk * a.kss1 + page * a.kss0 + place * a.kstok;
-      vx[h] = a.vmx + hk * a.vss1 + page * a.vss0 + place * a.vstok;
-      most[h] = it.len - 1 - run * 16;
-    }
-    const bool kh = lq & 16, vh = vrow & 16;
-    const int64_t kr = min(lq & 15, kh ? most[1] : most[0]);
-    const int64_t vr = min(vrow & 15, vh ? most[1] : most[0]);
-    const char *k = (kh ? kb[1] : kb[0]) + kr * a.ktok + 16 * g;
-    const char *v = (vh ? vb[1] : vb[0]) + vr * a.vtok + 16 * vblk;
-    const uint8_t *ks = (kh ? kx[1] : kx[0]) + kr * a.kstok;
-    const uint8_t *vs = (vh ? vx[1] : vx[0]) + vr * a.vstok + vblk;
-#pragma unroll
-    for (int t = 0; t < MU; ++t) {
-      kc[S][t] = *(const u32x4 *)(k + 32 * t);
-      vc[S][t] = *(const u32x4 *)(v + 16 * t);
-    }
-    ksb[S] = *(const krow_t *)ks;
-    vsb[S] = MU == 2 ? *(const uint16_t *)vs : *vs;
-  };
-
   f32x16 o[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[nb][r] = 0.0f;
   float m = kNegFltMax, lsum = 0.0f;
-  if constexpr (MX) {
-    if (ns > 0) static_for<DEPTH>([&](auto J) { fetch(decltype(J)::value, J); });
-  } else {
-    static_for<N>([&](auto J) {
-      if (decltype(J)::value < ns) {
-        copy_k(decltype(J)::value);
-        copy_v(decltype(J)::value);
-      }
-    });
-  }
+  static_for<N>([&](auto J) {
+    if (decltype(J)::value < ns) {
+      copy_k(decltype(J)::value);
+      copy_v(decltype(J)::value);
+    }
+  });
   bool special = false;
   // waits until the copies issued after a tile are all that is in flight: `pairs`
   // whole steps' (at most N - 1) and X tiles
@@ -479,39 +474,12 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
     asm volatile("" ::: "memory");  // no read of the tile before the wait
   };
 
-  auto take_step = [&](int i, auto slot) __attribute__((always_inline)) {
-    constexpr int S = decltype(slot)::value;
+  for (int i = 0; i < ns; ++i) {
     const int later = ns - 1 - i;
     const int key0 = (t0 + i) * STEP;
-    if constexpr (!MX) wait_tiles(later, std::integral_constant<int, 1>{});  // K(i) is there
+    wait_tiles(later, std::integral_constant<int, 1>{});  // K(i) is there
     f32x16 s = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-    if constexpr (MX) {
-      if (S == 0 || i < ns) {
-#pragma unroll
-        for (int st = 0; st < NST; ++st) {
-          const u32x4 A = widen8<E>(kc[S][st >> 2][st & 3], scale_byte(ksb[S], 2 * (st >> 2) + g));
-          s = E::mfma32(as_vec8<V8>(A), as_vec8<V8>(qf[st]), s);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        // (one register kept for the addresses of a step's stores, and of its reads)
-        int vto = vput;
-        asm volatile("" : "+v"(vto));
-#pragma unroll
-        for (int t = 0; t < MU; ++t) {
-          const float scale = scale_byte(vsb[S], t);
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            *(u32x4 *)(uint8_t *)(mine + (vto ^ ((4 * t + u) << 4))) =
-                widen8<E>(vc[S][t][u], scale);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      }
-      // (whatever the steps left: the compiler then knows how many loads lie between a
-      // slot's and its use)
-      fetch(i + DEPTH, slot);
-      __builtin_amdgcn_sched_barrier(0);
-      if (S > 0 && i >= ns) return;
-    } else {
+    {
       const uint8_t *kt = kslot(i) + lq * RB;
 #pragma unroll
       for (int st = 0; st < NST; ++st) {
@@ -526,10 +494,8 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
         s = E::mfma32(as_vec8<V8>(A), as_vec8<V8>(qf[st]), s);
       }
     }
-    if constexpr (!MX) {
-      __builtin_amdgcn_s_waitcnt(kWaitLgkm0);  // K(i) has been read
-      if (later >= N) copy_k(i + N);
-    }
+    __builtin_amdgcn_s_waitcnt(kWaitLgkm0);  // K(i) has been read
+    if (later >= N) copy_k(i + N);
     float vs[2] = {1.0f, 1.0f};
     if constexpr (FP8) {
       // the scales of both runs: K's before the mask, V's with P
@@ -554,7 +520,7 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
       for (int r = 0; r < 16; ++r) s[r] *= a.scale2;
     }
     const int lim = pos - key0 - 4 * g;  // element r holds key 4 g + 8 (r >> 2) + (r & 3)
-    if constexpr (MOD) shape(a, slope2, FP8 ? 1.0f : a.scale2, (float)-lim, 0, s);
+    if constexpr (MOD) shape<16>(a, slope2, FP8 ? 1.0f : a.scale2, (float)-lim, 0, s);
     bool masked = key0 + STEP - 1 > lo;
     if (masked) {
 #pragma unroll
@@ -593,15 +559,11 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
         pf[c][j] = FP8 ? E::pack2(p0 == 0.0f ? 0.0f : p0 * vs[c], p1 == 0.0f ? 0.0f : p1 * vs[c])
                        : E::pack2(p0, p1);
       }
-    if constexpr (MX)
-      asm volatile("" ::: "memory");  // no read of V before its stores
-    else if (later >= N)
+    if (later >= N)
       wait_tiles(N - 1, std::integral_constant<int, 1>{});  // V(i) is there, K(i + N) after it
     else
       wait_tiles(later, std::integral_constant<int, 0>{});
-    const uint8_t *vt = MX ? mine : vslot(i);
-    int vget = vgetb;
-    if constexpr (MX) asm volatile("" : "+v"(vget));
+    const uint8_t *vt = vslot(i);
     auto v_operand = [&](int c, int nb) {
       const int s16 = lane & 15, dh = (lane >> 4) & 1;
       if constexpr (FP8) {
@@ -613,42 +575,20 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
         return u32x4{y[0], y[1], z[0], z[1]};
       } else {
         const int j = s16 >> 2, r = 16 * c + 4 * g + j;
-        if constexpr (MX) {
-          // (the swizzle has bit 3 of the row in bit 1: eight rows on, unit ^ 2)
-          const uint8_t *p = vt + 16 * c * RB;
-          const u32x2 y = __builtin_bit_cast(u32x2, lds_read_tr16(p + (vget ^ (nb << 6))));
-          const u32x2 z = __builtin_bit_cast(u32x2, lds_read_tr16(p + 8 * RB + (vget ^ (nb << 6 | 32))));
-          return u32x4{y[0], y[1], z[0], z[1]};
-        }
         const uint8_t *p = vt + r * RB + (((4 * nb + 2 * dh) ^ vswz(j)) << 4) + 8 * (s16 & 3);
         const u32x2 y = __builtin_bit_cast(u32x2, lds_read_tr16(p));
         const u32x2 z = __builtin_bit_cast(u32x2, lds_read_tr16(p + 8 * RB));
         return u32x4{y[0], y[1], z[0], z[1]};
       }
     };
-    if (masked) {
-      // (MXFP4: half the registers at a time)
-      special |= Special<E, FP8>::template scrub<MX ? CH / 2 : CH>(vt, lane);
-      if constexpr (MX) special |= Special<E, FP8>::template scrub<CH / 2>(vt + CH * 512, lane);
-    }
-    if constexpr (MX) asm volatile("" ::: "memory");
+    if (masked) special |= Special<E, FP8>::template scrub<CH>(vt, lane);
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
         o[nb] = E::mfma32(as_vec8<V8>(v_operand(c, nb)), as_vec8<V8>(pf[c]), o[nb]);
-    if constexpr (MX) {
-      asm volatile("" ::: "memory");  // nor the next V's stores before these reads
-    } else {
-      __builtin_amdgcn_s_waitcnt(kWaitLgkm0);  // V(i) has been read
-      if (later >= N) copy_v(i + N);
-    }
-  };
-  if constexpr (MX) {
-    for (int i = 0; i < ns; i += DEPTH)
-      static_for<DEPTH>([&](auto J) { take_step(i + decltype(J)::value, J); });
-  } else {
-    for (int i = 0; i < ns; ++i) take_step(i, std::integral_constant<int, 0>{});
+    __builtin_amdgcn_s_waitcnt(kWaitLgkm0);  // V(i) has been read
+    if (later >= N) copy_v(i + N);
   }
 
   if (__builtin_expect(special, 0))
@@ -705,11 +645,352 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
   }
 }
 
+// The same over MXFP4 pools, with products of 16 by 16 by 32: a decoded token's few heads
+// fill a quarter of 16 rows, not an eighth of 32, so scores and products cost half. NQ
+// tiles of 16 rows. Lane (c, g) of 16 by 4 holds S^T's keys 4 g + r of each run of 16 for
+// row c, and O^T's head_dim 16 nd + 4 g + r.
+//
+// A step is 64 keys, four runs of 16. Its codes come in registers, a step ahead. K: a lane takes 32 (head_dim 64: 16)
+// elements of one row of each run, and one scale, as the products' operands (which
+// element a k-slot holds is free, as long as Q's agree). V goes through LDS widened,
+// and is read transposed; keys 16 t + 4 g + r take k-slot 8 g + 4 t + r, where P has
+// them. A run lies within a page, so a load's base is scalar and its offsets are the
+// same all along. (Two and four steps of 32 keys ahead, in a loop unrolled as often, were
+// slower by the code's length: 1 over 400 8.2 and 8.6 us, this 7.8.)
+template <class E, int HD, bool MOD, int NQ>
+__device__ inline void narrow_mx(const Item &it, int hk, int w, int lane, int kb0, int nv,
+                                 const uint8_t *smem, f32x2 *mlbox) {
+  const PagedArgs &a = arguments();
+  typedef typename E::vec8 V8;
+  constexpr int STEP = BN, RUNS = STEP / 16;
+  constexpr int RB = HD * 2;        // bytes of V's rows in LDS
+  constexpr int REGION = 16384;     // LDS per wave: V's tile, and its state at the end
+  constexpr int ND = HD / 16;       // 16-wide head_dim tiles of O^T
+  constexpr int KS = HD / 32;       // k-steps of S^T
+  constexpr int LB = HD / 8;        // bytes of codes a lane takes of a row
+  typedef typename std::conditional<HD == 128, u32x4, u32x2>::type codes_t;
+  const int c16 = lane & 15, g = lane >> 4;
+  const uint8_t *const mine = smem + w * REGION;
+  // 16-byte units of a row of V: eight rows' neighbouring pairs, which half a wave reads
+  // transposed at once, lie in different banks, and so do the single ones of rows 0, 1, 8
+  // and 9 (head_dim 64: 0 and 8) apart, which eight lanes write
+  auto vswz = [](int r) {
+    return (HD == 128 ? (r & 7) << 1 : ((r >> 1) & 3) << 1) | ((r >> 3) & 1);
+  };
+
+  const int off = it.len - it.n, base_row = it.tile * BM;
+  const int rows = min(it.n * a.group - base_row, NARROW);
+  int tok[NQ], hr[NQ], pos[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const int row = base_row + min(16 * q + c16, rows - 1);
+    tok[q] = quotient(row, a.group, a.group_inv);
+    hr[q] = row - tok[q] * a.group;
+    pos[q] = off + tok[q];
+  }
+  const int lo = __builtin_amdgcn_readfirstlane(off + quotient(base_row, a.group, a.group_inv));
+  const int last = off + quotient(base_row + rows - 1, a.group, a.group_inv);  // the last row's place
+  // the wave's steps of the item's
+  const int s0 = kb0, s1 = min(kb0 + nv, last < 0 ? 0 : last / STEP + 1);
+  const int share = (max(s1 - s0, 0) + 3) >> 2;
+  const int t0 = __builtin_amdgcn_readfirstlane(s0 + w * share);
+  const int ns = __builtin_amdgcn_readfirstlane(max(min(t0 + share, s1) - t0, 0));
+
+  const char *kp = a.k + hk * a.kps1, *vp = a.v + hk * a.vps1;
+  const char *ksp = (const char *)a.kmx + hk * a.kss1, *vsp = (const char *)a.vmx + hk * a.vss1;
+  const int32_t *tab = a.btab + (int64_t)it.b * a.maxp;
+  const int last_run = (it.len - 1) >> 4;
+  int tab0 = 0, tabv = 0;
+  auto load_tab = [&](int first) {
+    tab0 = first;
+    const int j = first + lane;
+    tabv = j < a.maxp ? tab[j] : 0;
+  };
+  if (ns > 0) {
+    int index, rest;
+    page_of(a, min(RUNS * t0, last_run), &index, &rest);
+    load_tab(index);
+  }
+  // Q: k-step u's 8 elements are those of K's operand
+  u32x4 qf[NQ][KS];
+  float slope2[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const uint16_t *qp = a.q + (int64_t)(it.row0 + tok[q]) * a.qs0 +
+                         (int64_t)(hk * a.group + hr[q]) * a.qs1 + 2 * LB * g;
+#pragma unroll
+    for (int u = 0; u < KS; ++u)
+      qf[q][u] = 16 * q + c16 < rows ? *(const u32x4 *)(qp + 8 * u) : u32x4{0, 0, 0, 0};
+    slope2[q] = 0.0f;
+    if constexpr (MOD)
+      if (a.slopes) slope2[q] = a.slopes[hk * a.group + hr[q]] * kLog2e;
+  }
+
+  // a lane's row of a run, and where it lies in it: K's row c16, its quarter g; V's in an
+  // order that keeps apart the eight neighbouring lanes that write at once, over 128 bytes
+  const int vq = lane_bits(lane, HD == 128 ? 0x30 : 0x10);
+  const int vrow = lane_bits(lane, HD == 128 ? 0x2541 : 0x2543);
+  codes_t kc[RUNS], vc[RUNS];
+  row_scales<HD> ks[RUNS], vs[RUNS];
+  // A run's 16 rows all lie in its page, those behind the sequence's end too: what they
+  // hold meets scores that are masked (K), or becomes nothing under a scale of 2^-127 (V).
+  const uint32_t koff = c16 * (uint32_t)a.ktok + LB * g, voff = vrow * (uint32_t)a.vtok + LB * vq;
+  const uint32_t ksoff = c16 * (uint32_t)a.kstok, vsoff = vrow * (uint32_t)a.vstok;
+  const int kblk = HD == 128 ? g : g >> 1, vblk = HD == 128 ? vq : vq >> 1;
+  // runs of a step that share a page, whatever page: its place is looked up once
+  const int same = a.ps16 & 1 ? 1 : a.ps16 & 2 ? 2 : 4;
+  auto fetch = [&](int i) __attribute__((always_inline)) {
+    const int run = RUNS * (t0 + i);
+    int index, rest;
+    page_of(a, min(run, last_run), &index, &rest);
+    const char *at[4];  // the run's first place: K, its scales, V, its scales
+#pragma unroll
+    for (int h = 0; h < RUNS; ++h) {
+      const bool more = run + h <= last_run;  // (behind the end: the last run again)
+      if (h & (same - 1)) {
+        at[0] += more ? 16 * (uint32_t)a.ktok : 0;
+        at[1] += more ? 16 * (uint32_t)a.kstok : 0;
+        at[2] += more ? 16 * (uint32_t)a.vtok : 0;
+        at[3] += more ? 16 * (uint32_t)a.vstok : 0;
+      } else {
+        if (h && more) {
+          rest += same;
+          if (rest >= a.ps16) {
+            rest -= a.ps16;
+            ++index;
+          }
+        }
+        if (index - tab0 >= 64) {
+          load_tab(max(index - 3, 0));  // the step's first run may lie three pages before
+          settle(tabv);
+        }
+        int page = __builtin_amdgcn_readlane(tabv, index - tab0);
+        page = min(max(page, 0), a.npages - 1);
+        const int place = rest * 16;
+        at[0] = mx_at(kp, page, a.kps0, place, a.ktok);
+        at[1] = mx_at(ksp, page, a.kss0, place, a.kstok);
+        at[2] = mx_at(vp, page, a.vps0, place, a.vtok);
+        at[3] = mx_at(vsp, page, a.vss0, place, a.vstok);
+      }
+      kc[h] = *(const codes_t *)(at[0] + offset(koff));
+      ks[h] = *(const row_scales<HD> *)(at[1] + offset(ksoff));
+      vc[h] = *(const codes_t *)(at[2] + offset(voff));
+      vs[h] = *(const row_scales<HD> *)(at[3] + offset(vsoff));
+    }
+  };
+  const int vput = vrow * RB + (((LB / 4 * vq) ^ vswz(vrow)) << 4);
+  // V's first operand: row 4 g + j, the run's second 16 rows on
+  const int vj = 4 * g + (c16 >> 2);
+  const int vget0 = vj * RB + ((((c16 >> 1) & 1) ^ vswz(vj)) << 4) + 8 * (c16 & 1);
+
+  f32x4 o[NQ][ND];
+  float m[NQ], lsum[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+    for (int nd = 0; nd < ND; ++nd) o[q][nd] = f32x4{0, 0, 0, 0};
+    m[q] = kNegFltMax;
+    lsum[q] = 0.0f;
+  }
+  bool special = false;
+  if (ns > 0) fetch(0);
+  // (Q was asked for before: waited for here, not in the loop for all)
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+    for (int u = 0; u < KS; ++u) settle(qf[q][u]);
+    settle(slope2[q]);
+  }
+
+  for (int i = 0; i < ns; ++i) {
+    const int key0 = (t0 + i) * STEP;
+    f32x4 s[NQ][RUNS];
+#pragma unroll
+    for (int h = 0; h < RUNS; ++h) {
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) s[q][h] = f32x4{0, 0, 0, 0};
+      const codes_t codes = whole(kc[h]);
+      const float scale = scale_of(ks[h], kblk);
+#pragma unroll
+      for (int u = 0; u < KS; ++u) {
+        const u32x4 A = widen8<E>(codes[u], scale);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+          s[q][h] = E::mfma16(as_vec8<V8>(A), as_vec8<V8>(qf[q][u]), s[q][h]);
+      }
+    }
+    int to = vput;  // (one register for the stores' addresses)
+    asm volatile("" : "+v"(to));
+#pragma unroll
+    for (int h = 0; h < RUNS; ++h) {
+      const codes_t codes = whole(vc[h]);
+      const float held = scale_of(vs[h], vblk);
+      const float scale = key0 + 16 * h + vrow < it.len ? held : 0.0f;
+#pragma unroll
+      for (int u = 0; u < LB / 4; ++u)
+        *(u32x4 *)(uint8_t *)(mine + 16 * h * RB + (to ^ (u << 4))) = widen8<E>(codes[u], scale);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    fetch(min(i + 1, ns - 1));
+    __builtin_amdgcn_sched_barrier(0);
+    bool masked = key0 + STEP - 1 > lo;
+    u32x4 pf[NQ][RUNS / 2];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const int lim = pos[q] - key0 - 4 * g;  // element (h, r) holds key 4 g + 16 h + r
+      float sc = a.scale2;
+      if constexpr (MOD) {
+#pragma unroll
+        for (int h = 0; h < RUNS; ++h) shape<4>(a, slope2[q], sc, (float)-lim, 16 * h, s[q][h]);
+        sc = 1.0f;
+      }
+      if (key0 + STEP - 1 > lo) {
+#pragma unroll
+        for (int h = 0; h < RUNS; ++h)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (16 * h + r > lim) s[q][h][r] = -INFINITY;
+      }
+      if constexpr (MOD)
+        if (a.window && key0 + a.window <= last) {  // some row's window begins behind its keys
+          masked = true;
+#pragma unroll
+          for (int h = 0; h < RUNS; ++h)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (16 * h + r <= lim - a.window) s[q][h][r] = -INFINITY;
+        }
+      float rs;
+      auto expo = [&]() {
+#pragma unroll
+        for (int h = 0; h < RUNS; ++h)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float p0 = fast_exp2(fmaf(s[q][h][2 * j], sc, -m[q]));
+            const float p1 = fast_exp2(fmaf(s[q][h][2 * j + 1], sc, -m[q]));
+            rs = h + j == 0 ? p0 : rs + p0;
+            rs += p1;
+            pf[q][h >> 1][2 * (h & 1) + j] = E::pack2(p0, p1);  // 16 bits, for P.V alone
+          }
+      };
+      // past the first step the max is formed only where a lane's sum passes 2^kSlack: up
+      // to that m keeps
+      bool full = i == 0;
+      if (!full) {
+        expo();
+        full = __any(!(rs <= kSumCap));
+      }
+      if (full) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < RUNS; ++h)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[q][h][r]);
+        const float m_new = fmaxf(m[q], max_xor32(max_xor16(mx)) * sc);
+        const float alpha = fast_exp2(m[q] - m_new);
+        lsum[q] *= alpha;
+#pragma unroll
+        for (int nd = 0; nd < ND; ++nd)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[q][nd][r] *= alpha;
+        m[q] = m_new;
+        expo();
+      }
+      lsum[q] += rs;
+    }
+    asm volatile("" ::: "memory");  // no read of V before its stores
+    if (masked) {
+#pragma unroll 1
+      for (int h = 0; h < RUNS; ++h)
+        special |= Special<E, false>::template scrub<HD / 32>(mine + 16 * h * RB, lane);
+      asm volatile("" ::: "memory");
+    }
+    int from = vget0;
+    asm volatile("" : "+v"(from));
+#pragma unroll
+    for (int nd = 0; nd < ND; ++nd)
+#pragma unroll
+      for (int c = 0; c < RUNS / 2; ++c) {
+        const uint8_t *p = mine + 32 * c * RB + (from ^ (nd << 5));
+        const u32x2 x = __builtin_bit_cast(u32x2, lds_read_tr16(p));
+        const u32x2 y = __builtin_bit_cast(u32x2, lds_read_tr16(p + 16 * RB));
+        const u32x4 A = {x[0], x[1], y[0], y[1]};
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+          o[q][nd] = E::mfma16(as_vec8<V8>(A), as_vec8<V8>(pf[q][c]), o[q][nd]);
+      }
+    asm volatile("" ::: "memory");  // nor the next V's stores before these reads
+  }
+
+  if (__builtin_expect(special, 0)) {
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+      add_special<E, HD, MXFP4, 16, ND>(
+          a, it, hk, MOD && a.window ? t0 * STEP : max(t0 * STEP, lo / STEP * STEP),
+          min((t0 + ns) * STEP, it.len), pos[q], g, [&](int i, int e, float x) { o[q][i][e] += x; });
+  }
+  // the waves' states, merged lane by lane, a quarter of a row's vectors a wave
+  constexpr int VECTORS = NQ * ND;
+  f32x4 *const box = (f32x4 *)mine + lane;
+#pragma unroll
+  for (int v = 0; v < VECTORS; ++v) box[v * 64] = o[v / ND][v % ND];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const float ltot = sum_xor32(sum_xor16(lsum[q]));
+    if (g == 0) mlbox[(w * NQ + q) * 16 + c16] = f32x2{m[q], ltot};
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    float M = kNegFltMax, L = 0.0f, wgt[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) M = fmaxf(M, mlbox[(k * NQ + q) * 16 + c16][0]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const f32x2 ml = mlbox[(k * NQ + q) * 16 + c16];
+      wgt[k] = fast_exp2(ml[0] - M);
+      L = fmaf(wgt[k], ml[1], L);
+    }
+    if (16 * q + c16 >= rows) continue;
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    const int64_t t = it.row0 + tok[q];
+    const int64_t part = ((int64_t)(it.part + it.split) * a.Hk + hk) * a.prows + 16 * q + c16;
+#pragma unroll
+    for (int k = 0; k < ND / 4; ++k) {
+      const int nd = w * (ND / 4) + k, d = 16 * nd + 4 * g;
+      f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 y = *((const f32x4 *)(smem + j * REGION) + (q * ND + nd) * 64 + lane);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = fmaf(wgt[j], y[e], x[e]);
+      }
+      if (it.splits > 1)
+        *(f32x4 *)(a.po + part * HD + d) = x;
+      else
+        *(u32x2 *)(a.o + t * a.os0 + (int64_t)(hk * a.group + hr[q]) * a.os1 + d) =
+            u32x2{E::pack2(x[0] * inv, x[1] * inv), E::pack2(x[2] * inv, x[3] * inv)};
+    }
+    if (w == 0 && g == 0) {
+      if (it.splits > 1)
+        *(f32x2 *)(a.pml + part * 2) = f32x2{M, L};
+      else if (a.lse)
+        a.lse[t * a.Hq + hk * a.group + hr[q]] = L == 0.0f ? -INFINITY : row_lse(M, L);
+    }
+  }
+}
+
 template <class E, int HD, int POOL, bool MOD>
-__global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
+__global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs args) {
   typedef typename E::vec8 V8;
   constexpr bool FP8 = POOL == E4M3, MX = POOL == MXFP4;
   constexpr bool CODES = FP8 || MX;  // widened on their way to LDS
+  // (E4M3's scores have a scale for each page; head_dim 64 forms every block's maximum)
+  constexpr bool FOLD = MOD && HD == 128 && !FP8;
+  // Biases grow towards the row's own place: from there back, the first block sets the
+  // maximum, and none after it raises it far
+  constexpr bool BACK = MOD;
+
   typedef TileLoader<HD> TL;
   constexpr int TILE = TL::TILE_BYTES;
   constexpr int ROWB = HD * 2;   // bytes per LDS row
@@ -730,10 +1011,12 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
 
   // kv heads fastest: with a multiple of 8 of them, id % 8 (the XCD) fixes the
   // head modulo 8 and the tiles of a head share an L2
-  const Plan plan = make_plan(a, lane);
-  const int idx = quotient((int)blockIdx.x, a.Hk, a.Hk_inv), hk = (int)blockIdx.x - idx * a.Hk;
+  const Plan plan = make_plan(args, lane);
+  const int idx = quotient((int)blockIdx.x, args.Hk, args.Hk_inv);
+  const int hk = (int)blockIdx.x - idx * args.Hk;
   Item it;
-  if (!find_item(a, plan, lane, idx, 0, &it)) return;
+  if (!find_item(args, plan, lane, idx, 0, &it)) return;
+  const PagedArgs &a = MX ? arguments() : args;
   const int rows = it.n * a.group;
   const int off = it.len - it.n;  // place of the sequence's first new token
   const int r0 = it.tile * BM + w * 32;
@@ -757,10 +1040,18 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   const int kb0 = __builtin_amdgcn_readfirstlane(before + it.split * per);
   const int nv = __builtin_amdgcn_readfirstlane(min(max(all - kb0, 0), per));
   if (rows - it.tile * BM <= NARROW) {
-    narrow_item<E, HD, POOL, MOD>(a, it, hk, w, lane, kb0, nv, smem, mlbox);
+    if constexpr (MX) {
+      if (rows - it.tile * BM <= 16)
+        narrow_mx<E, HD, MOD, 1>(it, hk, w, lane, kb0, nv, smem, mlbox);
+      else
+        narrow_mx<E, HD, MOD, 2>(it, hk, w, lane, kb0, nv, smem, mlbox);
+    } else {
+      narrow_item<E, HD, POOL, MOD>(a, it, hk, w, lane, kb0, nv, smem, mlbox);
+    }
     return;
   }
   if (lane == 0) special[w] = 0;
+  auto block = [&](int t) { return BACK ? nv - 1 - t : t; };  // of the t-th step
   const int nkw = __builtin_amdgcn_readfirstlane(
       r0 < rows ? min(max(blocks_to(r0 + 31) - kb0, 0), nv) : 0);
   const int lo_w = __builtin_amdgcn_readfirstlane(off + quotient(min(r0, rows - 1), a.group, a.group_inv));
@@ -771,7 +1062,7 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   const int last_key = it.len - 1;
 
   // the window of the block table: lane j holds entry tab0 + j; the copies' pages
-  // only ever move on
+  // only ever move on (BACK: back)
   int tab0 = 0, tabv = 0;
   auto load_tab = [&](int first) {
     tab0 = first;
@@ -781,13 +1072,13 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   // the wave's run of block t: its page's byte offset in each pool, and the
   // tokens of it that exist less one (a run behind the end takes the last run)
   auto run_at = [&](int t, int64_t *ko, int64_t *vo, int *most, int *in, int *at) {
-    int run = (kb0 + t) * (BN / 16) + w;
+    int run = (kb0 + block(t)) * (BN / 16) + w;
     const int key = min(run * 16, last_key & ~15);
     run = key >> 4;
     int index, rest;
     page_of(a, run, &index, &rest);
-    if (index - tab0 >= 64) {
-      load_tab(index);
+    if (BACK ? index < tab0 : index - tab0 >= 64) {
+      load_tab(BACK ? max(index - 63, 0) : index);
       settle(tabv);
     }
     int page = __builtin_amdgcn_readlane(tabv, index - tab0);
@@ -865,41 +1156,57 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
             u32x4{lo[0], lo[1], hi[0], hi[1]};
       }
   };
-  // MXFP4 pools: a lane takes 32 / 64 HD codes of a row with their scale. A cycle's 16
-  // lanes write four rows, whose bits 2 and 3 (head_dim 64: 0 and 2) differ for V
-  const int mrow = lane >> 2;
-  const int mvrow = HD == 128 ? (mrow & 3) << 2 | mrow >> 2
-                              : (mrow & 1) | (mrow & 2) << 1 | (mrow & 4) << 1 | (mrow & 8) >> 2;
+  // MXFP4 pools: a lane takes a quarter of a row's codes, with their scale. Eight
+  // neighbouring lanes write at once, over 128 bytes: two quarters (head_dim 64: four) of
+  // rows whose swizzle differs in the unit's lowest bits
+  const int mpart = lane_bits(lane, HD == 128 ? 0x30 : 0x10);
+  const int mrow = lane_bits(lane, HD == 128 ? 0x5421 : 0x5423);
+  const int mvrow = lane_bits(lane, HD == 128 ? 0x2154 : 0x5243);
   constexpr int MB = HD / 8;  // bytes of codes a lane takes
   typedef typename std::conditional<HD == 128, u32x4, u32x2>::type mx_t;
   mx_t kmx, vmx;
-  uint32_t ksb = 0, vsb = 0;
+  row_scales<HD> ksb = {}, vsb = {};
   const char *const ksp = MX ? (const char *)a.kmx + hk * a.kss1 : nullptr;
   const char *const vsp = MX ? (const char *)a.vmx + hk * a.vss1 : nullptr;
-  const int mblk = HD == 128 ? lane & 3 : (lane & 3) >> 1;
+  const int mblk = HD == 128 ? mpart : mpart >> 1;
   auto mxswz = [](int r) { return tile_swizzle<HD, true>(r) | ((r >> 2) & 3); };
   const int kmput = (16 * w + mrow) * ROWB +
-                    (((MB / 4 * (lane & 3)) ^ tile_swizzle<HD, false>(16 * w + mrow)) << 4);
-  const int vmput = (16 * w + mvrow) * ROWB + (((MB / 4 * (lane & 3)) ^ mxswz(mvrow)) << 4);
-  auto load_mx = [&](const char *base, int64_t tokb, const char *scales, int64_t stok, int most,
-                     int row, mx_t *codes, uint32_t *scale) {
-    const int r = min(row, most);
-    *codes = *(const mx_t *)(base + (uint32_t)(r * (int)tokb + (lane & 3) * MB));
-    *scale = *(const uint8_t *)(scales + (uint32_t)(r * (int)stok + mblk));
+                    (((MB / 4 * mpart) ^ tile_swizzle<HD, false>(16 * w + mrow)) << 4);
+  const int vmput = (16 * w + mvrow) * ROWB + (((MB / 4 * mpart) ^ mxswz(mvrow)) << 4);
+  const uint32_t kmoff = mrow * (uint32_t)a.ktok + mpart * MB, ksoff = mrow * (uint32_t)a.kstok;
+  const uint32_t vmoff = mvrow * (uint32_t)a.vtok + mpart * MB, vsoff = mvrow * (uint32_t)a.vstok;
+  // the wave's run of a block: its page, first place in it and tokens that exist less
+  // one (narrow_mx on the rows behind). V's run of a block is K's, looked up before.
+  int mpage = 0, mplace = 0, mmost = 0;
+  auto look_mx = [&](int t) {
+    int64_t ko, vo;
+    run_at(t, &ko, &vo, &mmost, &mpage, &mplace);
   };
-  auto store_mx = [&](const mx_t &codes, uint32_t scale, const uint8_t *tile, int put) {
+  auto load_k_mx = [&]() {
+    kmx = *(const mx_t *)(mx_at(kp, mpage, a.kps0, mplace, a.ktok) + offset(kmoff));
+    ksb = *(const row_scales<HD> *)(mx_at(ksp, mpage, a.kss0, mplace, a.kstok) + offset(ksoff));
+  };
+  auto load_v_mx = [&]() {
+    vmx = *(const mx_t *)(mx_at(vp, mpage, a.vps0, mplace, a.vtok) + offset(vmoff));
+    vsb = *(const row_scales<HD> *)(mx_at(vsp, mpage, a.vss0, mplace, a.vstok) + offset(vsoff));
+  };
+  auto store_mx = [&](mx_t codes, float scale, const uint8_t *tile, int put) {
     asm volatile("" : "+v"(put));
 #pragma unroll
     for (int u = 0; u < MB / 4; ++u)
-      *(u32x4 *)(uint8_t *)(tile + (put ^ (u << 4))) = widen8<E>(codes[u], scale_byte(scale, 0));
+      *(u32x4 *)(uint8_t *)(tile + (put ^ (u << 4))) = widen8<E>(codes[u], scale);
+  };
+  auto put_k_mx = [&](int t) { store_mx(whole(kmx), scale_of(ksb, mblk), kslot(t), kmput); };
+  auto put_v_mx = [&](int t) {
+    const int key = (kb0 + block(t)) * BN + 16 * w + mvrow;
+    const float held = scale_of(vsb, mblk);
+    store_mx(whole(vmx), key <= last_key ? held : 0.0f, vslot(t), vmput);
   };
   auto load_k = [&](int t) {
     int64_t ko, vo;
     int most, page, at;
     run_at(t, &ko, &vo, &most, &page, &at);
-    if constexpr (MX)
-      load_mx(kp + ko, a.ktok, ksp + page * a.kss0 + at * a.kstok, a.kstok, most, mrow, &kmx, &ksb);
-    else if constexpr (FP8)
+    if constexpr (FP8)
       load8(kp + ko, a.ktok, most, krow8, k8);
     else
       copy(kp + ko, koff, a.ktok, most, false, kslot(t));
@@ -908,32 +1215,39 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
     int64_t ko, vo;
     int most, page, at;
     run_at(t, &ko, &vo, &most, &page, &at);
-    if constexpr (MX)
-      load_mx(vp + vo, a.vtok, vsp + page * a.vss0 + at * a.vstok, a.vstok, most, mvrow, &vmx, &vsb);
-    else if constexpr (FP8)
+    if constexpr (FP8)
       load8(vp + vo, a.vtok, most, vrow8, v8);
     else
       copy(vp + vo, voff, a.vtok, most, true, vslot(t));
   };
-  // codes: what load_k / load_v have in registers to LDS
+  // E4M3: what load_k / load_v have in registers to LDS
   auto put_k = [&](int t) {
     if constexpr (FP8) store8(k8, kslot(t), false);
-    if constexpr (MX) store_mx(kmx, ksb, kslot(t), kmput);
   };
   auto put_v = [&](int t) {
     if constexpr (FP8) store8(v8, vslot(t), true);
-    if constexpr (MX) store_mx(vmx, vsb, vslot(t), vmput);
   };
   auto put_next = [&](int jb) {
-    if (jb + 1 < nv) put_v(jb + 1);
-    if (jb + 2 < nv) put_k(jb + 2);
+    if constexpr (MX) {
+      // in every block (past the last into slots that none reads, of the last again): a
+      // branch around the loads would have their registers copied, and so waited for,
+      // behind it
+      put_v_mx(jb + 1);
+      put_k_mx(jb + 2);
+      load_v_mx();
+      look_mx(min(jb + 3, nv - 1));
+      load_k_mx();
+    } else {
+      if (jb + 1 < nv) put_v(jb + 1);
+      if (jb + 2 < nv) put_k(jb + 2);
+    }
   };
   // the wave's own rows of a V tile, before the others read them (16-bit pools:
   // their copy has landed; E4M3: they have been stored)
   const int hi_tile = __builtin_amdgcn_readfirstlane(
       off + quotient(min(it.tile * BM + BM, rows) - 1, a.group, a.group_inv));
   auto scrub_v = [&](int t) {
-    const int key = (kb0 + t) * BN;
+    const int key = (kb0 + block(t)) * BN;
     const bool cut = MOD && a.window && key + a.window <= hi_tile;  // at some row's window
     if (key + BN - 1 <= lo_tile && !cut) return;
     asm volatile("" ::: "memory");  // no read before the copy's wait
@@ -943,8 +1257,8 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   };
   if (nv > 0) {
     int index, rest;
-    page_of(a, kb0 * (BN / 16), &index, &rest);
-    load_tab(index);
+    page_of(a, BACK ? min((kb0 + nv) * (BN / 16) - 1, last_key >> 4) : kb0 * (BN / 16), &index, &rest);
+    load_tab(BACK ? max(index - 63, 0) : index);
   }
 
   // Q^T operand: k-step st covers head_dim 16 st + 8 g .. +7 of the row
@@ -981,12 +1295,26 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   for (int st = 0; st < NST; ++st) settle(qf[st]);
   settle(tabv);
   if (nv > 0) {
-    load_k(0);
-    load_v(0);
-    put_k(0);
-    if (nv > 1) load_k(1);
-    put_v(0);
-    if (nv > 1) put_k(1);
+    if constexpr (MX) {
+      look_mx(0);
+      load_k_mx();
+      load_v_mx();
+      put_k_mx(0);
+      look_mx(min(1, nv - 1));
+      load_k_mx();
+      put_v_mx(0);
+      put_k_mx(1);
+      load_v_mx();
+      look_mx(min(2, nv - 1));
+      load_k_mx();
+    } else {
+      load_k(0);
+      load_v(0);
+      put_k(0);
+      if (nv > 1) load_k(1);
+      put_v(0);
+      if (nv > 1) put_k(1);
+    }
   }
 
   // per-lane LDS byte offsets of the operand reads
@@ -1046,20 +1374,27 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
   wait_vmem();
   if (nv > 0) scrub_v(0);
   __syncthreads();
-  if (nkw > 0) qk_from(kslot(0), k_operand(kslot(0), 0), k_operand(kslot(0), 1));
+  if (nv > 0 && block(0) < nkw) qk_from(kslot(0), k_operand(kslot(0), 0), k_operand(kslot(0), 1));
   __syncthreads();  // every wave is done with K slot 0 before it is refilled
 
   for (int jb = 0; jb < nv; ++jb) {
     // K of block jb + 2 goes to the slot block jb's K has left, V of block
     // jb + 1 to the slot of block jb - 1's V (E4M3: in registers until the softmax
     // is done, and written then, which the matrix products hide: 247 us against 254)
-    if (jb + 1 < nv) load_v(jb + 1);
-    if (jb + 2 < nv) load_k(jb + 2);
-    if (jb < nkw) {
+    if (!MX && jb + 1 < nv) load_v(jb + 1);
+    if (!MX && jb + 2 < nv) load_k(jb + 2);
+    const bool live = block(jb) < nkw;
+    const bool next_live = jb + 1 < nv && block(jb + 1) < nkw;
+    const uint8_t *const vt = vslot(jb);
+    u32x4 vp0 = {}, vp1 = {}, pf[4] = {};
+    if (live) {
       // the first two V^T operands of this block's P.V, read before the softmax
-      const uint8_t *vt = vslot(jb);
-      const u32x4 vp0 = v_operand(vt, 0), vp1 = v_operand(vt, 1);
-      const int key0 = (kb0 + jb) * BN;
+      // (codes and shaped scores leave no registers for them until then)
+      if constexpr (!(CODES && MOD)) {
+        vp0 = v_operand(vt, 0);
+        vp1 = v_operand(vt, 1);
+      }
+      const int key0 = (kb0 + block(jb)) * BN;
       float sc = a.scale2;
       // E4M3: V's scales (over scale_unit) meet P. Over a block within one page K's scale goes with
       // the score scale and V's into the exponent (lv), so they cost no operation
@@ -1072,8 +1407,8 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
       if constexpr (FP8) {
         int index, rest;
         page_of(a, key0 >> 4, &index, &rest);
-        if (index + 3 - sc0 >= 64) {
-          load_scales(index);
+        if (BACK ? index < sc0 : index + 3 - sc0 >= 64) {
+          load_scales(BACK ? max(index - 60, 0) : index);
           // here, not where they are read: that would drain the loads above too
           settle(kscv);
           settle(vscv);
@@ -1108,100 +1443,154 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
       // element (kb, r) holds key key0 + 4 g + c with c = 32 kb + 8 (r >> 2)
       // + (r & 3): it is masked when c passes the row's own place
       const int lim = pos - key0 - 4 * g;
-      if constexpr (MOD) {
+      const bool edge = MOD && a.window && key0 + a.window <= hi_w;  // of some row's window
+      float rs = 0.0f;
+      // Capped and biased scores, of blocks that every row sees whole and whose maxima
+      // stay where they were: the cap's polynomial and the bias are part of the exponent,
+      // 5 vector instructions an element and 1, where shape() takes 8 and 3
+      bool done = false;
+      if constexpr (FOLD) {
+        done = jb > 0 && key0 + BN - 1 <= lo_w && !edge;
+        if (done && a.cap2 != 0.0f) {
+          float big = 0.0f;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) shape(a, slope2, sc, (float)-lim, 32 * kb, s[kb]);
-        sc = 1.0f;
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(s[kb][r]));
+          done = !__any(!(big <= a.cap_most));
+        }
+        if (done) {
+          const float b0 = fmaf(slope2, (float)-lim, -m);
+          auto expo_of = [&](auto score) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int kb = c >> 1, r = 8 * (c & 1) + 2 * i, at = 32 * kb + 8 * (r >> 2) + (r & 3);
+                const float p0 = fast_exp2(score(s[kb][r], (float)at));
+                const float p1 = fast_exp2(score(s[kb][r + 1], (float)(at + 1)));
+                rs = c + i == 0 ? p0 : rs + p0;
+                rs += p1;
+                pf[c][i] = E::pack2(p0, p1);
+              }
+          };
+          auto capped = [&](float x, float b) {
+            const float w = x * x;
+            float p = fmaf(w, a.capq[3], a.capq[2]);
+            p = fmaf(w, p, a.capq[1]);
+            return fmaf(x, fmaf(w, p, a.capq[0]), b);
+          };
+          if (a.cap2 != 0.0f && a.slopes)
+            expo_of([&](float x, float c) { return capped(x, fmaf(slope2, c, b0)); });
+          else if (a.cap2 != 0.0f)
+            expo_of([&](float x, float) { return capped(x, -m); });
+          else if (a.slopes)
+            expo_of([&](float x, float c) { return fmaf(x, sc, fmaf(slope2, c, b0)); });
+          else
+            expo_of([&](float x, float) { return fmaf(x, sc, -m); });
+          done = !__any(!(rs <= kSumCap));
+        }
       }
-      if (key0 + BN - 1 > lo_w) {
+      if (!FOLD || !done) {
+        if constexpr (MOD) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+          for (int kb = 0; kb < 2; ++kb) shape<16>(a, slope2, sc, (float)-lim, 32 * kb, s[kb]);
+          sc = 1.0f;
+        }
+        if (key0 + BN - 1 > lo_w) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (32 * kb + 8 * (r >> 2) + (r & 3) > lim) s[kb][r] = -INFINITY;
-      }
-      if constexpr (MOD)
-        if (a.window && key0 + a.window <= hi_w) {  // some row's window begins behind its keys
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (32 * kb + 8 * (r >> 2) + (r & 3) > lim) s[kb][r] = -INFINITY;
+        }
+        if (edge) {
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
               if (32 * kb + 8 * (r >> 2) + (r & 3) <= lim - a.window) s[kb][r] = -INFINITY;
         }
-      // p = 2^(s sc - m) for the block, packed for P.V, and the lane's sum
-      float rs;
-      u32x4 pf[4];
-      auto expo = [&]() {
-        const float nm = FP8 ? lv - m : -m;
+        // p = 2^(s sc - m) for the block, packed for P.V, and the lane's sum
+        auto expo = [&]() {
+          const float nm = FP8 ? lv - m : -m;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int kb = c >> 1, hh = c & 1;
+          for (int c = 0; c < 4; ++c) {
+            const int kb = c >> 1, hh = c & 1;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float p0 = fast_exp2(fmaf(s[kb][8 * hh + 2 * i], sc, nm));
-            const float p1 = fast_exp2(fmaf(s[kb][8 * hh + 2 * i + 1], sc, nm));
-            rs = c + i == 0 ? p0 : rs + p0;
-            rs += p1;
-            pf[c][i] = E::pack2(p0, p1);  // 16 bits, for P.V alone
+            for (int i = 0; i < 4; ++i) {
+              const float p0 = fast_exp2(fmaf(s[kb][8 * hh + 2 * i], sc, nm));
+              const float p1 = fast_exp2(fmaf(s[kb][8 * hh + 2 * i + 1], sc, nm));
+              rs = c + i == 0 ? p0 : rs + p0;
+              rs += p1;
+              pf[c][i] = E::pack2(p0, p1);  // 16 bits, for P.V alone
+            }
           }
-        }
-        if constexpr (FP8) {
-          rs *= iv;
-          if (apart) {
+          if constexpr (FP8) {
+            rs *= iv;
+            if (apart) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+              for (int c = 0; c < 4; ++c)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float p0 = fast_exp2(fmaf(s[c >> 1][8 * (c & 1) + 2 * i], sc, nm));
-                const float p1 = fast_exp2(fmaf(s[c >> 1][8 * (c & 1) + 2 * i + 1], sc, nm));
-                // (a masked key's page may hold any scale)
-                pf[c][i] = E::pack2(p0 == 0.0f ? 0.0f : p0 * vs[c], p1 == 0.0f ? 0.0f : p1 * vs[c]);
-              }
+                for (int i = 0; i < 4; ++i) {
+                  const float p0 = fast_exp2(fmaf(s[c >> 1][8 * (c & 1) + 2 * i], sc, nm));
+                  const float p1 = fast_exp2(fmaf(s[c >> 1][8 * (c & 1) + 2 * i + 1], sc, nm));
+                  // (a masked key's page may hold any scale)
+                  pf[c][i] = E::pack2(p0 == 0.0f ? 0.0f : p0 * vs[c], p1 == 0.0f ? 0.0f : p1 * vs[c]);
+                }
+            }
           }
-        }
-      };
-      auto raise_max = [&](float slack) {  // m to the block's max where that passes m + slack
-        float mx = -INFINITY;
+        };
+        auto raise_max = [&](float slack) {  // m to the block's max where that passes m + slack
+          float mx = -INFINITY;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+          for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
-        mx = pair_max(mx);
-        const float m_blk = mx * sc;
-        if (__any(m_blk > m + slack)) {
-          const float m_new = fmaxf(m, m_blk);
-          const float alpha = fast_exp2(m - m_new);
-          lsum *= alpha;
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
+          mx = pair_max(mx);
+          const float m_blk = mx * sc;
+          if (__any(m_blk > m + slack)) {
+            const float m_new = fmaxf(m, m_blk);
+            const float alpha = fast_exp2(m - m_new);
+            lsum *= alpha;
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[nb][r] *= alpha;
-          m = m_new;
-        }
-      };
-      if constexpr (HD == 64) {
-        raise_max(0.0f);
-        expo();
-      } else {
-        // the block max is only formed when it can matter: past the first block,
-        // a lane sum of at most 2^kSlack bounds every p by it, and m keeps
-        bool full = jb == 0;
-        if (!full) {
+              for (int r = 0; r < 16; ++r) o[nb][r] *= alpha;
+            m = m_new;
+          }
+        };
+        if constexpr (HD == 64) {
+          raise_max(0.0f);
           expo();
-          full = __any(!(rs <= kSumCap));
-        }
-        if (full) {
-          raise_max(kSlack);
-          expo();
+        } else {
+          // the block max is only formed when it can matter: past the first block,
+          // a lane sum of at most 2^kSlack bounds every p by it, and m keeps
+          bool full = jb == 0;
+          if (!full) {
+            expo();
+            full = __any(!(rs <= kSumCap));
+          }
+          if (full) {
+            // (BACK: the first block may show a row few keys; a maximum left below the
+            // next ones' would bring every block here)
+            raise_max(BACK ? 0.0f : kSlack);
+            expo();
+          }
         }
       }
       lsum += rs;
-      if constexpr (CODES) put_next(jb);
-
+    }
+    if constexpr (CODES) put_next(jb);
+    if (live) {
       // O^T += V^T P^T, then the next block's S^T, at raised issue priority
       __builtin_amdgcn_s_setprio(1);
       // (reads run two MFMAs ahead, as above; the last are the next block's first two
       // K operands: past the last block those are stale and dropped)
+      if constexpr (CODES && MOD) {
+        vp0 = v_operand(vt, 0);
+        vp1 = v_operand(vt, 1);
+      }
       u32x4 next[4] = {vp0, vp1};
 #pragma unroll
       for (int st = 0; st < NPV; ++st) {
@@ -1211,10 +1600,11 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs a) {
         o[st % NB] = E::mfma32(as_vec8<V8>(next[st & 3]), as_vec8<V8>(pf[st / NB]), o[st % NB]);
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (jb + 1 < nkw) qk_from(kslot(jb + 1), next[NPV & 3], next[(NPV + 1) & 3]);
+      if (next_live) qk_from(kslot(jb + 1), next[NPV & 3], next[(NPV + 1) & 3]);
       __builtin_amdgcn_s_setprio(0);
-    } else if constexpr (CODES) {
-      put_next(jb);
+    } else if (BACK && next_live) {  // the wave's rows end before this block's keys
+      const uint8_t *kt = kslot(jb + 1);
+      qk_from(kt, k_operand(kt, 0), k_operand(kt, 1));
     }
     if constexpr (!CODES) wait_vmem();
     if (jb + 1 < nv) scrub_v(jb + 1);
@@ -1389,8 +1779,16 @@ inline PagedArgs paged_args(const PagedAttnLaunch &L) {
   if (L.softcap > 0.0f) {
     a.cap2 = L.softcap * kLog2e;
     a.cap_inv = 1.0f / a.cap2;
-    const float c[5] = {1.0f, -0x1.5554a6p-2f, 0x1.10e47ap-3f, -0x1.b2167ep-5f, 0x1.18d7e8p-6f};
-    for (int i = 0; i < 5; ++i) a.capp[i] = c[i] * a.cap2;
+    const float c[4] = {0x1.fffffep-1f, -0x1.5551cap-2f, 0x1.1011b4p-3f, -0x1.8b7eacp-5f};
+    // of the products themselves, where the powers of u stay ordinary numbers
+    const double u = (double)L.scale_log2 / a.cap2;
+    double power = u * a.cap2;
+    for (int i = 0; i < 4; ++i) {
+      a.capp[i] = c[i] * a.cap2;
+      a.capq[i] = (float)(c[i] * power);
+      power *= u * u;
+    }
+    a.cap_most = u >= 0x1p-16 && u <= 0x1p16 ? (float)(kCapPoly / u) : -1.0f;
   }
   return a;
 }

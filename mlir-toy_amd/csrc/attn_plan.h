@@ -18,6 +18,7 @@ constexpr int kParts = 2 * kSlots;  // items of cut tiles in a launch at most (m
 // tiles): 32 x 1 over 8000 164 / 182, E4M3 95 / 154, 16 x 1-4 over 8000 69 / 79, 1 over
 // 2000 12.6 / 13.7; a tile of more rows than one wave's 32 needs the wide one's waves.
 constexpr int NARROW = 32;
+constexpr float kCapPoly = 0.375f;  // |y| up to which the cap's polynomials hold
 
 struct PagedArgs {
   const uint16_t *q;
@@ -43,8 +44,10 @@ struct PagedArgs {
   const float *slopes;            // [Hq], nullable
   int32_t window;                 // keys a row sees at most; 0: all
   uint32_t blocks_1;              // blocks that a tile's windows span at most, plus 1; 0: all
-  float cap2, cap_inv, capp[5];   // the cap in log2 units (0: none), its inverse, tanh(y) / y
-                                  // times the cap as a polynomial of y^2
+  float cap2, cap_inv;            // the cap in log2 units (0: none) and its inverse
+  float capp[4], capq[4];         // tanh(y) / y times the cap as a polynomial of y^2, y the
+                                  // score over the cap, and one of the product's square
+  float cap_most;                 // products that the latter holds for (-1: none)
 };
 
 // floor(x / d), inv = floor((2^32 - 1) / d): the estimate is that or one less
