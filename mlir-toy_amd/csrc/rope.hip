@@ -97,6 +97,8 @@ struct RopeArgs {
   int32_t half, P, interleaved;    // pairs rotated, table rows
   int32_t B, ps, maxp, npages;
   float eps, inv_dim;
+  uint32_t keys, keys_step;        // append_mx: the keys' work-groups, their share of all as
+                                   // a fraction of 2^32, rounded up
 };
 
 // sum over aligned groups of N (4, 8 or 16) lanes, in every lane: DPP moves
@@ -199,16 +201,208 @@ __device__ inline uint32_t mx8(f32x4 a, f32x4 b, uint32_t *byte) {
   return e == 0u || e == 255u ? 0u : c;
 }
 
+// An appended token's position and slot; `live`: whether it is stored
+struct Slot {
+  int t, page = -1, place = 0;
+  bool live;
+};
+// end: chunk_end's, where there is cu_seqlens
+template <int LPR, bool POOL_ROW>
+__device__ inline Slot slot_of(const RopeArgs &a, int lane, int tok, int end, bool live) {
+  Slot s;
+  s.live = live;
+  int b = tok, left = 1;
+  if (a.cu) {
+    b = sequence_of<LPR>(a.cu, a.B, lane, tok, end);
+    s.live = s.live && b < a.B && a.cu[0] <= tok;  // rows behind the last sequence stay as they were
+    b = min(b, a.B - 1);
+    left = a.cu[b + 1] - tok;
+  }
+  s.t = a.lens[b] - left;
+  if constexpr (POOL_ROW) {
+    const int index = (int)((uint32_t)max(s.t, 0) / (uint32_t)a.ps);
+    s.place = max(s.t, 0) - index * a.ps;
+    if (s.t >= 0 && index < a.maxp) s.page = a.btab[(int64_t)b * a.maxp + index];
+    // a key or value without a slot is not stored
+    s.live = s.live && s.page >= 0 && s.page < a.npages;
+  }
+  return s;
+}
+
+// A row's codes and scales to its slot: 4 bytes of the lane's codes, the row's scales by
+// its first lane (byte: of the lane's block)
+template <int LPR>
+__device__ inline void store_mx(const RopeSide &x, const Slot &slot, int h, int l, uint32_t codes,
+                                uint32_t byte) {
+  byte <<= 8 * (l >> 2);
+  if constexpr (LPR == 16) {
+    byte |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)byte, 0x124, 0xf, 0xf, true);  // row_ror 4
+    byte |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)byte, 0x128, 0xf, 0xf, true);  // row_ror 8
+  } else {
+    byte |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)byte, 0x141, 0xf, 0xf, true);  // row_half_mirror
+  }
+  if (!slot.live || h >= x.heads) return;
+  *(uint32_t *)(x.out + slot.page * x.os[0] + slot.place * x.os[2] + h * x.os[1] + 4 * l) = codes;
+  uint8_t *to = x.bytes + slot.page * x.ss[0] + slot.place * x.ss[2] + h * x.ss[1];
+  if (l == 0) {
+    if constexpr (LPR == 16)
+      *(uint32_t *)to = byte;
+    else
+      *(uint16_t *)to = (uint16_t)byte;
+  }
+}
+
+// y rounded to fp32 so that no number of fp32 lies between them: towards 0, with the last
+// bit set where something was lost. A code's borders are such numbers, so the code is
+// the one nearest to y itself.
+__device__ inline float to_odd(double y) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, y);
+  constexpr uint32_t LOST = 0x1fffffffu;  // of an fp64's lower word
+  uint32_t lo = (uint32_t)u;
+  lo = (lo | ((lo & LOST) + LOST)) & ~LOST;
+  return (float)__builtin_bit_cast(double, u >> 32 << 32 | lo);
+}
+
+// sum over aligned groups of N (8 or 16) lanes, in every lane
+template <int N>
+__device__ inline double group_sum64(double x) {
+  auto add = [&](auto ctrl) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)u, decltype(ctrl)::value, 0xf, 0xf, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), decltype(ctrl)::value, 0xf, 0xf, true);
+    x += __builtin_bit_cast(double, (uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+  };
+  add(std::integral_constant<int, 0xb1>{});
+  add(std::integral_constant<int, 0x4e>{});
+  add(std::integral_constant<int, 0x141>{});
+  if constexpr (N == 16) add(std::integral_constant<int, 0x140>{});
+  return x;
+}
+
+// 1 / sqrt(x): v_rsq_f64 and two Newton steps
+__device__ inline double inverse_root64(double x) {
+  double r = __builtin_amdgcn_rsq(x);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) r = fma(r * 0.5, fma(-x * r, r, 1.0), r);
+  return r;
+}
+
+// Keys on their way into MXFP4 pools. Four bits leave borders far apart, and a key that
+// fp32's norm and rotation leave on the wrong side of one is off by a whole step: one in
+// 10^6 elements (0.00027 of 15000 tokens' norm). In fp64, which this GPU's vector unit
+// runs as fast, a key's code is the nearest one. A lane has eight neighbours, so that four
+// hold a block, and for half-split pairs their partners, loaded beside them.
+constexpr int keys_hpg(int hpg) { return hpg < 2 ? hpg : 2; }  // (fp64's factors take registers)
+template <class E, int D, int HPG>
+__device__ inline void keys_mx(const RopeArgs &a, uint32_t block) {
+  typedef typename E::raw raw;
+  constexpr int LPR = D / 8;
+  const int lane = threadIdx.x & 63, l = threadIdx.x % LPR;
+  const RopeSide &x = a.side[1];
+  const uint32_t gid = block * (NT / LPR) + threadIdx.x / LPR;
+  const int at = (int)divide(gid, x.runs, x.runs_inv), run = (int)gid - at * x.runs;
+  const int tok = min(at, a.tokens - 1);
+  int end = 0x7fffffff;
+  if (a.cu) end = chunk_end(a.cu, a.B, lane);
+  // the lane's two runs of four: their partners, and their pairs' places in the tables
+  const bool beside = !a.interleaved && a.half > 0;
+  int poff[2], pair[2];
+  bool turns[2], upper[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int e = 8 * l + 4 * i;
+    turns[i] = e < 2 * a.half;
+    upper[i] = beside && e >= a.half;
+    pair[i] = !turns[i] ? 0 : a.interleaved ? e / 2 : upper[i] ? e - a.half : e;
+    poff[i] = !turns[i] || !beside ? e : upper[i] ? e - a.half : e + a.half;
+  }
+  raw xr[HPG][2], ur[HPG][2];
+#pragma unroll
+  for (int i = 0; i < HPG; ++i) {
+    const char *src = x.in + tok * x.is[2] + min(run + i * x.runs, x.heads - 1) * x.is[1];
+    E::load8(src + 8 * E::SIZE * l, xr[i][0], xr[i][1]);
+    if (beside) {
+      ur[i][0] = *(const raw *)(src + poff[0] * E::SIZE);
+      ur[i][1] = *(const raw *)(src + poff[1] * E::SIZE);
+    }
+  }
+  const Slot slot = slot_of<LPR, true>(a, lane, tok, end, at < a.tokens);
+
+  // element e of run i: y = r (x p + partner q)
+  double p[2][4], q[2][4];
+  {
+    f32x4 c[2], s[2], w[2], wp[2];
+    const int64_t row = (int64_t)min(max(slot.t, 0), a.P - 1) * a.half;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      c[i] = w[i] = wp[i] = f32x4{1, 1, 1, 1};
+      s[i] = f32x4{0, 0, 0, 0};
+      if (a.half && a.interleaved) {  // two pairs
+        const f32x2 c2 = *(const f32x2 *)(a.cos + row + pair[i]);
+        const f32x2 s2 = *(const f32x2 *)(a.sin + row + pair[i]);
+        c[i] = f32x4{c2[0], c2[0], c2[1], c2[1]};
+        s[i] = f32x4{-s2[0], s2[0], -s2[1], s2[1]};
+      } else if (a.half) {
+        c[i] = *(const f32x4 *)(a.cos + row + pair[i]);
+        s[i] = *(const f32x4 *)(a.sin + row + pair[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = upper[i] ? s[i][j] : -s[i][j];
+      }
+      if (x.w) {
+        w[i] = *(const f32x4 *)(x.w + 8 * l + 4 * i);
+        wp[i] = *(const f32x4 *)(x.w + poff[i]);
+        if (a.interleaved) wp[i] = f32x4{wp[i][1], wp[i][0], wp[i][3], wp[i][2]};
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        p[i][j] = (double)w[i][j] * (turns[i] ? c[i][j] : 1.0f);
+        q[i][j] = (double)wp[i][j] * s[i][j];
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < HPG; ++k) {
+    f32x4 y[2], u[2];
+    double ss = 0.0, r = 1.0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      y[i] = E::load(xr[k][i]);
+      u[i] = beside ? E::load(ur[k][i]) : f32x4{y[i][1], y[i][0], y[i][3], y[i][2]};
+    }
+    if (x.w) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ss = fma((double)y[i][j], (double)y[i][j], ss);
+      r = inverse_root64(group_sum64<LPR>(ss) * (1.0 / D) + (double)a.eps);
+    }
+    f32x4 z[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        double v = (double)y[i][j] * p[i][j];
+        if (turns[i]) v = fma((double)u[i][j], q[i][j], v);  // (others have no partner)
+        z[i][j] = to_odd(v * r);
+      }
+    uint32_t byte;
+    const uint32_t codes = mx8(z[0], z[1], &byte);
+    store_mx<LPR>(x, slot, run + k * x.runs, l, codes, byte);
+  }
+}
+
 // KIND: 0 queries, 1 keys, 2 values
 template <class E, int D, bool APPEND, int POOL, int HPG, int KIND>
-__device__ inline void rows(const RopeArgs &a) {
+__device__ inline void rows(const RopeArgs &a, uint32_t block) {
   typedef typename E::raw raw;
   constexpr int LPR = D / 8;
   constexpr bool TO_POOL = APPEND && KIND > 0;
   constexpr bool FP8 = POOL == E4M3, MX = POOL == MXFP4 && TO_POOL;
   const int lane = threadIdx.x & 63, l = threadIdx.x % LPR;
   const RopeSide &x = a.side[KIND];
-  const uint32_t gid = (blockIdx.x - x.first) * (NT / LPR) + threadIdx.x / LPR;
+  const uint32_t gid = block * (NT / LPR) + threadIdx.x / LPR;
   const int at = (int)divide(gid, x.runs, x.runs_inv), run = (int)gid - at * x.runs;
   const int tok = min(at, a.tokens - 1);
   bool live = at < a.tokens;
@@ -224,24 +418,8 @@ __device__ inline void rows(const RopeArgs &a) {
 
   // this lane's two runs of four elements, the rotated ones' pairs 4l ..; flat: all
   // lanes' runs are neighbours
-  const bool flat = KIND == 2 || a.interleaved || a.half == 0 || MX;
+  const bool flat = KIND == 2 || a.interleaved || a.half == 0;
   const bool turns = KIND < 2 && 4 * l < a.half;
-  // MXFP4: a block's 32 elements are four lanes', so keys keep their order here, and a
-  // run's partners (half-split pairs) are loaded beside it: run i of the lane, its
-  // element e, has its partner at e + half or e - half
-  const bool beside = MX && KIND == 1 && !a.interleaved && a.half > 0;
-  int poff[2] = {}, pair[2] = {};
-  bool pairs[2] = {}, upper[2] = {};
-  if constexpr (MX && KIND == 1) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int e = 8 * l + 4 * i;
-      pairs[i] = beside && e < 2 * a.half;
-      upper[i] = e >= a.half;
-      pair[i] = pairs[i] ? (upper[i] ? e - a.half : e) : 0;
-      poff[i] = !pairs[i] ? e : upper[i] ? e - a.half : e + a.half;
-    }
-  }
   const int offa = turns && !flat ? 4 * l : 8 * l;
   const int offb = turns && !flat ? 4 * l + a.half : 8 * l + 4;
   const char *src = x.in + (APPEND ? 0 : t0 * x.is[0]) + t1 * x.is[2];
@@ -258,40 +436,19 @@ __device__ inline void rows(const RopeArgs &a) {
     }
   }
 
-  raw ua[MX ? HPG : 1], ub[MX ? HPG : 1];  // the partners' runs
-  if constexpr (MX && KIND == 1) {
-    if (beside) {
-#pragma unroll
-      for (int i = 0; i < HPG; ++i) {
-        ua[i] = *(const raw *)(row_in(i) + poff[0] * E::SIZE);
-        ub[i] = *(const raw *)(row_in(i) + poff[1] * E::SIZE);
-      }
-    }
-  }
-
   float scale[HPG];
   if constexpr (!APPEND) t = a.pos[tok];
   if constexpr (APPEND) {
-    int b = tok, left = 1;
-    if (a.cu) {
-      b = sequence_of<LPR>(a.cu, a.B, lane, tok, end);
-      live = live && b < a.B && a.cu[0] <= tok;  // rows behind the last sequence stay as they were
-      b = min(b, a.B - 1);
-      left = a.cu[b + 1] - tok;
-    }
-    t = a.lens[b] - left;
-    if constexpr (KIND > 0) {
-      const int index = (int)((uint32_t)max(t, 0) / (uint32_t)a.ps);
-      place = max(t, 0) - index * a.ps;
-      if (t >= 0 && index < a.maxp) page = a.btab[(int64_t)b * a.maxp + index];
-      // a key or value without a slot is not stored
-      live = live && page >= 0 && page < a.npages;
-      if constexpr (FP8 && TO_POOL)
+    const Slot slot = slot_of<LPR, (KIND > 0)>(a, lane, tok, end, live);
+    t = slot.t;
+    page = slot.page;
+    place = slot.place;
+    live = slot.live;
+    if constexpr (FP8 && TO_POOL)
 #pragma unroll
-        for (int i = 0; i < HPG; ++i)
-          scale[i] = live ? x.scales[(int64_t)page * x.heads + min(run + i * x.runs, x.heads - 1)]
-                          : 1.0f;
-    }
+      for (int i = 0; i < HPG; ++i)
+        scale[i] = live ? x.scales[(int64_t)page * x.heads + min(run + i * x.runs, x.heads - 1)]
+                        : 1.0f;
   }
 
   // the factors of the lane's elements, and of their partners: the other run's
@@ -300,38 +457,17 @@ __device__ inline void rows(const RopeArgs &a) {
   if constexpr (KIND < 2) {
     // all four loads are in flight before the first is waited for
     f32x4 c = pa, s = qa;
-    if (beside) {
-      const int64_t row = (int64_t)min(max(t, 0), a.P - 1) * a.half;
-      f32x4 cb = *(const f32x4 *)(a.cos + row + pair[1]), sb = *(const f32x4 *)(a.sin + row + pair[1]);
-      c = *(const f32x4 *)(a.cos + row + pair[0]);
-      s = *(const f32x4 *)(a.sin + row + pair[0]);
-      qa = qb = f32x4{1, 1, 1, 1};
-      if (x.w) {
-        pa = *(const f32x4 *)(x.w + offa);
-        pb = *(const f32x4 *)(x.w + offb);
-        qa = *(const f32x4 *)(x.w + poff[0]);
-        qb = *(const f32x4 *)(x.w + poff[1]);
-      }
-      asm volatile("" : "+v"(c), "+v"(s), "+v"(cb), "+v"(sb), "+v"(pa), "+v"(pb), "+v"(qa), "+v"(qb));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        pa[j] *= pairs[0] ? c[j] : 1.0f;
-        pb[j] *= pairs[1] ? cb[j] : 1.0f;
-        qa[j] *= upper[0] ? s[j] : -s[j];
-        qb[j] *= upper[1] ? sb[j] : -sb[j];
-      }
-    }
-    if (!beside && a.half) {
+    if (a.half) {
       const int64_t row = (int64_t)min(max(t, 0), a.P - 1) * a.half + min(4 * l, a.half - 4);
       c = *(const f32x4 *)(a.cos + row);
       s = *(const f32x4 *)(a.sin + row);
     }
-    if (!beside && x.w) {
+    if (x.w) {
       pa = *(const f32x4 *)(x.w + offa);
       pb = *(const f32x4 *)(x.w + offb);
     }
     asm volatile("" : "+v"(c), "+v"(s), "+v"(pa), "+v"(pb));
-    if (turns && !beside) {
+    if (turns) {
       if (a.interleaved) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -377,13 +513,7 @@ __device__ inline void rows(const RopeArgs &a) {
         const float oa = a.interleaved ? ya[j ^ 1] : yb[j], ob = a.interleaved ? yb[j ^ 1] : ya[j];
         za[j] = ya[j] * pa[j];
         zb[j] = yb[j] * pb[j];
-        if (beside) {
-          if constexpr (MX) {
-            const f32x4 oa = E::load(ua[i]), ob = E::load(ub[i]);
-            if (pairs[0]) za[j] = fmaf(oa[j], qa[j], za[j]);
-            if (pairs[1]) zb[j] = fmaf(ob[j], qb[j], zb[j]);
-          }
-        } else if (turns) {
+        if (turns) {
           za[j] = fmaf(oa, qa[j], za[j]);
           zb[j] = fmaf(ob, qb[j], zb[j]);
         }
@@ -391,30 +521,19 @@ __device__ inline void rows(const RopeArgs &a) {
       ya = za * r;
       yb = zb * r;
     }
-    uint32_t codes = 0, bytes = 0;
-    if constexpr (MX) {
-      codes = mx8(ya, yb, &bytes);
-      // the row's scales, a byte for each four lanes
-      bytes <<= 8 * (l >> 2);
-      if constexpr (LPR == 16) {
-        bytes |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)bytes, 0x124, 0xf, 0xf, true);  // row_ror 4
-        bytes |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)bytes, 0x128, 0xf, 0xf, true);  // row_ror 8
-      } else {
-        bytes |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)bytes, 0x141, 0xf, 0xf, true);  // row_half_mirror
-      }
+    if constexpr (MX) {  // values
+      Slot slot;
+      slot.page = page;
+      slot.place = place;
+      slot.live = live;
+      uint32_t byte;
+      const uint32_t codes = mx8(ya, yb, &byte);
+      store_mx<LPR>(x, slot, h, l, codes, byte);
+      continue;
     }
     if (!live || h >= x.heads) continue;
     char *p = dst + h * x.os[1];
-    if constexpr (MX) {
-      *(uint32_t *)(p + 4 * l) = codes;
-      uint8_t *to = x.bytes + page * x.ss[0] + place * x.ss[2] + h * x.ss[1];
-      if (l == 0) {
-        if constexpr (LPR == 16)
-          *(uint32_t *)to = bytes;
-        else
-          *(uint16_t *)to = (uint16_t)bytes;
-      }
-    } else if constexpr (FP8 && TO_POOL) {
+    if constexpr (FP8 && TO_POOL) {
       const u32x2 c = codes8(ya, yb, scale[i]);
       if (flat) {
         *(u32x2 *)(p + 8 * l) = c;
@@ -436,11 +555,26 @@ __device__ inline void rows(const RopeArgs &a) {
 template <class E, int D, bool APPEND, int POOL, int HPG>
 __global__ __launch_bounds__(NT) void norm_rope(RopeArgs a) {
   if (blockIdx.x < a.side[1].first)
-    rows<E, D, APPEND, POOL, HPG, 0>(a);
+    rows<E, D, APPEND, POOL, HPG, 0>(a, blockIdx.x - a.side[0].first);
   else if (!APPEND || blockIdx.x < a.side[2].first)
-    rows<E, D, APPEND, POOL, HPG, 1>(a);
+    rows<E, D, APPEND, POOL, HPG, 1>(a, blockIdx.x - a.side[1].first);
   else if constexpr (APPEND)
-    rows<E, D, APPEND, POOL, HPG, 2>(a);
+    rows<E, D, APPEND, POOL, HPG, 2>(a, blockIdx.x - a.side[2].first);
+}
+
+// The append into MXFP4 pools. Keys take the vector unit's time, queries memory's: the
+// keys' work-groups are spread evenly among the others (11700 tokens of 32 + 8 heads
+// 43.6 us, behind the queries 47.5; in fp32 41).
+template <class E, int D, int HPG>
+__global__ __launch_bounds__(NT) void append_mx(RopeArgs a) {
+  const uint32_t b = blockIdx.x;
+  const uint32_t before = min(__umulhi(b, a.keys_step), a.keys);  // keys' ahead of this one
+  if (min(__umulhi(b + 1, a.keys_step), a.keys) > before)
+    keys_mx<E, D, keys_hpg(HPG)>(a, before);
+  else if (b - before < a.side[1].first)
+    rows<E, D, true, MXFP4, HPG, 0>(a, b - before);
+  else
+    rows<E, D, true, MXFP4, HPG, 2>(a, b - before - a.side[1].first);
 }
 
 template <class E, int D, bool APPEND, int POOL>
@@ -453,11 +587,19 @@ hipError_t launch_hpg(RopeArgs a, hipStream_t s) {
       RopeSide &x = a.side[i];
       x.first = blocks;
       if (!x.heads) continue;
-      x.runs = (x.heads + HPG - 1) / HPG;
+      const int take = POOL == MXFP4 && i == 1 ? keys_hpg(HPG) : HPG;
+      x.runs = (x.heads + take - 1) / take;
       x.runs_inv = 0xffffffffu / (uint32_t)x.runs;
       blocks += (uint32_t)(((int64_t)a.tokens * x.runs + GPB - 1) / GPB);
     }
-    hipLaunchKernelGGL((norm_rope<E, D, APPEND, POOL, HPG>), dim3(blocks), dim3(NT), 0, s, a);
+    if constexpr (POOL == MXFP4) {
+      a.keys = a.side[2].first - a.side[1].first;
+      a.keys_step = (uint32_t)((((uint64_t)a.keys << 32) + blocks - 1) / blocks);
+    }
+    if constexpr (POOL == MXFP4)
+      hipLaunchKernelGGL((append_mx<E, D, HPG>), dim3(blocks), dim3(NT), 0, s, a);
+    else
+      hipLaunchKernelGGL((norm_rope<E, D, APPEND, POOL, HPG>), dim3(blocks), dim3(NT), 0, s, a);
   };
   // Several heads a group spare it most of its instructions, but leave fewer
   // work-groups: from 8 for every CU on. Measured (us, 1 / 2 / 4 / 8 heads): 16384
