@@ -79,12 +79,16 @@ struct RopeSide {
   const char *in;
   char *out;
   const float *w, *scales;  // norm weight; scales of an E4M3 pool (nullable)
-  uint8_t *bytes;           // scales of an MXFP4 pool
-  int64_t ss[3];            // their strides (page, head, place), bytes
   int64_t is[3], os[3];     // byte strides (batch, head, token); pool (page, head, place)
   int32_t heads, runs;      // runs: groups of lanes per token
   uint32_t runs_inv;
   uint32_t first;           // the operand's first work-group
+};
+
+// Scales of an MXFP4 pool
+struct MxScales {
+  uint8_t *bytes;
+  int64_t s[3];  // (page, head, place), bytes
 };
 
 struct RopeArgs {
@@ -97,8 +101,10 @@ struct RopeArgs {
   int32_t half, P, interleaved;    // pairs rotated, table rows
   int32_t B, ps, maxp, npages;
   float eps, inv_dim;
-  uint32_t keys, keys_step;        // append_mx: the keys' work-groups, their share of all as
-                                   // a fraction of 2^32, rounded up
+  // append_mx: keys' and values' scales; the keys' work-groups, and their share of all as a
+  // fraction of 2^32, rounded up
+  MxScales mx[2];
+  uint32_t keys, keys_step;
 };
 
 // sum over aligned groups of N (4, 8 or 16) lanes, in every lane: DPP moves
@@ -232,8 +238,8 @@ __device__ inline Slot slot_of(const RopeArgs &a, int lane, int tok, int end, bo
 // A row's codes and scales to its slot: 4 bytes of the lane's codes, the row's scales by
 // its first lane (byte: of the lane's block)
 template <int LPR>
-__device__ inline void store_mx(const RopeSide &x, const Slot &slot, int h, int l, uint32_t codes,
-                                uint32_t byte) {
+__device__ inline void store_mx(const RopeSide &x, const MxScales &mx, const Slot &slot, int h, int l,
+                                uint32_t codes, uint32_t byte) {
   byte <<= 8 * (l >> 2);
   if constexpr (LPR == 16) {
     byte |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)byte, 0x124, 0xf, 0xf, true);  // row_ror 4
@@ -243,7 +249,7 @@ __device__ inline void store_mx(const RopeSide &x, const Slot &slot, int h, int 
   }
   if (!slot.live || h >= x.heads) return;
   *(uint32_t *)(x.out + slot.page * x.os[0] + slot.place * x.os[2] + h * x.os[1] + 4 * l) = codes;
-  uint8_t *to = x.bytes + slot.page * x.ss[0] + slot.place * x.ss[2] + h * x.ss[1];
+  uint8_t *to = mx.bytes + slot.page * mx.s[0] + slot.place * mx.s[2] + h * mx.s[1];
   if (l == 0) {
     if constexpr (LPR == 16)
       *(uint32_t *)to = byte;
@@ -389,7 +395,7 @@ __device__ inline void keys_mx(const RopeArgs &a, uint32_t block) {
       }
     uint32_t byte;
     const uint32_t codes = mx8(z[0], z[1], &byte);
-    store_mx<LPR>(x, slot, run + k * x.runs, l, codes, byte);
+    store_mx<LPR>(x, a.mx[0], slot, run + k * x.runs, l, codes, byte);
   }
 }
 
@@ -528,7 +534,7 @@ __device__ inline void rows(const RopeArgs &a, uint32_t block) {
       slot.live = live;
       uint32_t byte;
       const uint32_t codes = mx8(ya, yb, &byte);
-      store_mx<LPR>(x, slot, h, l, codes, byte);
+      store_mx<LPR>(x, a.mx[1], slot, h, l, codes, byte);
       continue;
     }
     if (!live || h >= x.heads) continue;
@@ -677,12 +683,8 @@ hipError_t launch_rope(const RopeLaunch &L, hipStream_t s) {
   a.side[0] = {(const char *)L.q, (char *)L.qo, L.q_weight, nullptr};
   a.side[1] = {(const char *)L.k, (char *)L.ko, L.k_weight, L.k_scales};
   a.side[2] = {(const char *)L.v, (char *)L.vo, nullptr, L.v_scales};
-  a.side[1].bytes = L.k_bytes;
-  a.side[2].bytes = L.v_bytes;
-  for (int j = 0; j < 3; ++j) {
-    a.side[1].ss[j] = L.kss[j];
-    a.side[2].ss[j] = L.vss[j];
-  }
+  a.mx[0] = {L.k_bytes, {L.kss[0], L.kss[1], L.kss[2]}};
+  a.mx[1] = {L.v_bytes, {L.vss[0], L.vss[1], L.vss[2]}};
   const int64_t *const in[3] = {L.qs, L.ks, L.vs}, *const out[3] = {L.qos, L.kos, L.vos};
   for (int i = 0; i < 3; ++i) {
     a.side[i].heads = (int32_t)(i ? L.heads_kv : L.heads_q);

@@ -168,3 +168,25 @@ def test_every_row_has_its_own_mask():
     for window in (2, 17, 128, 200):
         o, lse = _run(cache, q, window=window)
         check_shaped(cache, q, o, lse, window=window)
+
+
+@pytest.mark.parametrize("form", ["cap", "slopes", "window of a page", "all"])
+@pytest.mark.parametrize("kind,D", [(BF16, 128), (FP8, 128), (FP8, 64), ("mx", 128), ("mx", 64)],
+                         ids=str)
+def test_tables_longer_than_a_wave(kind, D, form):
+    """Chunks over more pages than a wave holds entries of, read from the end back."""
+    cache = make_cache(kind, [(200, 2500), (40, 2100)], 2, D, 16, seed=D)
+    q = _q(cache, 8, BF16)
+    form = _form(FORMS[form], 8)
+    o, lse = _run(cache, q, **form)
+    check_shaped(cache, q, o, lse, **form)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_chains_of_single_tokens(D):
+    """Tiles enough that no keys are cut: each wave goes over more pages than it holds
+    table entries of."""
+    cache = make_cache("mx", [(1, 4500 + 37 * b) for b in range(8)], 64, D, 16, seed=D)
+    q = _q(cache, 64, BF16)
+    o, lse = _run(cache, q)
+    check_shaped(cache, q, o, lse)
