@@ -206,7 +206,7 @@ typedef struct neptune_append_desc {
   int64_t table_len;
   int64_t q_stride[2], k_stride[2], v_stride[2], qo_stride[2];
   int32_t dtype;    /* F16 or BF16: q, k, v and qo                             */
-  int32_t kv_dtype; /* the pools': dtype, or FP8_E4M3                          */
+  int32_t kv_dtype; /* the pools': dtype, FP8_E4M3, or MXFP4 (.._append_paged_mx) */
   int32_t interleaved;
   float eps;
 } neptune_append_desc;
@@ -222,7 +222,8 @@ typedef struct neptune_attn_paged_desc {
   int64_t seq_kv; /* the longest sequence; longer ones are cut to it           */
   int64_t q_stride[2], o_stride[2];
   int32_t dtype;    /* F16 or BF16: q and o                                    */
-  int32_t kv_dtype; /* the pools': dtype, or FP8_E4M3 (dtype BF16)             */
+  int32_t kv_dtype; /* the pools': dtype, FP8_E4M3 (dtype BF16), or MXFP4
+                     * (neptune_attn_paged_ext)                               */
   float scale_log2; /* 0 => log2(e)/sqrt(head_dim)                             */
   int32_t reserved;
 } neptune_attn_paged_desc;
@@ -398,14 +399,15 @@ NEPTUNE_API neptune_status neptune_kv_append_paged(
     const float *k_scales, const float *v_scales, void *qo, void *stream);
 
 /* neptune_kv_append_paged into MXFP4 pools (desc->kv_dtype MXFP4). No counterpart in
- * the reference. A block of 32 elements of a key (normed and rotated, in fp32) or value is
- * quantised as it is written: its scale's byte e is the exponent of the block's largest
+ * the reference. A block of 32 elements of a key (normed and rotated, not rounded before)
+ * or value is quantised as it is written: its scale's byte e is the exponent of the block's largest
  * magnitude, rounded to two significant bits, less 2 (so the largest is at most 6 scales,
  * or cut to that from less than 7), a code the nearest of x / 2^(e - 127), halves to the
  * even one. e is 252 at most; a block whose largest magnitude is below 2^-123 is held as
  * zeros (e = 0), one with an infinity or NaN as NaN (e = 255). k_scales and v_scales are
  * written where the codes are; they share no byte with each other, the pools, qo or an
- * input. The rest is neptune_kv_append_paged's. */
+ * input. Two rows sent to one slot may leave codes of one under scales of the other. The
+ * rest is neptune_kv_append_paged's. */
 NEPTUNE_API neptune_status neptune_kv_append_paged_mx(
     const neptune_append_desc *desc, const neptune_paged_kv_desc *pages,
     const neptune_mx_desc *mx, const void *k, const void *v, const void *q,
@@ -450,8 +452,9 @@ NEPTUNE_API neptune_status neptune_attn_paged(
 /* neptune_attn_paged over pools of any kind (desc->kv_dtype dtype, FP8_E4M3 or MXFP4; mx
  * and bytes for scales with MXFP4, dtype F16 or BF16), and with scores as in
  * neptune_score_desc (score NULL: plain). No counterpart in the reference. slopes
- * (nullable) [heads_q] fp32. Under the cap a score is off by some 2^-23 of itself, or of
- * the cap where it passes half of that. The rest is neptune_attn_paged's. */
+ * (nullable) [heads_q] fp32. Under the cap a score is off by some 2^-21 of itself, or of
+ * the cap where it passes a third of that. MXFP4 pools have pages, and tokens of a page,
+ * less than 2 GiB apart. The rest is neptune_attn_paged's. */
 NEPTUNE_API neptune_status neptune_attn_paged_ext(
     const neptune_attn_paged_desc *desc, const neptune_paged_kv_desc *pages,
     const neptune_mx_desc *mx, const neptune_score_desc *score, const void *q,

@@ -25,8 +25,8 @@ bool attn_paged_supported(const PagedAttnLaunch &L, const char **why) {
     return false;
   }
   if (L.pool == MXFP4)
+    // a page's offset is a product of 32-bit factors, and 32 bits hold a place's within it
     for (const int64_t *t : {L.kps, L.vps, L.kss, L.vss})
-      // (pages beyond the pool's are not looked at; factors below 2^31, as checked next)
       if (t[0] > INT32_MAX || t[2] > INT32_MAX / std::max<int64_t>(L.page_size, 1)) {
         *why = "MXFP4 pools' pages must lie less than 2 GiB apart, and their tokens within as much";
         return false;

@@ -5,8 +5,10 @@
 // (tests/data/flash_attention_htile.mlir:40-143) per query row:
 //   O_r = sum_{j <= t} 2^(s_rj - m) v_j / l,   s_rj = q_r . k_j scale log2(e),
 //   l = sum_j 2^(s_rj - m),   lse_r = (m + log2 l) ln 2,
-// with t the row's place in its sequence. 16-bit pools, or E4M3 codes with a
-// scale per page and KV head.
+// with t the row's place in its sequence. 16-bit pools, E4M3 codes with a scale per
+// page and KV head, or MXFP4: E2M1 codes, two to a byte, with an E8M0 byte for every
+// 32 elements of a place. A score may be capped, s -> c tanh(s / c) ahead of log2(e),
+// biased by slope_h (j - t), and dropped where j <= t - window (MOD; shape()).
 //
 // Tiles and items. The rows of a KV head's whole group, token by token, form a
 // sequence's run of rows (row r: token r / group, head r % group), cut into tiles
@@ -23,7 +25,9 @@
 // block-table entries, so no load waits on a load. E4M3 codes pass through
 // registers and are widened to bf16 (exact) on their way to LDS, once for the
 // work-group's four waves; the K scale meets the scores, the V scale P before
-// its rounding. Tiles of at most 32 rows take the narrow form (narrow_item).
+// its rounding. MXFP4 codes are widened under their scales there, exact in bf16, and the
+// products then are the 16-bit ones. Tiles of at most 32 rows take the narrow form
+// (narrow_item; MXFP4: narrow_mx).
 //
 // One rounding is not the plain form's: P goes to 16 bits for P.V, the operands that
 // the matrix instructions take (as a sum of two 16-bit numbers it would cost twice the
@@ -38,7 +42,10 @@
 // 32 heads of 128 over 8 unless said): 4 x 4096 causal 520-540, 1000 over 30000 460-478
 // (1050-1080 TFLOP/s; a bf16 GEMM of 8192^3 1344-1433), 2000 over 6000 E4M3 244
 // (bf16 222; head_dim 64 179 and 150; pages of 16 291), 32 x 1 over 8000 164-169 (6.2-6.4
-// TB/s), E4M3 96, 16 x 1-4 over 8000 69-71, 1 over 32768 29, 1 over 64 6.1-6.5.
+// TB/s), E4M3 96, MXFP4 54, 16 x 1-4 over 8000 69-71, 1 over 32768 29, MXFP4 18, 1 over 64
+// 6.1-6.5. MXFP4 chunks take 537 where bf16 takes 517 (4 x 4096): what widening costs
+// beside the matrix cores. Shaped scores, 1000 over 12000, 16 heads of 128 over 16, f16:
+// plain 114, biased 130, capped 145; over MXFP4 147 and 195.
 #pragma once
 
 #include <algorithm>
@@ -650,19 +657,22 @@ __device__ inline void narrow_item(const PagedArgs &a, const Item &it, int hk, i
 // tiles of 16 rows. Lane (c, g) of 16 by 4 holds S^T's keys 4 g + r of each run of 16 for
 // row c, and O^T's head_dim 16 nd + 4 g + r.
 //
-// A step is 64 keys, four runs of 16. Its codes come in registers, a step ahead. K: a lane takes 32 (head_dim 64: 16)
-// elements of one row of each run, and one scale, as the products' operands (which
-// element a k-slot holds is free, as long as Q's agree). V goes through LDS widened,
-// and is read transposed; keys 16 t + 4 g + r take k-slot 8 g + 4 t + r, where P has
-// them. A run lies within a page, so a load's base is scalar and its offsets are the
-// same all along. (Two and four steps of 32 keys ahead, in a loop unrolled as often, were
-// slower by the code's length: 1 over 400 8.2 and 8.6 us, this 7.8.)
+// A step is 32 keys, two runs of 16; its codes come in registers, a step ahead. K: a lane
+// takes 32 (head_dim 64: 16) elements of one row of each run, and one scale, as the
+// products' operands (which element a k-slot holds is free, as long as Q's agree). V goes
+// through LDS widened, and is read transposed; keys 16 t + 4 g + r take k-slot
+// 8 g + 4 t + r, where P has them. A run lies within a page, so a load's base is scalar and
+// its offsets are the same all along. Bound by the loads' latency where a wave has few
+// steps, by HBM where it has many (8 heads of 128, 4 queries each, in a replayed graph):
+// 1 by 4000 keys 11.3 us, 32 by 4000 32.0 us, 32 by 8000 53.9 us. Steps of 64 keys: 12.6,
+// 33.4, 54.3; three steps of 32 in flight, in a loop unrolled as often, were slower by the
+// code's length, 1 by 400 8.6 us against 8.2.
 template <class E, int HD, bool MOD, int NQ>
 __device__ inline void narrow_mx(const Item &it, int hk, int w, int lane, int kb0, int nv,
                                  const uint8_t *smem, f32x2 *mlbox) {
   const PagedArgs &a = arguments();
   typedef typename E::vec8 V8;
-  constexpr int STEP = BN, RUNS = STEP / 16;
+  constexpr int STEP = 32, RUNS = STEP / 16;
   constexpr int RB = HD * 2;        // bytes of V's rows in LDS
   constexpr int REGION = 16384;     // LDS per wave: V's tile, and its state at the end
   constexpr int ND = HD / 16;       // 16-wide head_dim tiles of O^T
@@ -691,7 +701,8 @@ __device__ inline void narrow_mx(const Item &it, int hk, int w, int lane, int kb
   const int lo = __builtin_amdgcn_readfirstlane(off + quotient(base_row, a.group, a.group_inv));
   const int last = off + quotient(base_row + rows - 1, a.group, a.group_inv);  // the last row's place
   // the wave's steps of the item's
-  const int s0 = kb0, s1 = min(kb0 + nv, last < 0 ? 0 : last / STEP + 1);
+  const int s0 = max(2 * kb0, MOD && a.window ? max(lo - a.window + 1, 0) / STEP : 0);
+  const int s1 = min(2 * (kb0 + nv), last < 0 ? 0 : last / STEP + 1);
   const int share = (max(s1 - s0, 0) + 3) >> 2;
   const int t0 = __builtin_amdgcn_readfirstlane(s0 + w * share);
   const int ns = __builtin_amdgcn_readfirstlane(max(min(t0 + share, s1) - t0, 0));
@@ -737,8 +748,8 @@ __device__ inline void narrow_mx(const Item &it, int hk, int w, int lane, int kb
   const uint32_t koff = c16 * (uint32_t)a.ktok + LB * g, voff = vrow * (uint32_t)a.vtok + LB * vq;
   const uint32_t ksoff = c16 * (uint32_t)a.kstok, vsoff = vrow * (uint32_t)a.vstok;
   const int kblk = HD == 128 ? g : g >> 1, vblk = HD == 128 ? vq : vq >> 1;
-  // runs of a step that share a page, whatever page: its place is looked up once
-  const int same = a.ps16 & 1 ? 1 : a.ps16 & 2 ? 2 : 4;
+  // pages of an even number of runs: a step lies within one, and its place is looked up once
+  const bool same = !(a.ps16 & 1);
   auto fetch = [&](int i) __attribute__((always_inline)) {
     const int run = RUNS * (t0 + i);
     int index, rest;
@@ -747,21 +758,18 @@ __device__ inline void narrow_mx(const Item &it, int hk, int w, int lane, int kb
 #pragma unroll
     for (int h = 0; h < RUNS; ++h) {
       const bool more = run + h <= last_run;  // (behind the end: the last run again)
-      if (h & (same - 1)) {
+      if (h && same) {
         at[0] += more ? 16 * (uint32_t)a.ktok : 0;
         at[1] += more ? 16 * (uint32_t)a.kstok : 0;
         at[2] += more ? 16 * (uint32_t)a.vtok : 0;
         at[3] += more ? 16 * (uint32_t)a.vstok : 0;
       } else {
-        if (h && more) {
-          rest += same;
-          if (rest >= a.ps16) {
-            rest -= a.ps16;
-            ++index;
-          }
+        if (h && more && ++rest == a.ps16) {
+          rest = 0;
+          ++index;
         }
         if (index - tab0 >= 64) {
-          load_tab(max(index - 3, 0));  // the step's first run may lie three pages before
+          load_tab(max(index - 1, 0));  // the step's first run may lie a page before
           settle(tabv);
         }
         int page = __builtin_amdgcn_readlane(tabv, index - tab0);
@@ -834,7 +842,7 @@ __device__ inline void narrow_mx(const Item &it, int hk, int w, int lane, int kb
     fetch(min(i + 1, ns - 1));
     __builtin_amdgcn_sched_barrier(0);
     bool masked = key0 + STEP - 1 > lo;
-    u32x4 pf[NQ][RUNS / 2];
+    u32x4 pf[NQ];
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
       const int lim = pos[q] - key0 - 4 * g;  // element (h, r) holds key 4 g + 16 h + r
@@ -870,7 +878,7 @@ __device__ inline void narrow_mx(const Item &it, int hk, int w, int lane, int kb
             const float p1 = fast_exp2(fmaf(s[q][h][2 * j + 1], sc, -m[q]));
             rs = h + j == 0 ? p0 : rs + p0;
             rs += p1;
-            pf[q][h >> 1][2 * (h & 1) + j] = E::pack2(p0, p1);  // 16 bits, for P.V alone
+            pf[q][2 * h + j] = E::pack2(p0, p1);  // 16 bits, for P.V alone
           }
       };
       // past the first step the max is formed only where a lane's sum passes 2^kSlack: up
@@ -908,17 +916,15 @@ __device__ inline void narrow_mx(const Item &it, int hk, int w, int lane, int kb
     int from = vget0;
     asm volatile("" : "+v"(from));
 #pragma unroll
-    for (int nd = 0; nd < ND; ++nd)
+    for (int nd = 0; nd < ND; ++nd) {
+      const uint8_t *p = mine + (from ^ (nd << 5));
+      const u32x2 x = __builtin_bit_cast(u32x2, lds_read_tr16(p));
+      const u32x2 y = __builtin_bit_cast(u32x2, lds_read_tr16(p + 16 * RB));
+      const u32x4 A = {x[0], x[1], y[0], y[1]};
 #pragma unroll
-      for (int c = 0; c < RUNS / 2; ++c) {
-        const uint8_t *p = mine + 32 * c * RB + (from ^ (nd << 5));
-        const u32x2 x = __builtin_bit_cast(u32x2, lds_read_tr16(p));
-        const u32x2 y = __builtin_bit_cast(u32x2, lds_read_tr16(p + 16 * RB));
-        const u32x4 A = {x[0], x[1], y[0], y[1]};
-#pragma unroll
-        for (int q = 0; q < NQ; ++q)
-          o[q][nd] = E::mfma16(as_vec8<V8>(A), as_vec8<V8>(pf[q][c]), o[q][nd]);
-      }
+      for (int q = 0; q < NQ; ++q)
+        o[q][nd] = E::mfma16(as_vec8<V8>(A), as_vec8<V8>(pf[q]), o[q][nd]);
+    }
     asm volatile("" ::: "memory");  // nor the next V's stores before these reads
   }
 
@@ -1069,8 +1075,9 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs args) {
     const int j = first + lane;
     tabv = j < a.maxp ? tab[j] : 0;
   };
-  // the wave's run of block t: its page's byte offset in each pool, and the
-  // tokens of it that exist less one (a run behind the end takes the last run)
+  // the wave's run of block t: its byte offset in each pool, the tokens of it that
+  // exist less one (a run behind the end takes the last run), its page, and its
+  // first place there
   auto run_at = [&](int t, int64_t *ko, int64_t *vo, int *most, int *in, int *at) {
     int run = (kb0 + block(t)) * (BN / 16) + w;
     const int key = min(run * 16, last_key & ~15);
@@ -1175,12 +1182,13 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs args) {
   const int vmput = (16 * w + mvrow) * ROWB + (((MB / 4 * mpart) ^ mxswz(mvrow)) << 4);
   const uint32_t kmoff = mrow * (uint32_t)a.ktok + mpart * MB, ksoff = mrow * (uint32_t)a.kstok;
   const uint32_t vmoff = mvrow * (uint32_t)a.vtok + mpart * MB, vsoff = mvrow * (uint32_t)a.vstok;
-  // the wave's run of a block: its page, first place in it and tokens that exist less
-  // one (narrow_mx on the rows behind). V's run of a block is K's, looked up before.
-  int mpage = 0, mplace = 0, mmost = 0;
+  // the wave's run of a block: its page and first place in it (of its rows behind the
+  // end: narrow_mx). V's run of a block is K's, looked up before.
+  int mpage = 0, mplace = 0;
   auto look_mx = [&](int t) {
     int64_t ko, vo;
-    run_at(t, &ko, &vo, &mmost, &mpage, &mplace);
+    int most;
+    run_at(t, &ko, &vo, &most, &mpage, &mplace);
   };
   auto load_k_mx = [&]() {
     kmx = *(const mx_t *)(mx_at(kp, mpage, a.kps0, mplace, a.ktok) + offset(kmoff));

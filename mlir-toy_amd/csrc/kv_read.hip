@@ -12,6 +12,9 @@
 // out once for 2 HPG rows.
 //
 // Bound: HBM, mostly the rows written; few rows by the chain of loads and the launch.
+// Measured in a replayed graph (8 heads of 128 to bf16 rows): 65536 tokens from MXFP4
+// 66 us (5.2 TB/s; a copy 5.0), 32768 from bf16 pages 41 (6.5), 16 tokens 3.6 (an empty
+// copy 2.0).
 #include <type_traits>
 
 #include "device_common.h"
@@ -151,11 +154,17 @@ hipError_t launch_hpg(ReadArgs a, hipStream_t s) {
     const uint32_t blocks = (uint32_t)(((int64_t)a.tokens * a.runs + GPB - 1) / GPB);
     hipLaunchKernelGGL((kv_read<O, D, POOL, HPG>), dim3(blocks), dim3(NT), 0, s, a);
   };
-  // Several heads a group where that leaves eight work-groups for every CU
-  if ((int64_t)a.tokens * a.heads >= 4 * 2048 * GPB)
-    go(std::integral_constant<int, 4>{});
-  else
-    go(std::integral_constant<int, 1>{});
+  // Codes: several heads a group where that leaves two work-groups for every CU. 8 heads of
+  // 128 from MXFP4, 65536, 16384, 4096 and 1024 tokens: 66, 16.5, 7.0 and 4.9 us, one head
+  // a group 100, 19.4, 7.1 and 4.3; E4M3 74, 17.9, 7.2 and 5.0, one head 100, 19.6, 6.9 and
+  // 4.3. 16-bit rows fill a group's loads alone: one head 22.0 and 7.3 for 16384 and 4096,
+  // four 23.0 and 8.5.
+  if constexpr (POOL != WIDE)
+    if (a.heads > 1 && (int64_t)a.tokens * a.heads >= 2048 * GPB) {
+      go(std::integral_constant<int, 4>{});
+      return hipGetLastError();
+    }
+  go(std::integral_constant<int, 1>{});
   return hipGetLastError();
 }
 

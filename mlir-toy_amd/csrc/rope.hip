@@ -6,7 +6,9 @@
 //   (y_i, y_j) -> (y_i c - y_j s, y_j c + y_i s) with c, s = cos, sin [p][pair]
 // for the R/2 pairs of the first R elements: (i, i + R/2), or (2i, 2i + 1)
 // interleaved. All of it in fp32, rounded once at the store; an E4M3 pool takes
-// the nearest code of the value's fp32 quotient by its page's scale.
+// the nearest code of the value's fp32 quotient by its page's scale. An MXFP4 pool takes
+// E2M1 codes and one power of two for every 32 elements, both formed here (mx8); its keys
+// are worked out in fp64, so that a code is the nearest to the exact key (keys_mx).
 //
 // D/8 lanes hold a row, eight elements each. Lane l of the rotated part holds
 // both sides of pairs 4l .. 4l+3, so a rotation never leaves the lane: two

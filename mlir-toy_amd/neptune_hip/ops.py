@@ -664,7 +664,8 @@ def kv_append_paged(
     page_size, D / 32] of bytes (uint8, or torch.float8_e8m0fnu), the scale 2^(e - 127)
     of 32 elements each (255: NaN), views of any page/head/position strides alike. The
     scales are outputs here: each block of 32 is quantised as it is written, by its
-    largest magnitude, to the nearest codes.
+    largest magnitude, to the nearest codes. (Two rows sent to one slot may leave codes of
+    one under scales of the other.)
 
     Keys are normalised (``k_weight``) and rotated (``cos``, ``sin``,
     ``interleaved``) at their positions on the way, as in ``qk_norm_rope``; with
@@ -833,8 +834,9 @@ def attention_paged(
     single token, none (``cu_seqlens`` and ``seq_lens`` as in
     ``kv_append_paged``, called before). k_pages / v_pages, block_table,
     k_scales / v_scales as in ``decode_paged`` (pools of q's dtype, or E4M3 with
-    bfloat16 q), or MXFP4 pools as ``kv_append_paged`` writes them; page sizes that
-    are multiples of 16; D 64 or 128.
+    bfloat16 q), or MXFP4 pools as ``kv_append_paged`` writes them (their values are
+    read in q's dtype: float16 has those past 65504 as infinite, and rounds those
+    below 2^-14 to steps of 2^-24); page sizes that are multiples of 16; D 64 or 128.
     ``max_seq_len`` (default max_pages * page_size) bounds the lengths. A row
     sees its sequence up to its own place; one with a negative place sees
     nothing: output 0, log-sum-exp -inf. Rows behind the last sequence are not

@@ -101,10 +101,11 @@ def shaped64(cache, q, *, softcap=None, slopes=None, window=None, scale=None):
 
     Bounds, with u half a step of q's type. A score x is a sum of D exact products in
     fp32 times the scale: off by (D + 2) 2^-24 of the sum of their magnitudes. The cap's
-    slope is at most 1; up to half the cap its polynomial is off by 1.1e-7 and eight
-    roundings of 2^-24, 5.9e-7 < 2^-20 of the score in all; beyond, exponent (2 |y| 2^-23
-    of it), v_exp_f32, sum, v_rcp_f32 and the last rounding make 2.2 2^-23 of the cap, of
-    which the score is at least 0.46: again less than 2^-20 of the score. A bias is off
+    slope is at most 1, and the score over the cap y has three roundings, 1.5 2^-23 of it.
+    Up to |y| = 3/8 the polynomial with its roundings is off by 1.5e-7, 1.3 2^-23 of the
+    score: less than 2^-20 in all. Beyond, a score is at least tanh(3/8) = 0.358 of the
+    cap, and exponent, v_exp_f32, sum, v_rcp_f32 and the last rounding make at most 2.3
+    2^-23 of the cap, 6.3 2^-23 of the score, y's 1.4: again less than 2^-20. A bias is off
     by three roundings of itself, the sum of both by one. So each score has a bound e,
     and with weights w the output is off by at most sum w e (|v| + |o|), the log-sum-exp
     by sum w e; p and V's products as in attend64: rounding to 16 bits (u), in f16 below
