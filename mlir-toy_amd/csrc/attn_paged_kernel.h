@@ -1021,7 +1021,7 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs args) {
   const int idx = quotient((int)blockIdx.x, args.Hk, args.Hk_inv);
   const int hk = (int)blockIdx.x - idx * args.Hk;
   Item it;
-  if (!find_item(args, plan, lane, idx, 0, &it)) return;
+  if (!find_item<MX>(args, plan, lane, idx, 0, &it)) return;
   const PagedArgs &a = MX ? arguments() : args;
   const int rows = it.n * a.group;
   const int off = it.len - it.n;  // place of the sequence's first new token
@@ -1775,6 +1775,7 @@ inline PagedArgs paged_args(const PagedAttnLaunch &L) {
   a.slots = (int32_t)room.slots;
   a.parts = (int32_t)room.parts;
   a.prows = (int32_t)part_rows(L);
+  a.longest = long_first(L);
   a.po = (float *)L.workspace;
   a.pml = a.po + (size_t)a.parts * L.heads_kv * a.prows * L.head_dim;
   a.scale2 = L.scale_log2;

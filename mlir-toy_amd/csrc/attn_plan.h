@@ -36,6 +36,7 @@ struct PagedArgs {
   int32_t items, slots, parts;    // per KV head: work-groups, those of one round, items of
                                   // cut tiles at most (0: no keys are cut)
   int32_t prows;                  // rows of a split item's states
+  int32_t longest;                // whether sequences of long items may come first
   float scale2;
   // MXFP4 pools: the scales' bytes, (page, head) and place strides
   const uint8_t *kmx, *vmx;
@@ -204,10 +205,24 @@ __device__ inline Plan make_plan(const PagedArgs &a, int lane) {
   }
 }
 
+// MXFP4 pools, chains of at least kLong blocks, 2 to kOrdered sequences: a work-group
+// alone on its CU there takes longer for a block than others do, and the order of the
+// sequences is worth 10% (4 of 231-585 new over up to 5000, in the orders they may come:
+// 129-152 us, so 134; capped 170-198, so 177; 16-bit pools 124 either way). Working it
+// out takes 0.5-1 us, too much for shorter launches (28.0 / 28.6).
+constexpr int kOrdered = 16, kLong = 24;
+bool long_first(const PagedAttnLaunch &L) {
+  return L.batch > 1 && L.batch <= kOrdered && L.seq_kv >= kLong * BN &&
+         L.tokens * (L.heads_q / L.heads_kv) > L.batch * NARROW;
+}
+
 // Item idx of one KV head, false if there is none. Sequences in order, a
 // sequence's tiles from the last (under the causal mask the longest), a tile's
 // splits together. take > 0 (it divides BM): instead the idx-th run of `take` rows
 // in a cut tile, split the run's first row in its tile.
+// LONG: sequences of long items come first (whatever the order, a tile's parts are the
+// same), so that the others' fill up beside them.
+template <bool LONG = false>
 __device__ inline bool find_item(const PagedArgs &a, const Plan &p, int lane, int idx, int take,
                                  Item *it) {
   int base = 0, parts = 0;
@@ -216,10 +231,22 @@ __device__ inline bool find_item(const PagedArgs &a, const Plan &p, int lane, in
     const int sp = a.parts ? splits_of(a, p, s) : 1;
     const int mparts = sp > 1 ? s.tiles * sp : 0;
     const int mine = take ? (sp > 1 ? (s.n * a.group + take - 1) / take : 0) : s.tiles * sp;
-    const int sum = wave_scan(mine), psum = a.parts ? wave_scan(mparts) : 0;
-    const uint64_t past = __ballot(base + sum > idx);
-    if (past) {
-      const int at = __builtin_ctzll(past);
+    const int psum = a.parts ? wave_scan(mparts) : 0;
+    int sum;  // with the sequences before
+    if (LONG && a.longest && p.chain_inv <= 1.0f / kLong) {
+      sum = mine;
+      const int length = (int)ceilf((float)s.blocks * __builtin_amdgcn_rcpf((float)sp));
+      for (int j = 0; j < a.B; ++j) {
+        const int other = __builtin_amdgcn_readlane(length, j);
+        const int x = __builtin_amdgcn_readlane(mine, j);
+        sum += other > length || (other == length && j < lane) ? x : 0;
+      }
+    } else {
+      sum = wave_scan(mine);
+    }
+    const uint64_t there = __ballot(base + sum > idx && base + sum - mine <= idx);
+    if (there) {
+      const int at = __builtin_ctzll(there);
       auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
       it->b = b0 + at;
       it->n = of(s.n);

@@ -190,3 +190,35 @@ def test_long_chains_of_single_tokens(D):
     q = _q(cache, 64, BF16)
     o, lse = _run(cache, q)
     check_shaped(cache, q, o, lse)
+
+
+@pytest.mark.parametrize("form", [{}, dict(softcap=5.0)], ids=str)
+@pytest.mark.parametrize("batch,heads", [
+    ([(211, 1203), (293, 2421), (0, 2600), (139, 2150), (316, 2616)], (64, 64)),
+    ([(40, 1600 + 61 * i) for i in range(16)], (64, 32))], ids=["5", "16"])
+def test_order_of_sequences_changes_nothing(batch, heads, form):
+    """Long chains over MXFP4 pools start with the sequences of long items: outputs are
+    those of the sequences in the order of their lengths, to the bit."""
+    Hq, Hk = heads
+    cache = make_cache("mx", batch, Hk, 128, 64, seed=5)
+    q = _q(cache, Hq, BF16)
+    (k, v, table, lens, cu), scales = cache.to_gpu()
+    ends = cu.tolist()
+    come = range(len(batch))
+    results = []
+    for order in (sorted(come, key=lambda b: -batch[b][1]), list(come), list(come)[::-1],
+                  sorted(come, key=lambda b: batch[b][1] % 7)):
+        rows = torch.cat([torch.arange(ends[b], ends[b + 1]) for b in order])
+        new = [0]
+        for b in order:
+            new.append(new[-1] + batch[b][0])
+        at = torch.tensor(order).cuda()
+        o, lse = ops.attention_paged(
+            q[rows].cuda(), k, v, table[at].contiguous(), lens[at].contiguous(),
+            torch.tensor(new, dtype=torch.int32).cuda(), return_lse=True,
+            max_seq_len=cache.max_len, **form, **scales)
+        back = rows.argsort()
+        results.append((o.cpu()[back], lse.cpu()[back]))
+    for o, lse in results[1:]:
+        assert torch.equal(o, results[0][0]) and torch.equal(lse, results[0][1])
+    assert torch.isfinite(results[0][0]).all() and torch.isfinite(results[0][1]).all()
