@@ -287,12 +287,15 @@ __device__ inline double group_sum64(double x) {
   return x;
 }
 
-// 1 / sqrt(x): v_rsq_f64 and two Newton steps
+// 1 / sqrt(x): v_rsq_f64 and two Newton steps, which an infinite mean square (a row with an
+// infinite element: the finite ones become 0) and 0 do without: they would multiply 0 by
+// infinity
 __device__ inline double inverse_root64(double x) {
-  double r = __builtin_amdgcn_rsq(x);
+  const double seed = __builtin_amdgcn_rsq(x);
+  double r = seed;
 #pragma unroll
   for (int i = 0; i < 2; ++i) r = fma(r * 0.5, fma(-x * r, r, 1.0), r);
-  return r;
+  return x > 0.0 && x < __builtin_inf() ? r : seed;
 }
 
 // Keys on their way into MXFP4 pools. Four bits leave borders far apart, and a key that
