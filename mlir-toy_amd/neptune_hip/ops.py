@@ -789,7 +789,8 @@ def _attn_paged_plan(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, k_s
             raise ValueError("attention_paged: softcap must be positive")
         if window is not None and window < 1:
             raise ValueError("attention_paged: window must be at least 1")
-        score = _abi.ScoreDesc(window or 0, softcap or 0.0, 0)
+        # (a window past 64 bits hides nothing: it must not wrap)
+        score = _abi.ScoreDesc(min(window or 0, 2**63 - 1), softcap or 0.0, 0)
         if softcap is not None and score.softcap == 0.0:  # none to the library
             raise ValueError("attention_paged: softcap must lie between 2^-60 and 2^60")
     if slopes is not None and (slopes[2] != torch.float32 or tuple(slopes[0]) != (Hq,) or

@@ -1,8 +1,6 @@
 """CPU tests of attention_paged's caps and windows that the library's own types do not
 hold: refused, or what they stand for."""
 
-import math
-
 import pytest
 import torch
 
@@ -36,3 +34,8 @@ def test_ordinary_scores(monkeypatch):
     assert s.softcap == 30.0 and s.window == 7
     assert _score(monkeypatch, softcap=1e-30).softcap == torch.tensor(1e-30).item()
     assert _score(monkeypatch, softcap=30.0).window == 0
+
+
+@pytest.mark.parametrize("window", [2**63 - 1, 2**63, 2**64, 2**64 + 5, 10**30])
+def test_a_window_past_64_bits_hides_nothing(monkeypatch, window):
+    assert _score(monkeypatch, window=window).window >= 512
