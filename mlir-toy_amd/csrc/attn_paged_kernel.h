@@ -50,6 +50,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "attn_tile.h"
@@ -1790,7 +1791,8 @@ inline PagedArgs paged_args(const PagedAttnLaunch &L) {
     a.cap2 = L.softcap * kLog2e;
     a.cap_inv = 1.0f / a.cap2;
     const float c[4] = {0x1.fffffep-1f, -0x1.5551cap-2f, 0x1.1011b4p-3f, -0x1.8b7eacp-5f};
-    // of the products themselves, where the powers of u stay ordinary numbers
+    // of the products themselves, where the powers of u stay ordinary numbers, and so do
+    // their products with the cap (an infinite factor would bring scores to -inf)
     const double u = (double)L.scale_log2 / a.cap2;
     double power = u * a.cap2;
     for (int i = 0; i < 4; ++i) {
@@ -1798,7 +1800,8 @@ inline PagedArgs paged_args(const PagedAttnLaunch &L) {
       a.capq[i] = (float)(c[i] * power);
       power *= u * u;
     }
-    a.cap_most = u >= 0x1p-16 && u <= 0x1p16 ? (float)(kCapPoly / u) : -1.0f;
+    a.cap_most = u >= 0x1p-16 && u <= 0x1p16 && std::isfinite(a.capq[3]) ? (float)(kCapPoly / u)
+                                                                         : -1.0f;
   }
   return a;
 }
