@@ -216,6 +216,14 @@ __device__ inline void shape(const PagedArgs &a, float slope2, float sc, float d
   }
 }
 
+// Whether some row's maximum is so large that p = 2^(s sc - m) needs its products rounded, as
+// the maximum's was. One fma takes the exact product: the largest p is then off 1 by half a
+// step of m in the exponent, and all of the row's with it. Below 2^24 that is 2^+-0.5; from
+// 2^31 on (f16: 2^28) it may be more than the type holds, and rows came out infinite or empty.
+// (Costs up to 1%: 6 x 32-130 head_dim-64 tokens over 1500 20.0 / 20.1 us, MXFP4 capped chunks
+// 176.6 / 178.4, E4M3 chunks 167.6 / 169.7; 4 x 4096 nothing.)
+__device__ inline bool huge(float m) { return __any(fabsf(m) >= 0x1p24f); }
+
 // The scale that V's scales are taken relative to where they meet P: that of the
 // first page looked at, in lane 0 of vscv. P is rounded to 16 bits with the ratio
 // in it, so its large values, at most 1, stay next to 1 and below, where bf16's
@@ -883,10 +891,20 @@ __device__ inline void narrow_mx(const Item &it, int hk, int w, int lane, int kb
             pf[q][2 * h + j] = E::pack2(p0, p1);  // 16 bits, for P.V alone
           }
       };
+      auto products = [&]() {  // rounded, where huge() asks for it
+        if (!MOD && __builtin_expect(huge(m[q]), 0)) {
+#pragma unroll
+          for (int h = 0; h < RUNS; ++h)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[q][h][r] *= sc;
+          sc = 1.0f;
+        }
+      };
       // past the first step the max is formed only where a lane's sum passes 2^kSlack: up
       // to that m keeps
       bool full = i == 0;
       if (!full) {
+        products();
         expo();
         full = __any(!(rs <= kSumCap));
       }
@@ -904,6 +922,7 @@ __device__ inline void narrow_mx(const Item &it, int hk, int w, int lane, int kb
 #pragma unroll
           for (int r = 0; r < 4; ++r) o[q][nd][r] *= alpha;
         m[q] = m_new;
+        products();
         expo();
       }
       lsum[q] += rs;
@@ -1349,6 +1368,7 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs args) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[nb][r] = 0.0f;
   float m = kNegFltMax, lsum = 0.0f;
+  bool large = false;
   const f32x16 zero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 
   // The A operand of MFMA i = 2 st + kb of S^T = K.Q^T (32 keys x 16 head_dim)
@@ -1412,7 +1432,7 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs args) {
       // Across pages, or where the exponent would not hold V's scale or K's is not
       // positive and finite, each run's are multiplied in: K's here, before the mask
       // (such a scale must not meet -inf), V's with P.
-      float vs[4] = {1.0f, 1.0f, 1.0f, 1.0f}, lv = 0.0f, iv = 1.0f;
+      float vs[4] = {1.0f, 1.0f, 1.0f, 1.0f}, v0 = 1.0f, lv = 0.0f, iv = 1.0f;
       bool apart = false;
       if constexpr (FP8) {
         int index, rest;
@@ -1428,7 +1448,8 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs args) {
               float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i - sc0));
         };
         const int runs = last_key / 16 - (key0 >> 4);  // runs behind the end take the last one's
-        const float k0 = sc * scale_at(kscv, index), v0 = unit_inv * scale_at(vscv, index);
+        const float k0 = sc * scale_at(kscv, index);
+        v0 = unit_inv * scale_at(vscv, index);
         apart = (rest + 3 >= a.ps16 && runs > 0) || !(v0 >= 0x1p-64f && v0 <= 0x1p64f) ||
                 !(k0 > 0.0f && k0 <= 3.4e38f);
         if (apart) {
@@ -1470,7 +1491,10 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs args) {
           done = !__any(!(big <= a.cap_most));
         }
         if (done) {
-          const float b0 = fmaf(slope2, (float)-lim, -m);
+          // (NaN where huge(), so that the block is done the other way: a comparison and a
+          // branch here cost the biased chunk 5%)
+          const float nm = fmaf(m * 0x1p104f, 0.0f, -m);
+          const float b0 = fmaf(slope2, (float)-lim, nm);
           auto expo_of = [&](auto score) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
@@ -1493,11 +1517,11 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs args) {
           if (a.cap2 != 0.0f && a.slopes)
             expo_of([&](float x, float c) { return capped(x, fmaf(slope2, c, b0)); });
           else if (a.cap2 != 0.0f)
-            expo_of([&](float x, float) { return capped(x, -m); });
+            expo_of([&](float x, float) { return capped(x, nm); });
           else if (a.slopes)
             expo_of([&](float x, float c) { return fmaf(x, sc, fmaf(slope2, c, b0)); });
           else
-            expo_of([&](float x, float) { return fmaf(x, sc, -m); });
+            expo_of([&](float x, float) { return fmaf(x, sc, nm); });
           done = !__any(!(rs <= kSumCap));
         }
       }
@@ -1568,16 +1592,37 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs args) {
 #pragma unroll
               for (int r = 0; r < 16; ++r) o[nb][r] *= alpha;
             m = m_new;
+            if constexpr (!MOD || FP8) large = huge(m);
+          }
+        };
+        auto products = [&]() {  // rounded, where huge() asks for it
+          if ((!MOD || FP8) && __builtin_expect(large, 0)) {
+            if constexpr (!MOD) {
+#pragma unroll
+              for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[kb][r] *= sc;
+              sc = 1.0f;
+            }
+            if (FP8 && !apart) {  // such an exponent has no room for V's scale
+              apart = true;
+#pragma unroll
+              for (int c = 0; c < 4; ++c) vs[c] = v0;
+              lv = 0.0f;
+              iv = 1.0f;
+            }
           }
         };
         if constexpr (HD == 64) {
           raise_max(0.0f);
+          products();
           expo();
         } else {
           // the block max is only formed when it can matter: past the first block,
           // a lane sum of at most 2^kSlack bounds every p by it, and m keeps
           bool full = jb == 0;
           if (!full) {
+            products();
             expo();
             full = __any(!(rs <= kSumCap));
           }
@@ -1585,6 +1630,7 @@ __global__ __launch_bounds__(NT, 2) void attn_paged(PagedArgs args) {
             // (BACK: the first block may show a row few keys; a maximum left below the
             // next ones' would bring every block here)
             raise_max(BACK ? 0.0f : kSlack);
+            products();
             expo();
           }
         }
