@@ -15,10 +15,12 @@ __device__ inline uint32_t divide(uint32_t x, uint32_t d, uint32_t inv) {
 }
 
 // The search's first load, for the caller to issue ahead of others: the end of the
-// lane's chunk of ceil(B / 64) sequences.
+// lane's chunk of ceil(B / 64) sequences (cu nullable: there is none to look for).
 __device__ inline int chunk_end(const int32_t *cu, int B, int lane) {
   const int chunk = (B + 63) >> 6;
-  return lane * chunk < B ? cu[min((lane + 1) * chunk, B)] : 0x7fffffff;
+  int end = 0x7fffffff;
+  if (cu && lane * chunk < B) end = cu[min((lane + 1) * chunk, B)];
+  return end;
 }
 
 // The sequence of row tok, the same for LPR lanes together: as many ends of sequences

@@ -313,8 +313,7 @@ __device__ inline void keys_mx(const RopeArgs &a, uint32_t block) {
   const uint32_t gid = block * (NT / LPR) + threadIdx.x / LPR;
   const int at = (int)divide(gid, x.runs, x.runs_inv), run = (int)gid - at * x.runs;
   const int tok = min(at, a.tokens - 1);
-  int end = 0x7fffffff;
-  if (a.cu) end = chunk_end(a.cu, a.B, lane);
+  const int end = chunk_end(a.cu, a.B, lane);
   // the lane's two runs of four: their partners, and their pairs' places in the tables
   const bool beside = !a.interleaved && a.half > 0;
   int poff[2], pair[2];
@@ -424,8 +423,7 @@ __device__ inline void rows(const RopeArgs &a, uint32_t block) {
   // tokens, one head a group.)
   const int t0 = APPEND ? 0 : (int)divide(tok, a.S, a.S_inv), t1 = APPEND ? tok : tok - t0 * a.S;
   int t, page = -1, place = 0, end = 0x7fffffff;
-  if constexpr (APPEND)
-    if (a.cu) end = chunk_end(a.cu, a.B, lane);
+  if constexpr (APPEND) end = chunk_end(a.cu, a.B, lane);
 
   // this lane's two runs of four elements, the rotated ones' pairs 4l ..; flat: all
   // lanes' runs are neighbours
