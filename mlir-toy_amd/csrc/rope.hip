@@ -299,9 +299,9 @@ __device__ inline double inverse_root64(double x) {
 }
 
 // Keys on their way into MXFP4 pools. Four bits leave borders far apart, and a key that
-// fp32's norm and rotation leave on the wrong side of one is off by a whole step: one in
-// 10^6 elements (0.00027 of 15000 tokens' norm). In fp64, which this GPU's vector unit
-// runs as fast, a key's code is the nearest one. A lane has eight neighbours, so that four
+// fp32's norm and rotation leave on the wrong side of one is off by a whole step: 18 of 92
+// million elements of N(0, 1) keys (0.00017 of their norm; fp32 emulated on a CPU). In
+// fp64, which this GPU's vector unit runs as fast, a key's code is the nearest one. A lane has eight neighbours, so that four
 // hold a block, and for half-split pairs their partners, loaded beside them.
 constexpr int keys_hpg(int hpg) { return hpg < 2 ? hpg : 2; }  // (fp64's factors take registers)
 template <class E, int D, int HPG>
