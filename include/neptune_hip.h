@@ -400,11 +400,12 @@ NEPTUNE_API neptune_status neptune_kv_append_paged(
 
 /* neptune_kv_append_paged into MXFP4 pools (desc->kv_dtype MXFP4). No counterpart in
  * the reference. A block of 32 elements of a key (normed and rotated, not rounded before)
- * or value is quantised as it is written: its scale's byte e is the exponent of the block's largest
- * magnitude, rounded to two significant bits, less 2 (so the largest is at most 6 scales,
- * or cut to that from less than 7), a code the nearest of x / 2^(e - 127), halves to the
- * even one. e is 252 at most; a block whose largest magnitude is below 2^-123 is held as
- * zeros (e = 0), one with an infinity or NaN as NaN (e = 255). k_scales and v_scales are
+ * or value is quantised as it is written: its scale's byte e is the exponent of the block's
+ * largest magnitude, rounded to two significant bits, less 2 (so the largest is at most 6
+ * scales, or cut to that from less than 7), a code the nearest of x / 2^(e - 127), halves
+ * to the even one. e is 252 at most, so magnitudes of 7 2^125 and more are cut to 6 2^125
+ * from less than 8; a block whose largest magnitude is below 2^-123 is held as zeros
+ * (e = 0), one with an infinity or NaN as NaN (e = 255). k_scales and v_scales are
  * written where the codes are; they share no byte with each other, the pools, qo or an
  * input. Two rows sent to one slot may leave codes of one under scales of the other. The
  * rest is neptune_kv_append_paged's. */

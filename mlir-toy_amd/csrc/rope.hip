@@ -187,7 +187,9 @@ __device__ inline uint32_t quad_max(uint32_t x) {
 // significant bits that a code has: below 7 / 4 of its power of two the largest is 6
 // scales and less, or passes 6 by less than a sixth and becomes 6; from 7 / 4 on, the
 // next scale, it is 3.5 and more. (Without that rounding magnitudes up to 8 scales would
-// become 6.) A block below 2^-123 is held as zeros, one with an infinity or NaN as NaN.
+// become 6.) The byte is 252 at most, since 6 of the next scale pass fp32's range: there
+// magnitudes up to 8 scales do become 6. A block below 2^-123 is held as zeros, one with an
+// infinity or NaN as NaN.
 __device__ inline uint32_t mx8(f32x4 a, f32x4 b, uint32_t *byte) {
   uint32_t top = 0;
 #pragma unroll
@@ -301,8 +303,9 @@ __device__ inline double inverse_root64(double x) {
 // Keys on their way into MXFP4 pools. Four bits leave borders far apart, and a key that
 // fp32's norm and rotation leave on the wrong side of one is off by a whole step: 18 of 92
 // million elements of N(0, 1) keys (0.00017 of their norm; fp32 emulated on a CPU). In
-// fp64, which this GPU's vector unit runs as fast, a key's code is the nearest one. A lane has eight neighbours, so that four
-// hold a block, and for half-split pairs their partners, loaded beside them.
+// fp64, which this GPU's vector unit runs as fast, a key's code is the nearest one. A lane
+// has eight neighbours, so that four hold a block, and for half-split pairs their partners,
+// loaded beside them.
 constexpr int keys_hpg(int hpg) { return hpg < 2 ? hpg : 2; }  // (fp64's factors take registers)
 template <class E, int D, int HPG>
 __device__ inline void keys_mx(const RopeArgs &a, uint32_t block) {
