@@ -45,8 +45,9 @@
 // TB/s), E4M3 96, MXFP4 54, 16 x 1-4 over 8000 69-71, 1 over 32768 29, MXFP4 18, 1 over 64
 // 6.1-6.5. MXFP4 chunks take 537 where bf16 takes 517 (4 x 4096): what widening costs
 // beside the matrix cores. Shaped scores, 1000 over 12000, 16 heads of 128 over 16, f16:
-// plain 115, biased 128, capped 149; four ragged chunks over up to 5000, 32 heads over 8:
-// plain 124, MXFP4 133, capped MXFP4 176.
+// plain 116, biased 128, capped 150, windowed to 4096 64 (E4M3 124, 149, 175, 77; f16 of
+// head_dim 64 84, 109, 134, 58); four ragged chunks over up to 5000, 32 heads over 8:
+// plain 125, MXFP4 133, capped MXFP4 178.
 #pragma once
 
 #include <algorithm>

@@ -207,9 +207,10 @@ __device__ inline Plan make_plan(const PagedArgs &a, int lane) {
 
 // MXFP4 pools, chains of at least kLong blocks, 2 to kOrdered sequences: a work-group
 // alone on its CU there takes longer for a block than others do, and the order of the
-// sequences is worth 10% (4 of 231-585 new over up to 5000, in the orders they may come:
-// 129-152 us, so 134; capped 170-198, so 177; 16-bit pools 124 either way). Working it
-// out takes 0.5-1 us, too much for shorter launches (28.0 / 28.6).
+// sequences is worth 10% and more (4 of 231-585 new over up to 5000, in the orders they may
+// come: 129-152 us, so 134; capped 170-198, so 177; 8 of 100-400 over up to 5000 137-156,
+// so 136-143; 16 of 50-250 141-185, so 143; capped 176-245, so 179; 16-bit pools 124 either
+// way). Working it out takes 0.5-1 us, too much for shorter launches (28.0 / 28.6).
 constexpr int kOrdered = 16, kLong = 24;
 bool long_first(const PagedAttnLaunch &L) {
   return L.batch > 1 && L.batch <= kOrdered && L.seq_kv >= kLong * BN &&
